@@ -41,6 +41,8 @@ MODULES: Dict[str, List[str]] = {
                "attention_masked_mma.cu", "experts.cu", "experts_tc.cu", "norm_act.cu", "short_conv.cu", "attention_pooled.cu",
                "attention_mixed_heads.cu", "attention_mixed_heads_mma.cu", "gated_delta.cu", "gated_delta_mma.cu",
                "gated_linear_attention.cu", "gated_linear_attention_mma.cu", "ssd.cu", "ssd_mma.cu"],
+    # pages in 4 bits (append, read, attention) and rows of tokens in 8 bits
+    "packed": ["cache4.cu", "quantize8.cu"],
     # the entry point that allocates nothing (leone_static.h); it compiles attention_tiled.cu in
     "static": ["attention_decode_static.cu"],
     # the host side of the runtime (pages, block tables, step metadata, the scheduler's decisions,
@@ -52,7 +54,7 @@ MODULES: Dict[str, List[str]] = {
 HOST_ONLY = {"host", "call"}
 OPTIONAL = {"call"}                # what the package does without where it cannot be built
 HEADERS = ["common.cuh", "mma_tile.cuh", "tc_common.cuh", "gemm_parts.cuh", "leone_static.h", "attention_tiled.cu", "random_draw.h",
-           "pair_sums.h", "gla_parts.cuh", "ssd_parts.cuh", "experts_tc.h", "gemm_f32.h"]
+           "pair_sums.h", "gla_parts.cuh", "ssd_parts.cuh", "experts_tc.h", "gemm_f32.h", "cache4.cuh"]
 
 # -fno-gnu-unique: statics inside inline functions and templates (the once-per-kernel set-up
 # flags, the launch mode switch) must belong to one library image each; with GNU unique

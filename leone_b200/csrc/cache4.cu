@@ -1,0 +1,383 @@
+// A step's keys and values into pages in 4 bits (cache4.cuh), what such pages hold, and attention over them at any size.
+#include "cache4.cuh"
+
+namespace leone {
+namespace cache4 {
+
+// Where token t's row of a cached head lies: its unit and its place there; false (and a status) where the step's metadata names no
+// page.
+struct Place {
+  long long page;
+  int slot;
+};
+__device__ __forceinline__ bool find_place(Place& place, int t, int pos, const int* seq_of_token, int n_seqs, const int* block_table,
+                                           int table_width, int num_pages, int page_tokens, int* status, bool report) {
+  const int s = seq_of_token[t];
+  if (s < 0 || s >= n_seqs) {
+    if (report) set_status(status, kBadSequence, t, s);
+    return false;
+  }
+  const int blk = pos / page_tokens;
+  const int page = (pos >= 0 && blk < table_width) ? block_table[(size_t)s * table_width + blk] : -1;
+  if (page < 0 || page >= num_pages) {
+    if (report) set_status(status, kBadPage, t, page, pos);
+    return false;
+  }
+  place.page = page;
+  place.slot = pos % page_tokens;
+  return true;
+}
+
+// The largest float not above v, then the largest bfloat16 not above that: rounding down twice rounds down once.
+__device__ __forceinline__ __nv_bfloat16 bf16_down(double v) { return __float2bfloat16_rd(__double2float_rd(v)); }
+__device__ __forceinline__ __nv_bfloat16 bf16_up(double v) { return __float2bfloat16_ru(__double2float_ru(v)); }
+
+// RMSNorm and rotation of q and k per head as in qk_norm_rope_write (elementwise.cu), queries back into qkv, keys and values into
+// the pools in 4 bits.  One warp per (token, head).  Everything in 64 bits: the code of a key next to the border of two codes then
+// does not depend on the order in which the head's squares are added.
+template <typename T, typename TW>
+__global__ void append_kernel(T* __restrict__ qkv, int n_tokens, int n_q, int n_kv, int d, const TW* __restrict__ q_w,
+                              const TW* __restrict__ k_w, float eps, const float2* __restrict__ rope, int rotary_dim,
+                              int max_positions, const int* __restrict__ positions, const int* __restrict__ seq_of_token,
+                              const int* __restrict__ block_table, int table_width, int n_seqs, uint8_t* __restrict__ k_pool,
+                              uint8_t* __restrict__ v_pool, int num_pages, int page_tokens, int adjacent, int* status) {
+  extern __shared__ double row_s[];
+  pdl_trigger();
+  pdl_wait();
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = n_q + 2 * n_kv;
+  const long long item = (long long)blockIdx.x * warps + warp;
+  if (item >= (long long)n_tokens * heads) return;
+  const int t = (int)(item / heads), h = (int)(item - (long long)t * heads);
+  double* x = row_s + (size_t)warp * d;
+  T* row = qkv + ((size_t)t * heads + h) * d;
+  const bool is_q = h < n_q, is_k = !is_q && h < n_q + n_kv;
+  const int pos = positions[t];
+  if ((is_q || is_k) && rope != nullptr && (pos < 0 || pos >= max_positions)) {
+    if (lane == 0) set_status(status, kBadPosition, t, pos);
+    return;
+  }
+  Place place;
+  if (!is_q && !find_place(place, t, pos, seq_of_token, n_seqs, block_table, table_width, num_pages, page_tokens, status, lane == 0))
+    return;
+
+  const TW* w = is_q ? q_w : (is_k ? k_w : nullptr);
+  double ss = 0.0;
+  for (int c = lane; c < d; c += 32) {
+    const double v = (double)to_float<T>(row[c]);
+    x[c] = v;
+    ss = fma(v, v, ss);
+  }
+  if (w != nullptr) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const double factor = rsqrt(ss / d + (double)eps);
+    for (int c = lane; c < d; c += 32) x[c] *= (double)to_float<TW>(w[c]) * factor;
+  }
+  __syncwarp();
+  if ((is_q || is_k) && rope != nullptr) {
+    const int half = rotary_dim >> 1;
+    for (int i = lane; i < half; i += 32) {
+      const float2 cs = rope[(size_t)pos * half + i];
+      const int at = adjacent ? 2 * i : i, bt = adjacent ? 2 * i + 1 : i + half;
+      const double a = x[at], b = x[bt];
+      x[at] = a * cs.x - b * cs.y;
+      x[bt] = a * cs.y + b * cs.x;
+    }
+    __syncwarp();
+  }
+  if (is_q) {
+    for (int c = lane; c < d; c += 32) row[c] = from_float<T>((float)x[c]);
+    return;
+  }
+  const int G = groups(d), size = d / G;
+  uint8_t* unit = (is_k ? k_pool : v_pool) +
+                  unit_at(place.page, n_kv, is_k ? h - n_q : h - n_q - n_kv, page_tokens, place.slot / kUnit * kUnit, d);
+  const int slot = place.slot % kUnit;
+  for (int g = 0; g < G; ++g) {
+    double lo = INFINITY, hi = -INFINITY;
+    bool odd = false;                                       // a NaN or an infinity
+    for (int c = lane; c < size; c += 32) {
+      const double v = x[g * size + c];
+      odd |= !isfinite(v);
+      lo = fmin(lo, v);
+      hi = fmax(hi, v);
+    }
+    odd = __any_sync(0xffffffffu, odd);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      lo = fmin(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmax(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    __nv_bfloat16 z16 = bf16_down(lo);
+    const double z = __bfloat162float(z16);
+    __nv_bfloat16 s16 = bf16_up((hi - z) / 15.0);
+    if (__bfloat162float(s16) < 1.17549435e-38f) s16 = __float2bfloat16_rn(0.f);
+    odd |= !isfinite(z) || !isfinite(__bfloat162float(s16));
+    if (odd) z16 = s16 = __ushort_as_bfloat16(0x7fc0);
+    const double s = __bfloat162float(s16);
+    for (int i = lane; i < size / 8; i += 32) {
+      uint32_t word = 0;
+      if (!odd && s > 0.0) {
+        for (int e = 0; e < 8; ++e) {
+          const double q = rint((x[g * size + 8 * i + e] - z) / s);
+          word |= (uint32_t)fmin(fmax(q, 0.0), 15.0) << (4 * (e >> 1) + 16 * (e & 1));
+        }
+      }
+      const int word_at = g * (size / 8) + i;
+      *reinterpret_cast<uint32_t*>(unit + (is_k ? key_word_at(slot, word_at, d) : value_word_at(slot, word_at, d))) = word;
+    }
+    if (lane == 0)
+      *reinterpret_cast<uint32_t*>(unit + scale_at(slot, g, d)) =
+          (uint32_t)__bfloat16_as_ushort(s16) | (uint32_t)__bfloat16_as_ushort(z16) << 16;
+  }
+}
+
+// What the pages hold for the step's tokens: rows [n_tokens][n_kv * d] of keys and of values.  One warp per (token, cached head).
+template <typename T>
+__global__ void read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, int n_tokens, int n_kv, int d,
+                            const int* __restrict__ positions, const int* __restrict__ seq_of_token,
+                            const int* __restrict__ block_table, int table_width, int n_seqs, const uint8_t* __restrict__ k_pool,
+                            const uint8_t* __restrict__ v_pool, int num_pages, int page_tokens, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  if (item >= (long long)n_tokens * n_kv) return;
+  const int t = (int)(item / n_kv), h = (int)(item - (long long)t * n_kv);
+  Place place;
+  if (!find_place(place, t, positions[t], seq_of_token, n_seqs, block_table, table_width, num_pages, page_tokens, status, lane == 0))
+    return;
+  const long long unit = unit_at(place.page, n_kv, h, page_tokens, place.slot / kUnit * kUnit, d);
+  const int slot = place.slot % kUnit, size = d / groups(d);
+  for (int w = lane; w < d / 8; w += 32) {
+    const uint32_t kw = *reinterpret_cast<const uint32_t*>(k_pool + unit + key_word_at(slot, w, d));
+    const uint32_t vw = *reinterpret_cast<const uint32_t*>(v_pool + unit + value_word_at(slot, w, d));
+    const int at = scale_at(slot, 8 * w / size, d);
+    const uint32_t ks = *reinterpret_cast<const uint32_t*>(k_pool + unit + at);
+    const uint32_t vs = *reinterpret_cast<const uint32_t*>(v_pool + unit + at);
+    T* k = k_out + item * d + 8 * w;
+    T* v = v_out + item * d + 8 * w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      k[e] = from_float<T>(fmaf(scale_of(ks), (float)code_of(kw, e), offset_of(ks)));
+      v[e] = from_float<T>(fmaf(scale_of(vs), (float)code_of(vw, e), offset_of(vs)));
+    }
+  }
+}
+
+// Causal grouped-query attention over pages in 4 bits, any sizes, any cut: the formulas of attention_generic.cu.  One block per
+// (token, cached head, up to 8 of its query heads) walks the keys in tiles of 32: a tile's keys, then its values, are brought into
+// shared memory in fp32; warp w has the scores of heads w and w + 4, a lane a key; thread c sums the outputs' columns c, c + 128, ..
+constexpr int kAnyThreads = 128;
+constexpr int kAnyKeys = 32;
+constexpr int kAnyHeads = 8;
+__host__ __device__ constexpr int any_row(int d) { return d + 1; }      // floats between the tile's rows: lanes on different banks
+
+template <typename T>
+__global__ void __launch_bounds__(kAnyThreads)
+attention_any_kernel(const T* __restrict__ qkv, int row_stride, T* __restrict__ out, int out_stride,
+                     const uint8_t* __restrict__ k_pool, const uint8_t* __restrict__ v_pool, const int* __restrict__ block_table,
+                     int table_width, const int* __restrict__ seq_of_token, const int* __restrict__ positions, int n_q, int n_kv,
+                     int d, float scale, int window, int page_tokens, int num_pages, int n_seqs, int* status) {
+  extern __shared__ float smem_f[];
+  float* tile = smem_f;                                    // [32][any_row(d)]
+  float* q_s = tile + kAnyKeys * any_row(d);               // [8][d]
+  float* p_s = q_s + kAnyHeads * d;                        // [8][32]
+  float* alpha_s = p_s + kAnyHeads * kAnyKeys;             // [8]
+  float* l_s = alpha_s + kAnyHeads;                        // [8]
+  __shared__ long long unit_s[kAnyKeys];
+  pdl_trigger();
+  pdl_wait();
+  const int t = blockIdx.x, g = n_q / n_kv, parts = (g + kAnyHeads - 1) / kAnyHeads;
+  const int kvh = blockIdx.y / parts, part = blockIdx.y - kvh * parts;
+  const int head0 = kvh * g + part * kAnyHeads, heads = min(kAnyHeads, g - part * kAnyHeads);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int pos = positions[t], s = seq_of_token[t];
+  T* dst = out + (size_t)t * out_stride + (size_t)head0 * d;
+  if (s < 0 || s >= n_seqs || pos < 0) {
+    if (tid == 0) set_status(status, s < 0 || s >= n_seqs ? kBadSequence : kBadPosition, t, s < 0 || s >= n_seqs ? s : pos);
+    for (int c = tid; c < heads * d; c += kAnyThreads) dst[c] = from_float<T>(0.f);
+    return;
+  }
+  const T* q = qkv + (size_t)t * row_stride + (size_t)head0 * d;
+  for (int c = tid; c < heads * d; c += kAnyThreads) q_s[c] = to_float<T>(q[c]);
+  const int G = groups(d), size = d / G, words = d / 8;
+  const int lo = window > 0 ? max(0, pos - window + 1) : 0;
+  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+  float acc[kAnyHeads][kMaxDim / kAnyThreads];
+#pragma unroll
+  for (int h = 0; h < kAnyHeads; ++h)
+#pragma unroll
+    for (int i = 0; i < kMaxDim / kAnyThreads; ++i) acc[h][i] = 0.f;
+  auto fetch = [&](const uint8_t* pool, bool keys, int j0) {
+    for (int idx = tid; idx < kAnyKeys * words; idx += kAnyThreads) {
+      const int r = idx / words, w = idx - r * words;
+      float* to = tile + r * any_row(d) + 8 * w;
+      if (unit_s[r] < 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) to[e] = 0.f;
+        continue;
+      }
+      const int slot = (j0 + r) % page_tokens % kUnit;
+      const uint8_t* unit = pool + unit_s[r];
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(unit + (keys ? key_word_at(slot, w, d) : value_word_at(slot, w, d)));
+      const uint32_t sz = *reinterpret_cast<const uint32_t*>(unit + scale_at(slot, 8 * w / size, d));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) to[e] = fmaf(scale_of(sz), (float)code_of(word, e), offset_of(sz));
+    }
+  };
+  for (int j0 = lo; j0 <= pos; j0 += kAnyKeys) {
+    __syncthreads();                                       // the tile before is done with
+    if (tid < kAnyKeys) {
+      const int j = j0 + tid;
+      long long unit = -1;
+      if (j <= pos) {
+        const int blk = j / page_tokens;
+        const int page = blk < table_width ? block_table[(size_t)s * table_width + blk] : -1;
+        if (page < 0 || page >= num_pages) set_status(status, kBadPage, t, page, j);
+        else unit = unit_at(page, n_kv, kvh, page_tokens, j % page_tokens / kUnit * kUnit, d);
+      }
+      unit_s[tid] = unit;
+    }
+    __syncthreads();
+    fetch(k_pool, true, j0);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int h = warp + 4 * u;
+      if (h >= heads) break;
+      const float* k = tile + lane * any_row(d);
+      float dot = 0.f;
+      for (int c = 0; c < d; ++c) dot = fmaf(q_s[h * d + c], k[c], dot);
+      const bool here = unit_s[lane] >= 0;
+      const float score = here ? dot * scale : -INFINITY;
+      // (fmaxf leaves out a NaN; the weight of its key is NaN all the same, and with it the sum)
+      const float m_new = fmaxf(m_run[u], warp_max(score));
+      const float p = here ? (m_new == -INFINITY ? (isnan(score) ? score : 0.f) : expf(score - m_new)) : 0.f;
+      const float alpha = m_run[u] == -INFINITY ? (l_run[u] == 0.f ? 0.f : 1.f) : expf(m_run[u] - m_new);
+      l_run[u] = l_run[u] * alpha + warp_sum(p);
+      m_run[u] = m_new;
+      p_s[h * kAnyKeys + lane] = p;
+      if (lane == 0) alpha_s[h] = alpha;
+    }
+    __syncthreads();
+    fetch(v_pool, false, j0);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMaxDim / kAnyThreads; ++i) {
+      const int c = tid + i * kAnyThreads;
+      if (c >= d) break;
+#pragma unroll
+      for (int h = 0; h < kAnyHeads; ++h) {
+        if (h >= heads) break;
+        float a = acc[h][i] * alpha_s[h];
+        for (int r = 0; r < kAnyKeys; ++r) a = fmaf(p_s[h * kAnyKeys + r], tile[r * any_row(d) + c], a);
+        acc[h][i] = a;
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (warp + 4 * u < heads && lane == 0) l_s[warp + 4 * u] = l_run[u];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kMaxDim / kAnyThreads; ++i) {
+    const int c = tid + i * kAnyThreads;
+    if (c >= d) break;
+#pragma unroll
+    for (int h = 0; h < kAnyHeads; ++h) {
+      if (h >= heads) break;
+      // no key at all: 0; a sum that is NaN stays one
+      dst[(size_t)h * d + c] = from_float<T>(l_s[h] == 0.f ? 0.f : acc[h][i] / l_s[h]);
+    }
+  }
+}
+
+}  // namespace cache4
+}  // namespace leone
+
+using namespace leone;
+
+extern "C" void leone_packed_set_pdl(int enabled) { pdl_flag() = enabled ? 1 : 0; }
+
+static bool pool_ok(int d, int n_kv, int page_tokens, int table_width, const void* k_pool, const void* v_pool) {
+  return cache4::dim_ok(d) && n_kv > 0 && page_tokens > 0 && page_tokens % cache4::kUnit == 0 && table_width > 0 &&
+         k_pool != nullptr && v_pool != nullptr;
+}
+
+// Arguments as leone_qk_norm_rope_write, the pools in 4 bits.
+extern "C" int leone_append4(int dtype, void* qkv, int n_tokens, int n_q, int n_kv, int d, const void* q_w, const void* k_w,
+                             int w_dtype, float eps, const float* rope, int rotary_dim, int max_positions, const int* positions,
+                             const int* seq_of_token, const int* block_table, int table_width, int n_seqs, void* k_pool,
+                             void* v_pool, int num_pages, int page_tokens, int adjacent, int* status, cudaStream_t stream) {
+  if (n_tokens <= 0) return 0;
+  if (n_q <= 0 || !pool_ok(d, n_kv, page_tokens, table_width, k_pool, v_pool)) return kRefusedSize;
+  if (rope != nullptr && (rotary_dim <= 0 || rotary_dim > d || (rotary_dim & 1))) return kRefusedSize;
+  if (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return kRefusedAlignment;
+  const int warps = 4;
+  const long long blocks = ((long long)n_tokens * (n_q + 2 * n_kv) + warps - 1) / warps;
+  if (blocks > 0x7fffffff) return kRefusedSize;
+  const size_t smem = (size_t)warps * d * sizeof(double);
+#define LAUNCH(T, TW)                                                                                                          \
+  return launch_kernel(cache4::append_kernel<T, TW>, dim3((unsigned)blocks), dim3(warps * 32), smem, stream, (T*)qkv, n_tokens, \
+                       n_q, n_kv, d, (const TW*)q_w, (const TW*)k_w, eps, (const float2*)rope, rotary_dim, max_positions,       \
+                       positions, seq_of_token, block_table, table_width, n_seqs, (uint8_t*)k_pool, (uint8_t*)v_pool,           \
+                       num_pages, page_tokens, adjacent, status)
+  if (dtype == 0 && w_dtype == 0) LAUNCH(float, float);
+  if (dtype == 1 && w_dtype == 0) LAUNCH(__nv_bfloat16, float);
+  if (dtype == 0 && w_dtype == 1) LAUNCH(float, __nv_bfloat16);
+  if (dtype == 1 && w_dtype == 1) LAUNCH(__nv_bfloat16, __nv_bfloat16);
+#undef LAUNCH
+  return kRefusedDtype;
+}
+
+extern "C" int leone_read4(int dtype, void* k_out, void* v_out, int n_tokens, int n_kv, int d, const int* positions,
+                           const int* seq_of_token, const int* block_table, int table_width, int n_seqs, const void* k_pool,
+                           const void* v_pool, int num_pages, int page_tokens, int* status, cudaStream_t stream) {
+  if (n_tokens <= 0) return 0;
+  if (!pool_ok(d, n_kv, page_tokens, table_width, k_pool, v_pool)) return kRefusedSize;
+  if (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return kRefusedAlignment;
+  const int warps = 4;
+  const long long blocks = ((long long)n_tokens * n_kv + warps - 1) / warps;
+  if (blocks > 0x7fffffff) return kRefusedSize;
+#define LAUNCH(T)                                                                                                            \
+  return launch_kernel(cache4::read_kernel<T>, dim3((unsigned)blocks), dim3(warps * 32), 0, stream, (T*)k_out, (T*)v_out,    \
+                       n_tokens, n_kv, d, positions, seq_of_token, block_table, table_width, n_seqs, (const uint8_t*)k_pool, \
+                       (const uint8_t*)v_pool, num_pages, page_tokens, status)
+  if (dtype == 0) LAUNCH(float);
+  if (dtype == 1) LAUNCH(__nv_bfloat16);
+#undef LAUNCH
+  return kRefusedDtype;
+}
+
+// Arguments as leone_attention_generic, the pools in 4 bits.
+extern "C" int leone_attention4_any(int dtype, const void* qkv, int row_stride, void* out, int out_stride, const void* k_pool,
+                                    const void* v_pool, const int* block_table, int table_width, const int* seq_of_token,
+                                    const int* positions, int n_tokens, int n_q, int n_kv, int d, float scale, int window,
+                                    int page_tokens, int num_pages, int n_seqs, int* status, cudaStream_t stream) {
+  if (n_tokens <= 0) return 0;
+  if (n_q <= 0 || !pool_ok(d, n_kv, page_tokens, table_width, k_pool, v_pool) || n_q % n_kv != 0) return kRefusedSize;
+  if (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return kRefusedAlignment;
+  const long long rows = (long long)n_kv * ((n_q / n_kv + cache4::kAnyHeads - 1) / cache4::kAnyHeads);
+  if (rows > 65535) return kRefusedSize;
+  const int smem = (cache4::kAnyKeys * cache4::any_row(d) + cache4::kAnyHeads * (d + cache4::kAnyKeys + 2)) * 4;
+#define LAUNCH(T)                                                                                                              \
+  do {                                                                                                                         \
+    static bool configured = false;                                                                                            \
+    if (!configured) {                                                                                                         \
+      cudaError_t e = cudaFuncSetAttribute(cache4::attention_any_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,        \
+                                           100 * 1024);                                                                        \
+      if (e != cudaSuccess) return (int)e;                                                                                     \
+      configured = true;                                                                                                       \
+    }                                                                                                                          \
+    return launch_kernel(cache4::attention_any_kernel<T>, dim3(n_tokens, (unsigned)rows), dim3(cache4::kAnyThreads), smem, stream, \
+                         (const T*)qkv, row_stride, (T*)out, out_stride, (const uint8_t*)k_pool, (const uint8_t*)v_pool,        \
+                         block_table, table_width, seq_of_token, positions, n_q, n_kv, d, scale, window, page_tokens,           \
+                         num_pages, n_seqs, status);                                                                           \
+  } while (0)
+  if (dtype == 0) LAUNCH(float);
+  if (dtype == 1) LAUNCH(__nv_bfloat16);
+#undef LAUNCH
+  return kRefusedDtype;
+}

@@ -45,9 +45,12 @@ __host__ __device__ inline NarrowShape narrow_shape(int m, int bn, int k_blocks,
   return c;
 }
 
+// kInt8: both operands are 8-bit integers (128 of them a k-block), the sums int32 (see GemmParams::row_scale).
+template <bool kInt8>
 __global__ void __launch_bounds__(kNarrowThreads, 1)
 gemm_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const GemmParams p,
                    const int BN, const NarrowShape cfg) {
+  constexpr int kElems = kInt8 ? 2 * kTileK : kTileK;        // elements of K in a k-block
   const int kStages = cfg.stages, blocks = cfg.blocks, stage_bytes = blocks * (cfg.a_bytes + cfg.b_bytes);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -60,7 +63,7 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int m_tiles = (p.M + kTileW - 1) / kTileW, n_tiles = (p.N + BN - 1) / BN;
-  const int total = m_tiles * n_tiles, k_blocks = (p.K + kTileK - 1) / kTileK;
+  const int total = m_tiles * n_tiles, k_blocks = (p.K + kElems - 1) / kElems;
   if (threadIdx.x == 0) {
     gave_up = 0;
     for (int s = 0; s < kStages; ++s) {
@@ -104,10 +107,10 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         const int here = min(blocks, k_blocks - c.kb);
         mbar_expect_tx(bar, (uint32_t)(here * (cfg.a_bytes + cfg.b_bytes)));
         for (int i = 0; i < here; ++i)
-          tma_load_2d(dst + blocks * cfg.a_bytes + i * cfg.b_bytes, &map_w, bar, (c.kb + i) * kTileK, c.n);
+          tma_load_2d(dst + blocks * cfg.a_bytes + i * cfg.b_bytes, &map_w, bar, (c.kb + i) * kElems, c.n);
       };
       auto load_x = [&](const Cursor& c, uint32_t dst, uint32_t bar) {
-        for (int i = 0; i < min(blocks, k_blocks - c.kb); ++i) tma_load_2d(dst + i * cfg.a_bytes, &map_x, bar, (c.kb + i) * kTileK, c.m);
+        for (int i = 0; i < min(blocks, k_blocks - c.kb); ++i) tma_load_2d(dst + i * cfg.a_bytes, &map_x, bar, (c.kb + i) * kElems, c.m);
       };
       Cursor c{(int)blockIdx.x, 0, 0, 0};
       start(c);
@@ -115,7 +118,7 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       int early = 0;
       for (; early < kStages && c.t < total; ++early, advance(c)) load_w(c, tiles_base + early * stage_bytes, full0 + 8 * early);
       for (int ahead = p.l2_ahead; ahead > 0 && c.t < total; ahead -= blocks, advance(c))
-        for (int i = 0; i < min(blocks, k_blocks - c.kb); ++i) tma_prefetch_2d(&map_w, (c.kb + i) * kTileK, c.n);
+        for (int i = 0; i < min(blocks, k_blocks - c.kb); ++i) tma_prefetch_2d(&map_w, (c.kb + i) * kElems, c.n);
       pdl_wait();
       c = first;
       for (int i = 0; i < early; ++i, advance(c)) load_x(c, tiles_base + i * stage_bytes, full0 + 8 * i);
@@ -135,7 +138,11 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     }
   } else if (warp == 1) {
     if (elect_one()) {
-      const uint32_t idesc = instr_desc_bf16(kTileW, BN);
+      const uint32_t idesc = kInt8 ? instr_desc_i8(kTileW, BN) : instr_desc_bf16(kTileW, BN);
+      auto issue = [&](uint32_t d, uint32_t x, uint32_t w, uint32_t add) {
+        if constexpr (kInt8) umma_k128_i8(d, x, w, idesc, add);
+        else umma_k64(d, x, w, idesc, add);
+      };
       const uint32_t first = desc_low(tiles_base), step = stage_bytes >> 4;
       const uint32_t a_step = cfg.a_bytes >> 4, b_step = cfg.b_bytes >> 4, b_at = blocks * a_step;
       uint32_t a = first, bar = full0, phase = 0;
@@ -149,9 +156,9 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         int left = k_blocks;
         for (; left > 0; left -= blocks) {
           if (!mbar_wait(bar, phase, giveup)) break;
-          umma_k64(tmem_d, a, a + b_at, idesc, sum);
+          issue(tmem_d, a, a + b_at, sum);
           sum = 1;
-          if (blocks == 2 && left > 1) umma_k64(tmem_d, a + a_step, a + b_at + b_step, idesc, 1);
+          if (blocks == 2 && left > 1) issue(tmem_d, a + a_step, a + b_at + b_step, 1);
           umma_commit(bar + 8 * kStages);
           bar += 8;
           a += step;
@@ -179,7 +186,7 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         if (ok) tc_fence_after();
         return ok;
       };
-      if (!finish_rows(p, taddr, m_tile * kTileW + quarter * 32, n_tile * BN, 0, BN, box, complete, [](const float (&)[8]) {})) break;
+      if (!finish_rows<kInt8>(p, taddr, m_tile * kTileW + quarter * 32, n_tile * BN, 0, BN, box, complete, [](const float (&)[8]) {})) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_empty0 + 8 * buf);
@@ -207,6 +214,30 @@ gemm_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
 using namespace leone;
 using namespace leone::tc;
 
+static int launch_narrow(bool int8, const void* x, const void* w, int ldx, int ldw, int width, int sm_count, const GemmParams& p,
+                         cudaStream_t stream) {
+  const int k_blocks = int8 ? (p.K + 2 * kTileK - 1) / (2 * kTileK) : (p.K + kTileK - 1) / kTileK;
+  const long long total = (long long)((p.N + width - 1) / width) * ((p.M + kTileW - 1) / kTileW);
+  if (total > 0x7fffffff) return kRefusedSize;
+  const int grid = (int)(total < sm_count ? total : sm_count), most = (int)((total + grid - 1) / grid);
+  const NarrowShape cfg = narrow_shape(p.M, width, k_blocks, most > 64 ? 64 : most);
+  if (cfg.stages < 2 && (k_blocks + cfg.blocks - 1) / cfg.blocks * (long long)most >= 2) return kRefusedSize;
+  auto kernel = int8 ? gemm_narrow_kernel<true> : gemm_narrow_kernel<false>;
+  static bool configured[2] = {false, false};
+  if (!configured[int8]) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 64);
+    if (e != cudaSuccess) return (int)e;
+    configured[int8] = true;
+  }
+  auto make_map = int8 ? make_tensor_map_2d_i8 : make_tensor_map_2d;
+  CUtensorMap mw, mx;
+  int r = make_map(&mw, w, (uint64_t)p.N, (uint64_t)p.K, (uint64_t)ldw, (uint32_t)width);
+  if (r != 0) return r;
+  r = make_map(&mx, x, (uint64_t)p.M, (uint64_t)p.K, (uint64_t)ldx, (uint32_t)cfg.token_rows);
+  if (r != 0) return r;
+  return launch_kernel(kernel, dim3((unsigned)grid), dim3(kNarrowThreads), (size_t)cfg.smem_bytes, stream, mw, mx, p, width, cfg);
+}
+
 // The arguments and epilogues of leone_gemm_pair (0 bf16, 1 fp32, 2 fp32 += residual, 3 gate) with tiles of 128 tokens x `width` weight
 // rows (a multiple of 16 from 16 to 256, of 32 with the gate); a norm before the product, none after it.  (The callers' rules
 // take it for products without a norm on either side.)
@@ -221,27 +252,29 @@ extern "C" int leone_gemm_narrow(const void* x, const void* w, void* out, const 
   if (epilogue == 3 && ((n % 32) != 0 || (width % 32) != 0)) return kRefusedSize;
   if (norm_in_ss != nullptr && norm_in_parts < 1) return kRefusedSize;
   if ((uintptr_t)bias & 15) return kRefusedAlignment;
-  const int k_blocks = (k + kTileK - 1) / kTileK;
-  const long long total = (long long)((n + width - 1) / width) * ((m + kTileW - 1) / kTileW);
-  if (total > 0x7fffffff) return kRefusedSize;
-  const int grid = (int)(total < sm_count ? total : sm_count), most = (int)((total + grid - 1) / grid);
-  const NarrowShape cfg = narrow_shape(m, width, k_blocks, most > 64 ? 64 : most);
-  if (cfg.stages < 2 && (k_blocks + cfg.blocks - 1) / cfg.blocks * (long long)most >= 2) return kRefusedSize;
-  static bool configured = false;
-  if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_narrow_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 64);
-    if (e != cudaSuccess) return (int)e;
-    configured = true;
-  }
-  CUtensorMap mw, mx;
-  int r = make_tensor_map_2d(&mw, w, (uint64_t)n, (uint64_t)k, (uint64_t)ldw, (uint32_t)width);
-  if (r != 0) return r;
-  r = make_tensor_map_2d(&mx, x, (uint64_t)m, (uint64_t)k, (uint64_t)ldx, (uint32_t)cfg.token_rows);
-  if (r != 0) return r;
   GemmParams p{out, residual, m, n, k, ldc, epilogue, 1, 0, nullptr, nullptr, status, nullptr,
                nullptr, nullptr, nullptr, 0, norm_in_ss, norm_in_parts, norm_eps, 8};
   set_gate_shape(p, gate_shape);
   p.bias = bias;
-  return launch_kernel(gemm_narrow_kernel, dim3((unsigned)grid), dim3(kNarrowThreads), (size_t)cfg.smem_bytes, stream, mw, mx, p,
-                       width, cfg);
+  return launch_narrow(false, x, w, ldx, ldw, width, sm_count, p, stream);
+}
+
+// The same product of 8-bit integers: x [m, k] and w [n, k] hold codes, out[m, n] = sum * x_scale[m] * w_scale[n] (then bias and
+// epilogue).  k a multiple of 16; `width` a multiple of 32.
+extern "C" int leone_gemm_narrow_i8(const void* x, const float* x_scale, const void* w, const float* w_scale, void* out,
+                                    const float* residual, int m, int n, int k, int ldx, int ldw, int ldc, int epilogue, int width,
+                                    int* status, int sm_count, const float* gate_shape, const float* bias, cudaStream_t stream) {
+  if (m <= 0 || n <= 0) return 0;
+  if (k <= 0 || (k % 16) != 0 || (ldx % 16) != 0 || (ldw % 16) != 0) return kRefusedAlignment;
+  if (epilogue < 0 || epilogue > 3 || sm_count < 1 || width < 32 || width > 256 || (width % 32) != 0) return kRefusedSize;
+  if ((epilogue == 2 && residual == nullptr) || (epilogue == 3 && (n % 32) != 0) || x_scale == nullptr || w_scale == nullptr)
+    return kRefusedSize;
+  if (((uintptr_t)bias | (uintptr_t)w_scale) & 15) return kRefusedAlignment;
+  GemmParams p{out, residual, m, n, k, ldc, epilogue, 1, 0, nullptr, nullptr, status, nullptr,
+               nullptr, nullptr, nullptr, 0, nullptr, 0, 0.f, 8};
+  set_gate_shape(p, gate_shape);
+  p.bias = bias;
+  p.row_scale = x_scale;
+  p.col_scale = w_scale;
+  return launch_narrow(true, x, w, ldx, ldw, width, sm_count, p, stream);
 }

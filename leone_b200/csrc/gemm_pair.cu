@@ -60,7 +60,7 @@ __host__ __device__ inline PairShape pair_shape(int bn, int blocks) {
 inline int pair_blocks(int bn) { return bn <= 96 ? 2 : 1; }
 
 __device__ __forceinline__ void umma2_k64(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(LEONE_UMMA_K64("2") ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh) : "memory");
+  asm volatile(LEONE_UMMA_BLOCK("2", "f16") ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh) : "memory");
 }
 // One arrival on the barrier at this offset in both blocks of the pair when every MMA issued so
 // far by this thread is done.
@@ -336,7 +336,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         __threadfence();
         break;
       }
-      if (!finish_rows(p, taddr, m_tile * kTileW + quarter * 32, n_tile * BN, c_lo, c_hi, box, complete, squares)) break;
+      if (!finish_rows<false>(p, taddr, m_tile * kTileW + quarter * 32, n_tile * BN, c_lo, c_hi, box, complete, squares)) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {

@@ -66,6 +66,10 @@ struct GemmParams {
   // One fp32 number per weight row added to its sums (before a gate, a residual or a norm after the product), or
   // null.
   const float* bias;
+  // Products of 8-bit integers: the accumulators are int32 sums, and the sum of token m and weight row n stands for
+  // sum * row_scale[m] * col_scale[n].
+  const float* row_scale;
+  const float* col_scale;
 };
 
 // Host side: the gate fields from an optional {slope, limit, shift, cubic} (null: SwiGLU).
@@ -125,6 +129,29 @@ __device__ __forceinline__ void add_bias16(const GemmParams& p, float* v, int n)
     for (int j = 0; j < 16; ++j)
       if (n + j < p.N) v[j] += p.bias[n + j];
   }
+}
+
+// v[j] = v[j] * col_scale[n + j] * row for 16 weight rows, as above.  The weights' scale first: times a token's, which may be near the
+// largest number, a sum of hundreds of thousands would not fit.
+__device__ __forceinline__ void mul_scale16(const GemmParams& p, float* v, int n, float row) {
+  if (n + 16 <= p.N) {
+    const float4* b = reinterpret_cast<const float4*>(p.col_scale + n);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 q = __ldg(b + j);
+      v[4 * j] *= q.x; v[4 * j + 1] *= q.y; v[4 * j + 2] *= q.z; v[4 * j + 3] *= q.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (n + j < p.N) v[j] *= p.col_scale[n + j];
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] *= row;
+}
+// A sum as tensor memory holds it.
+template <bool kInt8> __device__ __forceinline__ float sum_value(uint32_t r) {
+  return kInt8 ? __int2float_rn((int)r) : __uint_as_float(r);
 }
 
 // Swapped orientation: the thread that owns weight row n finishes NC token columns
@@ -531,7 +558,7 @@ __device__ __forceinline__ void fetch_residual_chunk(const GemmParams& p, float4
 // `ready`: waits until the accumulator is complete (false: gave up); the first residual values are requested before it.
 // Called by whole warps.  `squares(s)`: s[i] is the sum of squares of output row m0 + 4 i + lane / 8 over these
 // columns, for the norm after the product (the row's eight lanes have it).
-template <class Ready, class Squares>
+template <bool kInt8, class Ready, class Squares>
 __device__ __forceinline__ bool finish_rows(const GemmParams& p, uint32_t taddr, int m0, int n0, int c_lo, int c_hi,
                                             uint32_t box, Ready ready, Squares squares) {
   const int lane = threadIdx.x & 31;
@@ -539,7 +566,7 @@ __device__ __forceinline__ bool finish_rows(const GemmParams& p, uint32_t taddr,
   const int sw = lane & 7;
   const int row_out = lane >> 3, unit = lane & 7;                     // on the way out: rows 4 i + row_out, 16-byte piece `unit`
   if (m0 >= p.M) return ready();                                      // no such tokens: nothing to store
-  const float rs = norm_in_factor(p, m0 + lane);
+  const float rs = kInt8 ? (m0 + lane < p.M ? p.row_scale[m0 + lane] : 0.f) : norm_in_factor(p, m0 + lane);
   auto put = [&](int u, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((u ^ sw) << 4)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
   };
@@ -584,7 +611,8 @@ __device__ __forceinline__ bool finish_rows(const GemmParams& p, uint32_t taddr,
           if (q == 1 && !whole) break;
           float v[16];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[16 * q + j]) * rs;
+          for (int j = 0; j < 16; ++j) v[j] = sum_value<kInt8>(r[16 * q + j]) * (kInt8 ? 1.f : rs);
+          if constexpr (kInt8) mul_scale16(p, v, n0 + c + 16 * q, rs);
           if (p.bias != nullptr) add_bias16(p, v, n0 + c + 16 * q);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -671,8 +699,14 @@ __device__ __forceinline__ bool finish_rows(const GemmParams& p, uint32_t taddr,
         float u[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          v[j] = __uint_as_float(r[j]) * rs;
-          u[j] = __uint_as_float(r[16 + j]) * rs;
+          v[j] = sum_value<kInt8>(r[j]) * (kInt8 ? 1.f : rs);
+          u[j] = sum_value<kInt8>(r[16 + j]) * (kInt8 ? 1.f : rs);
+        }
+        if constexpr (kInt8) {
+          if (n0 + at < p.N) {                         // (rows come in whole groups of 32)
+            mul_scale16(p, v, n0 + at, rs);
+            mul_scale16(p, u, n0 + at + 16, rs);
+          }
         }
         if (__builtin_expect(p.bias != nullptr, 0) && n0 + at < p.N) {
           add_bias16(p, v, n0 + at);
@@ -690,7 +724,8 @@ __device__ __forceinline__ bool finish_rows(const GemmParams& p, uint32_t taddr,
         tmem_ld16_issue(taddr + at, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) * rs;
+        for (int j = 0; j < 16; ++j) v[j] = sum_value<kInt8>(r[j]) * (kInt8 ? 1.f : rs);
+        if constexpr (kInt8) mul_scale16(p, v, n0 + at, rs);
         if (__builtin_expect(p.bias != nullptr, 0)) add_bias16(p, v, n0 + at);
       }
       put(2 * h, pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));

@@ -155,18 +155,26 @@ __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t a_desc, uint
 // with narrow tiles: the descriptors' high words are constants, and 16 elements further along K are 32 bytes, 2 in the low word.
 constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);       // as in smem_desc_sw128
 __device__ __forceinline__ uint32_t desc_low(uint32_t smem_addr) { return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16); }
-#define LEONE_UMMA_K64(group)                                                                                                  \
+#define LEONE_UMMA_BLOCK(group, kind)                                                                                          \
   "{\n\t.reg .pred p, t;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\t"                                                            \
-  "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, %0, %0;\n\t"                                                                       \
-  "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\ttcgen05.mma.cta_group::" group ".kind::f16 [%0], a, b, %3, p;\n\t"           \
+  "setp.ne.b32 p, %4, 0;\n\tsetp.eq.b32 t, %0, %0;\n\t"                                                                        \
+  "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\ttcgen05.mma.cta_group::" group ".kind::" kind " [%0], a, b, %3, p;\n\t"     \
   "add.u32 x, %1, 2;\n\tadd.u32 y, %2, 2;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\t"                                   \
-  "tcgen05.mma.cta_group::" group ".kind::f16 [%0], a, b, %3, t;\n\t"                                                          \
+  "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], a, b, %3, t;\n\t"                                                     \
   "add.u32 x, %1, 4;\n\tadd.u32 y, %2, 4;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\t"                                   \
-  "tcgen05.mma.cta_group::" group ".kind::f16 [%0], a, b, %3, t;\n\t"                                                          \
+  "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], a, b, %3, t;\n\t"                                                     \
   "add.u32 x, %1, 6;\n\tadd.u32 y, %2, 6;\n\tmov.b64 a, {x, %5};\n\tmov.b64 b, {y, %5};\n\t"                                   \
-  "tcgen05.mma.cta_group::" group ".kind::f16 [%0], a, b, %3, t;\n\t}"
+  "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], a, b, %3, t;\n\t}"
 __device__ __forceinline__ void umma_k64(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(LEONE_UMMA_K64("1") ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh) : "memory");
+  asm volatile(LEONE_UMMA_BLOCK("1", "f16") ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh) : "memory");
+}
+// The same for 8-bit integers: a k-block of 128 of them fills the same 128 bytes of a row, and an MMA takes 32 of them.
+__device__ __forceinline__ void umma_k128_i8(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(LEONE_UMMA_BLOCK("1", "i8") ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh) : "memory");
+}
+// Instruction descriptor: signed 8-bit integers x the same -> int32, both operands K-major, M x N tile.
+__host__ __device__ constexpr uint32_t instr_desc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 // The mbarrier gets one arrival when every MMA issued so far by this thread is done.
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
@@ -250,6 +258,22 @@ inline int make_tensor_map_2d(CUtensorMap* map, const void* base, uint64_t rows,
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides,
                   box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : kRefusedAlignment;
+}
+
+// The same for 8-bit integers: tiles of [box_rows, 128].
+inline int make_tensor_map_2d_i8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
+                                 uint32_t box_rows) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (fn == nullptr) return kRefusedSize;
+  if (((uintptr_t)base & 15) != 0 || ld % 16 != 0 || box_rows == 0 || box_rows > 256) return kRefusedAlignment;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {ld};
+  cuuint32_t box[2] = {128, box_rows};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : kRefusedAlignment;
 }
 

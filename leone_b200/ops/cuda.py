@@ -18,9 +18,11 @@ from typing import Optional
 import numpy as np
 import torch
 
+from ..cache import packed
 from ..csrc.build import ensure_built
 from .entry_points import EntryPoints
 from .fast import leading_ones
+from .int8 import MAX_K, Int8Matrix, Int8Products
 
 _STATUS_TEXT = {
     1: "a token id outside the vocabulary reached the embedding kernel",
@@ -171,6 +173,8 @@ class CudaOps:
         self.core.leone_core_set_pdl(1 if enabled else 0)
         if self.__dict__.get("_mixers") is not None:
             self._mixers.leone_mixers_set_pdl(1 if enabled and self._mixers_pdl else 0)
+        if self.__dict__.get("_packed") is not None:
+            self._packed.leone_packed_set_pdl(1 if enabled else 0)
         if self.fast is not None:
             self.fast.lib.leone_bf16_set_pdl(1 if enabled else 0)
 
@@ -216,6 +220,58 @@ class CudaOps:
                            None if gate_bias is None else torch.cat([gate_bias, up_bias]))
         m.gate_up_layout = "stacked"
         return m
+
+    def prepare_matrix_int8(self, codes: torch.Tensor, scales: torch.Tensor, bias: Optional[torch.Tensor] = None) -> Int8Matrix:
+        """A matrix in 8-bit integers: ``codes`` int8 ``[out, in]``, ``scales`` fp32 ``[out]``
+        (:func:`leone_b200.ops.int8.quantize_matrix` makes both of a matrix), ``bias`` ``[out]``.  ``linear`` takes it in place of a
+        :class:`PreparedMatrix`."""
+        _need(codes.dim() == 2 and codes.dtype == torch.int8 and codes.is_contiguous(), "int8 codes must be contiguous int8 [out, in]")
+        _need(codes.shape[1] % 16 == 0 and 0 < codes.shape[1] <= MAX_K and codes.shape[0] > 0,
+              f"a matrix in 8 bits has a width that is a multiple of 16 up to {MAX_K}, not {tuple(codes.shape)}")
+        _need(codes.data_ptr() % 16 == 0, "int8 codes must start on 16 bytes")
+        _need(scales.dtype == torch.float32 and scales.shape == (codes.shape[0],) and scales.device == codes.device,
+              "int8 scales must be fp32, one per row")
+        _need(bias is None or bias.shape == (codes.shape[0],), "a bias has one number per row of its matrix")
+        _need(codes.device == self._here(), f"an int8 matrix lies on {codes.device}, these kernels run on {self._here()}")
+
+        def row(t):                                        # read 16 bytes at a time
+            t = t.to(device=codes.device, dtype=torch.float32).contiguous()
+            return t if t.data_ptr() % 16 == 0 else t.clone()
+
+        return Int8Matrix(codes, row(scales), None if bias is None else row(bias))
+
+    def prepare_gate_up_int8(self, gate_codes: torch.Tensor, gate_scales: torch.Tensor, up_codes: torch.Tensor, up_scales: torch.Tensor,
+                             gate_bias: Optional[torch.Tensor] = None, up_bias: Optional[torch.Tensor] = None) -> Int8Matrix:
+        """A gate and an up matrix in 8-bit integers for :meth:`linear_swiglu`; biases as in :meth:`prepare_gate_up`."""
+        inter = gate_codes.shape[0]
+        _need(gate_codes.shape == up_codes.shape and gate_scales.shape == up_scales.shape == (inter,)
+              and (gate_bias is None) == (up_bias is None), "gate and up matrices differ in shape")
+        layout = "interleaved16" if inter % 16 == 0 and self.dtype == torch.bfloat16 else "stacked"
+
+        def join(gate, up):
+            if gate is None:
+                return None
+            if layout == "stacked":
+                return torch.cat([gate, up])
+            # groups of 32 rows: 16 gate rows, then the 16 up rows of the same columns
+            return torch.stack([gate.unflatten(0, (-1, 16)), up.unflatten(0, (-1, 16))], dim=1).flatten(0, 2).contiguous()
+
+        m = self.prepare_matrix_int8(join(gate_codes, up_codes).contiguous(), join(gate_scales, up_scales), join(gate_bias, up_bias))
+        m.gate_up_layout = layout
+        return m
+
+    def _here(self) -> torch.device:
+        """This object's device with its number."""
+        if self.device.index is None:
+            return torch.device("cuda", torch.cuda.current_device())
+        return self.device
+
+    @property
+    def int8(self) -> Int8Products:
+        products = self.__dict__.get("_int8")
+        if products is None:
+            products = self.__dict__["_int8"] = Int8Products(self)
+        return products
 
     # -- kernels ------------------------------------------------------------------------
     def embedding(self, table, ids, out, status, scale: float = 1.0):
@@ -346,7 +402,8 @@ class CudaOps:
         dtype, out_dtype = x.dtype, out.dtype
         if k != w.in_features or out.shape != (m, w.out_features):
             raise KernelError("linear: shapes do not chain")
-        if dtype != w.weight.dtype or x.stride(1) != 1 or out.stride(1) != 1:
+        int8 = isinstance(w, Int8Matrix)
+        if (dtype != w.weight.dtype and not (int8 and dtype in _DTYPE_CODES)) or x.stride(1) != 1 or out.stride(1) != 1:
             raise KernelError("linear: dtype/stride")
         if residual is not None:
             if out_dtype != torch.float32 or not (residual is out or (
@@ -360,6 +417,13 @@ class CudaOps:
                 raise KernelError("linear: output dtype")
             epilogue = 0
         if m == 0:
+            return
+        if int8:
+            _need(norm_in is None and norm_out is None, "linear: a product in 8 bits folds no norm")
+            # (in a 32-bit run `out` is fp32 without a residual: the epilogue that stores fp32)
+            if epilogue == 0 and out_dtype == torch.float32:
+                epilogue = 1
+            self.launches += self.int8.run(x, w, out, epilogue, residual, None)
             return
         if norm_in is not None or norm_out is not None:
             _need(norm_out is None or epilogue in (1, 2), "linear: norm_out needs fp32 output")
@@ -380,8 +444,15 @@ class CudaOps:
         inter = w_gate_up.out_features // 2
         _need(out.shape == (m, inter) and out.dtype == x.dtype and out.is_contiguous(),
               "linear_swiglu: output shape")
+        int8 = isinstance(w_gate_up, Int8Matrix)
+        if int8:
+            _need(x.shape[1] == w_gate_up.in_features and x.stride(1) == 1 and x.dtype in _DTYPE_CODES and norm_in is None
+                  and hasattr(w_gate_up, "gate_up_layout"), "linear_swiglu: a gate and up matrix in 8 bits and its input")
         _need(gate_shape is None or (len(gate_shape) == 4 and gate_shape[1] > 0), "linear_swiglu: gate shape")
         if m == 0:
+            return
+        if int8 and w_gate_up.gate_up_layout == "interleaved16" and out.dtype == torch.bfloat16:
+            self.launches += self.int8.run(x, w_gate_up, out, 3, None, gate_shape)
             return
         if norm_in is not None:
             ni, _ = self._norm_args(m, w_gate_up, norm_in, None)
@@ -389,12 +460,15 @@ class CudaOps:
                   "linear_swiglu: fused norm off the tensor-core path")
             self.launches += 1
             return
-        if self.fast is not None and self.fast.linear_swiglu(x, w_gate_up, out, None, gate_shape):
+        if not int8 and self.fast is not None and self.fast.linear_swiglu(x, w_gate_up, out, None, gate_shape):
             self.launches += 1
             return
         _need(getattr(w_gate_up, "gate_up_layout", None) == "stacked", "gate/up layout")
         scratch = self._scratch("gate_up", m, 2 * inter, x.dtype)
-        self._gemm_simt(x, w_gate_up.weight, scratch, 0, None, w_gate_up.bias)
+        if int8:
+            self.linear(x, w_gate_up, scratch)
+        else:
+            self._gemm_simt(x, w_gate_up.weight, scratch, 0, None, w_gate_up.bias)
         self.launches += 1
         if gate_shape is None:
             _check(self.core_calls.leone_swiglu(_dt(x.dtype), scratch, out, m, inter,
@@ -455,6 +529,14 @@ class CudaOps:
             if table.dtype != torch.float32 or len(shape) != 3 or shape[1] * 2 != rotary_dim or shape[2] != 2 or not table.is_contiguous():
                 raise KernelError("rotary table layout")
             max_pos = shape[0]
+        if cache is not None and getattr(cache, "bits", None) == 4:
+            pool_args = self._pool4(cache, n_kv, d)
+            self.launches += 1
+            _check(self.packed_calls.leone_append4(
+                _dt(dtype), qkv, n, n_q, n_kv, d, q_norm_w, k_norm_w, w_dtype, float(eps), table, rotary_dim, max_pos, ctx.positions,
+                ctx.seq_of_token, *pool_args, 1 if pairing == "adjacent" else 0, ctx.status, self._stream()),
+                "qk_norm_rope_write (4 bits)")
+            return
         if cache is not None:
             kp, vp, bt = cache.k_pool, cache.v_pool, cache.block_table
             pages, heads, rows, width = kp.shape
@@ -473,6 +555,53 @@ class CudaOps:
             ctx.seq_of_token, *pool_args, 1 if pairing == "adjacent" else 0, ctx.status,
             self._stream()), "qk_norm_rope_write")
 
+    # -- pages in 4 bits (compiled when a cache first needs them) --------------------------------------
+    @property
+    def packed_calls(self):
+        calls = self.__dict__.get("_packed_calls")
+        if calls is None:
+            lib = ctypes.CDLL(ensure_built("packed"))
+            lib.leone_packed_set_pdl(1 if self._pdl else 0)
+            self.__dict__["_packed"] = lib
+            calls = self.__dict__["_packed_calls"] = EntryPoints(lib)
+        return calls
+
+    def _pool4(self, cache, n_kv, d):
+        """The arguments of a cache in 4 bits, checked."""
+        kp, vp, bt = cache.k_pool, cache.v_pool, cache.block_table
+        if not packed.dim_ok(d):
+            raise KernelError(f"rows of {d} elements cannot be held in 4 bits")
+        if vp is None or kp.dtype != torch.uint8 or vp.dtype != torch.uint8 or kp.dim() != 4 or vp.shape != kp.shape \
+                or kp.shape[1:] != (n_kv, cache.page_tokens, packed.row_bytes(d)) or cache.page_tokens % packed.UNIT \
+                or not kp.is_contiguous() or not vp.is_contiguous() or cache.tokens_per_row != 1:
+            raise KernelError("cache pool layout (4 bits)")
+        if bt.dtype != torch.int32 or bt.dim() != 2 or not bt.is_contiguous():
+            raise KernelError("block table")
+        return bt, bt.shape[1], bt.shape[0], kp, vp, kp.shape[0], cache.page_tokens
+
+    def read_packed_rows(self, ctx, cache, n_kv, d, k_out, v_out):
+        """What a cache in 4 bits holds for the step's tokens: ``k_out`` and ``v_out`` ``[tokens, n_kv * d]``, fp32 or bfloat16.  A
+        token without a page sets the status and leaves its rows as they were."""
+        n = k_out.shape[0]
+        for t in (k_out, v_out):
+            _need(t.shape == (n, n_kv * d) and t.dtype == k_out.dtype and t.is_contiguous(), "read_packed_rows: output layout")
+        _need(ctx.positions.numel() == n == ctx.seq_of_token.numel(), "read_packed_rows: one row per token of the step")
+        self.launches += 1
+        _check(self.packed_calls.leone_read4(_dt(k_out.dtype), k_out, v_out, n, n_kv, d, ctx.positions, ctx.seq_of_token,
+                                             *self._pool4(cache, n_kv, d), ctx.status, self._stream()), "read_packed_rows")
+
+    def _attention4(self, ctx, qkv, out, n_q, n_kv, d, scale, window, cache) -> None:
+        """:meth:`attention` over a cache in 4 bits."""
+        bt, width, rows, kp, vp, pages, page_tokens = self._pool4(cache, n_kv, d)
+        n = qkv.shape[0]
+        _need(n_q > 0 and n_q % n_kv == 0 and qkv.stride(1) == 1 and qkv.shape[1] >= n_q * d, "attention: query rows")
+        if n == 0:
+            return
+        self.launches += 1
+        _check(self.packed_calls.leone_attention4_any(
+            _dt(qkv.dtype), qkv, qkv.stride(0), out, out.stride(0), kp, vp, bt, width, ctx.seq_of_token, ctx.positions, n, n_q, n_kv, d,
+            float(scale), int(window or 0), page_tokens, pages, rows, ctx.status, self._stream()), "attention (4 bits)")
+
     def can_fuse_decode(self, ctx, qkv, n_q, n_kv, d) -> bool:
         """True if the attention kernel can do the q/k norm, rotation and cache write itself
         for this step (then ``qk_norm_rope_write`` is not called and ``attention`` gets
@@ -486,6 +615,10 @@ class CudaOps:
         dtype, shape = qkv.dtype, kp.shape
         if out.shape != (n, n_q * d) or out.dtype != dtype or not out.is_contiguous():
             raise KernelError("attention output layout")
+        if getattr(cache, "bits", None) == 4:
+            _need(fuse is None, "a cache in 4 bits is written before its attention")
+            self._attention4(ctx, qkv, out, n_q, n_kv, d, scale, window, cache)
+            return
         if kp.dtype != dtype or shape[1] != n_kv or shape[3] != d or not kp.is_contiguous() or not vp.is_contiguous():
             raise KernelError("cache pool layout")
         if self.fast is not None and self.fast.attention(ctx, qkv, out, n_q, n_kv, d, scale,

@@ -136,6 +136,7 @@ class PagedCacheView:
     page_tokens: int
     writes: bool = True           # False for a layer that borrows another layer's cache
     tokens_per_row: int = 1       # > 1: a cache of summaries, see PagedKV
+    bits: Optional[int] = None    # 4: pages in 4 bits (leone_b200.cache.packed); None: elements of the pools' dtype
 
 
 @dataclass

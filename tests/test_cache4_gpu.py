@@ -1,0 +1,260 @@
+"""Pages in 4 bits: append, read and attention against plain 64-bit forms."""
+import math
+
+import pytest
+import torch
+
+from leone_b200.cache import packed
+from leone_b200.ops.cuda import KernelError
+from leone_b200.parts.rotary import build_rotary_table
+from tests.fewer_bits import Step, attention64, quantize4, rotate, values4
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+BF16, FP32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops_of():
+    from leone_b200.ops.cuda import CudaOps
+    made = {}
+
+    def get(dtype):
+        if dtype not in made:
+            made[dtype] = CudaOps(DEV, dtype)
+            made[dtype].bind_status(torch.zeros(4, dtype=torch.int32, device=DEV))
+        return made[dtype]
+    return get
+
+
+def _gen(seed):
+    return torch.Generator(DEV).manual_seed(seed)
+
+
+def _pools(step, n_kv, d, fill=0):
+    return [torch.full((step.pages, n_kv, step.page_tokens, packed.row_bytes(d)), fill, dtype=torch.uint8, device=DEV) for _ in range(2)]
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+APPENDS = [
+    # dtype, d, n_q, n_kv, norm, pairing, rotary elements, page tokens, lens
+    (BF16, 128, 16, 8, True, "half_split", 128, 16, [(1, 700)]),
+    (BF16, 128, 32, 8, True, "half_split", 128, 16, [(75, 0), (1, 30), (40, 9)]),
+    (BF16, 128, 3, 1, True, "adjacent", 128, 48, [(33, 47), (1, 0)]),
+    (BF16, 64, 14, 2, False, "half_split", 64, 32, [(5, 3), (17, 40)]),
+    (BF16, 64, 4, 4, True, "adjacent", 32, 16, [(20, 1)]),                    # a part of a head rotates
+    (BF16, 256, 8, 2, True, "half_split", 256, 16, [(9, 100)]),
+    (BF16, 128, 8, 2, True, None, 0, 16, [(30, 2)]),                          # no rotation
+    (FP32, 64, 12, 4, False, "adjacent", 64, 16, [(30, 77), (2, 0)]),
+    (FP32, 128, 2, 1, True, "half_split", 128, 16, [(1, 0), (1, 15), (1, 16), (50, 3)]),
+    (FP32, 16, 4, 2, True, "half_split", 16, 16, [(21, 2), (7, 0)]),
+    (FP32, 96, 4, 2, True, "half_split", 96, 16, [(11, 6)]),
+    (FP32, 512, 2, 1, True, "half_split", 512, 16, [(3, 14)]),
+    (BF16, 192, 4, 2, True, "adjacent", 192, 16, [(6, 10)]),
+]
+
+
+@pytest.mark.parametrize("dtype,d,n_q,n_kv,norm,pairing,rot,page,lens", APPENDS)
+@pytest.mark.parametrize("wdtype", [FP32, BF16])
+def test_append_and_read(ops_of, dtype, d, n_q, n_kv, norm, pairing, rot, page, lens, wdtype):
+    ops = ops_of(dtype)
+    step = Step(lens, page, DEV, seed=d)
+    n = step.ctx.n_tokens
+    rows = torch.randn((n, (n_q + 2 * n_kv) * d), generator=_gen(d + n), device=DEV)
+    rows[:, ::37] *= 9
+    rows = rows.to(dtype)
+    weights = (1 + 0.1 * torch.randn((2, d), generator=_gen(2), device=DEV)).to(wdtype) if norm else (None, None)
+    k_pool, v_pool = _pools(step, n_kv, d, fill=0xA5)
+    view = step.view(k_pool, v_pool)
+    table = build_rotary_table(int(step.pos.max()) + 1, rot, 10000.0).to(DEV) if rot else None
+    got = rows.clone()
+    kw = {} if pairing is None else {"pairing": pairing}
+    eps = 2.0 ** -20
+    ops.qk_norm_rope_write(step.ctx, got, n_q, n_kv, d, weights[0], weights[1], eps, table, rot, view, **kw)
+
+    q, k, v = rows.double().unflatten(1, (n_q + 2 * n_kv, d)).split([n_q, n_kv, n_kv], 1)
+    if norm:
+        q, k = (x * w.double() * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) for x, w in ((q, weights[0]), (k, weights[1])))
+    if rot:
+        q, k = (rotate(x, step.pos, 10000.0, pairing, rot) for x in (q, k))
+    # queries: one rounding to the type of a 64-bit value (in two steps over fp32 for bfloat16)
+    want = q.flatten(1)
+    bound = want.abs() * (_half_step(dtype) + 2.0 ** -23) + 1e-30
+    assert ((got[:, :n_q * d].double() - want).abs() <= bound).all()
+    assert torch.equal(got[:, n_q * d:], rows[:, n_q * d:])                    # keys and values are not written back
+    held = []
+    for pool, x, values in ((k_pool, k, False), (v_pool, v, True)):
+        codes, s, z = packed.unpack_pages(pool, d, values)
+        have = (codes[step.page, :, step.slot], s[step.page, :, step.slot], z[step.page, :, step.slot])
+        want_codes, want_s, want_z = quantize4(x)
+        assert torch.equal(have[0].long(), want_codes)
+        assert torch.equal(have[1].double(), want_s) and torch.equal(have[2].double(), want_z)
+        # off by at most half a scale
+        err = (values4(*have) - x).abs().unflatten(-1, (s.shape[-1], -1))
+        assert (err <= want_s[..., None] * (0.5 + 2.0 ** -20) + 1e-300).all()
+        # no other byte moved
+        other = torch.ones(pool.shape[:3], dtype=torch.bool, device=DEV)
+        other[step.page, :, step.slot] = False
+        fill = packed.unpack_pages(torch.full_like(pool, 0xA5), d, values)
+        for a, b in zip((codes, s, z), fill):
+            assert torch.equal(a[other].float(), b[other].float())
+        held.append(values4(*have))
+    k_out, v_out = torch.full((2, n, n_kv * d), 7.0, dtype=dtype, device=DEV)
+    ops.read_packed_rows(step.ctx, view, n_kv, d, k_out, v_out)
+    for out, x in zip((k_out, v_out), held):
+        assert torch.equal(out, x.flatten(1).float().to(dtype))
+    assert step.ctx.status.tolist() == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("d", [64, 128, 32])
+def test_append_of_odd_groups(ops_of, dtype, d):
+    """Constant groups, zeros, the smallest and largest numbers, infinities and NaN."""
+    ops = ops_of(dtype)
+    step = Step([(9, 3)], 16, DEV)
+    x = torch.randn((9, 3, d), generator=_gen(5), device=DEV)
+    x[0] = 0.0
+    x[1] = -2.7
+    x[2] *= 1e-38
+    x[3, :, 0] = math.inf
+    x[4, :, d - 1] = math.nan
+    x[5, :, 0], x[5, :, 1] = 3.3e38, -3.3e38
+    x[6] = 5e-39                                             # no normal number
+    x[7, :, 3] = -math.inf
+    x[8] = 1000.0 + x[8]
+    rows = x.to(dtype).flatten(1)
+    pools = _pools(step, 1, d)
+    ops.qk_norm_rope_write(step.ctx, rows.clone(), 1, 1, d, None, None, 1e-6, None, 0, step.view(*pools))
+    want = quantize4(rows.double().unflatten(1, (3, d)))
+    for i, (pool, values) in enumerate(zip(pools, (False, True))):
+        codes, s, z = (t[step.page, 0, step.slot] for t in packed.unpack_pages(pool, d, values))
+        assert torch.equal(codes.long(), want[0][:, 1 + i])
+        torch.testing.assert_close(s.double(), want[1][:, 1 + i], rtol=0, atol=0, equal_nan=True)
+        torch.testing.assert_close(z.double(), want[2][:, 1 + i], rtol=0, atol=0, equal_nan=True)
+    assert step.ctx.status.tolist() == [0, 0, 0, 0]
+
+
+def test_append_and_read_report_bad_metadata(ops_of):
+    ops = ops_of(BF16)
+    d, n_kv = 128, 2
+    rows = torch.randn((3, 4 * d + 2 * d), generator=_gen(1), device=DEV).to(BF16)
+    table = build_rotary_table(64, d, 10000.0).to(DEV)
+    for spoil, code in (("page", 2), ("far page", 2), ("sequence", 5), ("position", 3)):
+        step = Step([(3, 17)], 16, DEV)
+        if spoil == "page":
+            step.table[0, 1] = -1
+        if spoil == "far page":
+            step.table[0, 1] = step.pages
+        if spoil == "sequence":
+            step.ctx.seq_of_token[1] = 1
+        if spoil == "position":
+            step.ctx.positions[2] = 64
+        pools = _pools(step, n_kv, d, fill=3)
+        ops.qk_norm_rope_write(step.ctx, rows.clone(), 2, n_kv, d, None, None, 1e-6, table, d, step.view(*pools))
+        assert int(step.ctx.status[0]) == code, spoil
+        step.ctx.status.zero_()
+        out = torch.full((2, 3, n_kv * d), 5.0, dtype=BF16, device=DEV)
+        ops.read_packed_rows(step.ctx, step.view(*pools), n_kv, d, *out)
+        assert int(step.ctx.status[0]) == (2 if spoil == "position" else code), spoil
+
+
+def _attention_case(ops, dtype, n_q, n_kv, d, lens, page, window, seed=0, stale=True, stride=0, scale=None):
+    step = Step(lens, page, DEV, seed=seed, window=window)
+    pools, plain = [], []
+    for values in (False, True):
+        x = torch.randn((step.pages, n_kv, page, d), generator=_gen(seed + 3 + values), device=DEV).double()
+        if not values:
+            x[..., ::19] *= 4
+        codes, s, z = quantize4(x)
+        plain.append(values4(codes, s, z))
+        pool = packed.pack_pages(codes, s, z, values)
+        if stale:
+            # rows that hold no token of a sequence are NaN: nothing of them may reach a result
+            owned = torch.zeros((step.pages, page), dtype=torch.bool, device=DEV)
+            for i, (new, past) in enumerate(lens):
+                p = torch.arange(max(0, past - window + 1) if window else 0, new + past, device=DEV)
+                owned[step.table[i, p // page].long(), p % page] = True
+            broken = packed.pack_pages(codes, torch.where(owned[:, None, :, None], s, math.nan),
+                                       torch.where(owned[:, None, :, None], z, math.nan), values)
+            pool = broken
+        pools.append(pool)
+    n = step.ctx.n_tokens
+    cols = (n_q + 2 * n_kv) * d + stride
+    qkv = torch.randn((n, cols), generator=_gen(seed + 9), device=DEV).to(dtype)
+    scale = d ** -0.5 if scale is None else scale
+    out = torch.full((n, n_q * d), 77.0, dtype=dtype, device=DEV)
+    ops.attention(step.ctx, qkv, out, n_q, n_kv, d, scale, window or None, step.view(*pools))
+    want, top_s, top_v = attention64(qkv[:, :n_q * d].double().unflatten(1, (n_q, d)), *plain, lens, step.table, page, scale, window)
+    assert step.ctx.status.tolist() == [0, 0, 0, 0]
+    return step, qkv, pools, out.unflatten(1, (n_q, d)).double(), want, top_s.double(), top_v.double()
+
+
+def _bounds(dtype, step, d, n_q, want, top_s, top_v, tensor_cores):
+    """How far an output may be off, per (token, head).
+
+    Scores: d products summed in fp32, relative to sum |q k| at most (d + 4) 2^-23 (a tensor core's additions truncate).  On tensor cores
+    codes are 128 + code, 9 times the largest code, and the offset is taken out again: 10 times that.  A score's error moves each
+    weight by that much relative to itself, twice (the sum too).  Weights and sums: (keys + 8) 2^-23.  On tensor cores a weight times its
+    scale is rounded to bfloat16: a half step of the weighted codes around their middle, 8 s <= 0.54 (max - min) of 2^-8 each; again
+    codes of 128 + code in the sums.  Then one rounding to the type."""
+    keys = torch.tensor(step.ctx.ctx_lens, device=DEV).double()[step.seq]
+    score = (d + 4) * 2.0 ** -23 * top_s * (10 if tensor_cores else 1)
+    weight = (keys + 8)[:, None] * 2.0 ** -23 * (10 if tensor_cores else 1)
+    off = top_v * (2 * score + 2 * weight + (0.54 * 2 * 2.0 ** -8 if tensor_cores else 0))
+    return off[..., None] + want.abs() * _half_step(dtype) + 1e-30
+
+
+ANY = [
+    # dtype, n_q, n_kv, d, lens, page, window
+    (FP32, 4, 2, 16, [(5, 0), (1, 40)], 16, 0),
+    (FP32, 12, 4, 64, [(3, 77), (1, 0), (20, 5)], 16, 0),
+    (FP32, 16, 1, 128, [(1, 200), (2, 31)], 32, 0),                           # 16 query heads a cached one
+    (FP32, 3, 1, 96, [(33, 30)], 16, 20),
+    (FP32, 2, 2, 512, [(4, 60)], 48, 0),
+    (FP32, 64, 8, 128, [(1, 300), (7, 100)], 16, 64),
+    (BF16, 6, 2, 32, [(9, 50), (1, 0)], 16, 0),
+    (BF16, 20, 1, 96, [(1, 130)], 16, 0),
+    (BF16, 4, 2, 256, [(17, 100)], 16, 33),
+]
+
+
+@pytest.mark.parametrize("dtype,n_q,n_kv,d,lens,page,window", ANY)
+def test_attention_any_size(ops_of, dtype, n_q, n_kv, d, lens, page, window):
+    step, _, _, out, want, top_s, top_v = _attention_case(ops_of(dtype), dtype, n_q, n_kv, d, lens, page, window, seed=d)
+    assert ((out - want).abs() <= _bounds(dtype, step, d, n_q, want, top_s, top_v, False)).all()
+
+
+def test_attention_refusals(ops_of):
+    ops = ops_of(BF16)
+    step = Step([(1, 20)], 16, DEV)
+    d, n_q, n_kv = 128, 4, 2
+    pools = _pools(step, n_kv, d)
+    qkv = torch.zeros((1, (n_q + 2 * n_kv) * d), dtype=BF16, device=DEV)
+    out = torch.zeros((1, n_q * d), dtype=BF16, device=DEV)
+    good = step.view(*pools)
+
+    def refused(match, **kw):
+        args = dict(ctx=step.ctx, qkv=qkv, out=out, n_q=n_q, n_kv=n_kv, d=d, cache=good)
+        args.update(kw)
+        with pytest.raises(KernelError, match=match):
+            ops.attention(args["ctx"], args["qkv"], args["out"], args["n_q"], args["n_kv"], args["d"], 0.1, None, args["cache"],
+                          **({"fuse": {}} if "fuse" in kw else {}))
+
+    refused("pool layout", cache=step.view(pools[0].view(torch.int8), pools[1]))
+    refused("pool layout", cache=step.view(pools[0], None))
+    refused("pool layout", cache=step.view(pools[0][:, :, :, :64], pools[1]))
+    refused("pool layout", cache=step.view(pools[0].transpose(0, 1), pools[1].transpose(0, 1)))
+    refused("output layout", out=out[:, :64])
+    refused("written before", fuse=True)
+    refused("query rows", n_q=3, out=out[:, :3 * d].contiguous())
+    odd = Step([(1, 20)], 24, DEV)
+    refused("pool layout", cache=odd.view(*_pools(odd, n_kv, d)))
+    with pytest.raises(KernelError, match="cannot be held"):
+        ops.qk_norm_rope_write(step.ctx, torch.zeros((1, 3 * 20), dtype=BF16, device=DEV), 1, 1, 20, None, None, 1e-6, None, 0, good)
+    bad = step.view(*pools)
+    bad.block_table = step.table.long()
+    refused("block table", cache=bad)
