@@ -150,10 +150,11 @@ class GroupSpec:
     dtype: object = None        # storage dtype of the pages (None: the engine's run dtype)
     tag: str = ""               # groups with different tags are never merged
     tokens_per_row: int = 1     # > 1: one cached row per so many positions (a cache of summaries)
+    bits: Optional[int] = None  # 4: rows in 4 bits (packed.py), whose widths here are bytes
 
     def key(self):
         return (self.kind, self.num_kv_heads, self.head_dim, self.window, self.value_head_dim, self.dtype, self.tag,
-                self.tokens_per_row)
+                self.tokens_per_row, self.bits)
 
     def page_rows(self, page_tokens: int) -> int:
         """Rows a page holds: one per token, or one per ``tokens_per_row`` positions."""

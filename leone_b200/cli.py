@@ -45,9 +45,9 @@ def cmd_generate(args) -> int:
         return 2
     if args.kv is not None:
         want = {"bfloat16": "bf16", "float32": "f32"}[args.dtype]
-        if args.kv != want:
+        if args.kv not in (want, "q4"):
             print(f"leone generate: --kv {args.kv} is not available; the cache is stored in the run "
-                  f"dtype ({want}); quantized and f16 caches are not built", file=sys.stderr)
+                  f"dtype ({want}) or in 4 bits (q4); q8 and f16 caches are not built", file=sys.stderr)
             return 2
     from .engine.engine import Engine
     from .engine.generate import generate
@@ -58,7 +58,8 @@ def cmd_generate(args) -> int:
     longest = max(len(p) for p in prompts) + args.tokens
     pages = args.num_pages or (-(-longest // args.page_tokens) + 1) * len(prompts)
     kw = dict(dtype=args.dtype, page_tokens=args.page_tokens, num_pages=pages, max_requests=max(len(prompts), 1),
-              max_batch_tokens=args.max_batch_tokens)
+              max_batch_tokens=args.max_batch_tokens, cache_bits=4 if args.kv == "q4" else None,
+              weight_bits=8 if args.weights == "int8" else None)
     if args.random_weights:
         from .engine.generate import load_config
         engine = Engine.from_config(load_config(args.model),
@@ -257,8 +258,10 @@ def build_parser() -> argparse.ArgumentParser:
                         "weights are drawn from --weights-seed")
     g.add_argument("--weights-seed", type=int, default=None, help="seed of --random-weights. Default: --seed")
     g.add_argument("--eager-decode", action="store_true", help="disable decode graph replay")
-    g.add_argument("--kv", choices=["q8", "f16", "f32", "bf16"], default=None,
-                   help="KV cache storage; only the run dtype is available")
+    g.add_argument("--kv", choices=["q4", "q8", "f16", "f32", "bf16"], default=None,
+                   help="KV cache storage: the run dtype or q4 (4 bits)")
+    g.add_argument("--weights", choices=["int8"], default=None,
+                   help="keep the matrices of attention and dense feed-forward layers in 8-bit integers")
     g.add_argument("--debug-tokens", help="write generated token ids as JSON")
     g.add_argument("--debug-logits", help="write the top five logits for each token")
     g.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")

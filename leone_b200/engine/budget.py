@@ -61,6 +61,16 @@ def plan_memory(model, specs, stored_dtypes: Optional[Dict[str, torch.dtype]], r
         state += n
     plan = dict(weights=weights, load=model.load_transient_bytes(), cache=cache, state=state,
                 scratch=model.scratch_bytes(max_batch_tokens, 2 * max_requests))
+    shapes = model.matrices()
+    if shapes:
+        # Matrices in 8 bits: every tensor is uploaded in its own type first and leaves part by part, before the cache is
+        # allocated; what is needed is the larger of the two states.  A matrix's codes stand beside it (and, of a gate and its
+        # up matrix, once more where they are joined), with 64-bit quotients of up to 2^24 elements.
+        largest = max(r * c for r, c in shapes)
+        loading = weights + plan["load"] + 2 * largest + 32 * min(largest, 1 << 24)
+        kept = weights + sum(r * c + 4 * r - r * c * run_dtype.itemsize for r, c in shapes)
+        plan["weights"] = kept
+        plan["load"] = max(0, loading - kept - plan["cache"] - plan["state"] - plan["scratch"])
     plan["required"] = sum(plan.values())
     return plan
 

@@ -20,6 +20,7 @@ from typing import Dict, Hashable, List, Optional, Sequence
 import numpy as np
 import torch
 
+from ..cache import packed
 from ..cache.pages import CacheManager, GroupSpec, OutOfPages
 from ..cache.slots import SlotRecords
 from ..parts.base import BundleView, CacheBundle, FixedState, PagedCacheView, PagedKV, Runtime, StateView
@@ -62,8 +63,13 @@ class Engine:
                  dtype="bfloat16", device="cuda:0", page_tokens: int = 16,
                  max_tokens: Optional[int] = None, num_pages: Optional[int] = None,
                  max_requests: int = 64, max_batch_tokens: int = 2048, ops=None,
-                 folder: Optional[str] = None, random_seed: Optional[int] = None, free_bytes=None):
-        """``free_bytes``: a callable that says how many bytes the device has free, for the
+                 folder: Optional[str] = None, random_seed: Optional[int] = None, free_bytes=None,
+                 cache_bits: Optional[int] = None, weight_bits: Optional[int] = None):
+        """``cache_bits = 4``: keys and values are cached in 4 bits (``csrc/cache4.cuh``; 0.28 of the bytes of bfloat16), by every layer
+        that caches any, in pages of a multiple of 16 tokens.  ``weight_bits = 8``: the matrices of attention and dense
+        feed-forward layers are kept in 8-bit integers with a scale for each row, and tokens are rounded to 8 bits for their
+        products; other parts (embedding, output head, experts, ..) keep the run dtype.
+        ``free_bytes``: a callable that says how many bytes the device has free, for the
         memory budget (default: the CUDA driver's figure plus what torch's allocator holds
         unused; no check on a device without such a figure)."""
         self.dtype = parse_dtype(dtype)
@@ -72,10 +78,17 @@ class Engine:
         if ops is None:
             ops = default_ops(self.device, self.dtype)
         self.ops = ops
-        self.rt = Runtime(self.device, self.dtype, ops, max_batch_tokens)
+        self.rt = Runtime(self.device, self.dtype, ops, max_batch_tokens, cache_bits, weight_bits)
         self.max_batch_tokens = max_batch_tokens
         self.model = Model(spec, self.rt)
         specs = self.model.weight_specs()
+        if weight_bits is not None and not self.model.matrices():
+            raise ValueError("weight_bits: no part of this model keeps its matrices in 8 bits")
+        narrow = sorted({cols for _, cols in self.model.matrices() if cols % 16})
+        if narrow:
+            raise ValueError(f"weight_bits: rows of matrices in 8 bits are a multiple of 16 elements, not {narrow}")
+        if cache_bits is not None and page_tokens % packed.UNIT:
+            raise ValueError(f"cache_bits: pages in 4 bits hold a multiple of {packed.UNIT} tokens, not {page_tokens}")
 
         # -- what the cache will hold (nothing is allocated yet) ------------------------------
         self.page_tokens = page_tokens
@@ -105,7 +118,9 @@ class Engine:
                 # the part says what it caches (widths, dtype, when pages go back); equal requests share a group
                 r = req.resolved(self.dtype)
                 gs = GroupSpec(r.lifetime, r.num_kv_heads, r.head_dim, r.window, value_head_dim=r.value_head_dim,
-                               dtype=r.dtype, tag=r.tag, tokens_per_row=r.tokens_per_row)
+                               dtype=r.dtype, tag=r.tag, tokens_per_row=r.tokens_per_row, bits=r.bits)
+                if cache_bits is not None and r.bits != cache_bits:
+                    raise ValueError(f"cache_bits: run position {key[0]} caches rows that are not held in {cache_bits} bits")
                 for gid, existing in enumerate(group_specs):
                     if existing.key() == gs.key():
                         break
@@ -126,6 +141,9 @@ class Engine:
                 self._run_source[pos] = source
             else:
                 self._run_binding[pos] = bind((pos,), req)
+
+        if cache_bits is not None and not group_specs:
+            raise ValueError("cache_bits: no layer of this model caches keys and values")
 
         # -- the memory budget, before anything is uploaded -----------------------------------
         stored = None
@@ -290,7 +308,7 @@ class Engine:
                 _, gid, k, per_row = binding
                 kp, vp = self.pools[gid]
                 return PagedCacheView(kp[k], None if vp is None else vp[k], ctx.block_tables[gid],
-                                      self.page_tokens, writes, per_row)
+                                      self.page_tokens, writes, per_row, self.cache.groups[gid].spec.bits)
             return StateView(self._run_state[binding[1]], writes)
 
         ctx.embedding_cache = view(self._embedding_binding, True)

@@ -62,7 +62,8 @@ def generate(model: Union[str, Engine], prompts: Sequence[Sequence[int]], max_ne
              max_batch_tokens: int = 2048, max_running: int = 64, policy: str = "reserve",
              device: str = "cuda:0", return_stats: bool = False, decode_quantum: int = 1,
              use_graphs: bool = True, prefill_first: bool = True, truncations=(), penalties=None, mirostat=None,
-             random_weights: bool = False, weights_seed: Optional[int] = None):
+             random_weights: bool = False, weights_seed: Optional[int] = None, cache_bits: Optional[int] = None,
+             weight_bits: Optional[int] = None):
     """Generate ``max_new_tokens`` tokens for each prompt (a list of token ids).
 
     ``model`` is a model folder (config.json + model.safetensors) or an :class:`Engine`.
@@ -83,9 +84,12 @@ def generate(model: Union[str, Engine], prompts: Sequence[Sequence[int]], max_ne
     :class:`leone_b200.sampling.sampler.Penalties` applied to the logits from each request's own
     history before sampling (greedy included).  ``mirostat``: ``(target surprise, learning rate)``
     for Mirostat v2, which keeps a maximum surprise per request.
+    ``cache_bits`` (4) and ``weight_bits`` (8): see :class:`Engine`; an engine that is given has its own.
     """
     prompts = [list(map(int, p)) for p in prompts]
     if isinstance(model, Engine):
+        if (cache_bits, weight_bits) != (None, None) and (cache_bits, weight_bits) != (model.rt.cache_bits, model.rt.weight_bits):
+            raise ValueError(f"generate: the given engine has cache_bits {model.rt.cache_bits} and weight_bits {model.rt.weight_bits}")
         engine = model
     else:
         longest = max((len(p) for p in prompts), default=0) + max_new_tokens
@@ -93,7 +97,7 @@ def generate(model: Union[str, Engine], prompts: Sequence[Sequence[int]], max_ne
             per_request = -(-longest // page_tokens) + 1
             num_pages = per_request * min(len(prompts), max_running)
         kw = dict(dtype=dtype, device=device, page_tokens=page_tokens, num_pages=num_pages,
-                  max_requests=max_running, max_batch_tokens=max_batch_tokens)
+                  max_requests=max_running, max_batch_tokens=max_batch_tokens, cache_bits=cache_bits, weight_bits=weight_bits)
         if random_weights:
             engine = Engine.from_config(load_config(model), seed if weights_seed is None else weights_seed, **kw)
         else:

@@ -177,6 +177,10 @@ class Model:
         ops_scratch = getattr(self.rt.ops, "scratch_bytes", None)
         return total + (ops_scratch() if ops_scratch is not None else 0)
 
+    def matrices(self):
+        """``(rows, cols)`` of every matrix that a part keeps as the runtime says (:meth:`Runtime.prepare_matrix`)."""
+        return [shape for h in self._holders for shape in h.part.matrices()] if self.rt.weight_bits else []
+
     def load_transient_bytes(self) -> int:
         """The most any one part holds beyond its inputs while it loads."""
         parts = [h.part for h in self._holders] + [self.embedding, self.head, self.final_norm] + \

@@ -149,10 +149,10 @@ class Attention(Mixer):
         if self.bias_names:
             bias = torch.zeros(self.in_cols, dtype=torch.float32, device=rows[0].device)
             bias[:self.qkv_cols] = torch.cat([tensors[name].float() for name in self.bias_names])
-            self.w_qkv = self.rt.ops.prepare_matrix(torch.cat(rows, dim=0).contiguous(), bias)
+            self.w_qkv = self.rt.prepare_matrix(torch.cat(rows, dim=0).contiguous(), bias)
         else:
-            self.w_qkv = self.rt.ops.prepare_matrix(torch.cat(rows, dim=0).contiguous())
-        self.w_o = self.rt.ops.prepare_matrix(tensors[self.names["o"]])
+            self.w_qkv = self.rt.prepare_matrix(torch.cat(rows, dim=0).contiguous())
+        self.w_o = self.rt.prepare_matrix(tensors[self.names["o"]])
         self.q_norm_f32 = self.k_norm_f32 = None
         if self.qk_norm:
             self.q_norm_w = tensors[self.q_norm_name]
@@ -167,15 +167,23 @@ class Attention(Mixer):
         self.sink = tensors[self.sink_name].float().contiguous() if self.sink_name else None
 
     def weight_bytes(self):
-        return (self.in_cols * self.hidden + self.hidden * self.n_q * self.dv) * self.rt.dtype.itemsize
+        return sum(self.rt.matrix_bytes(*shape) for shape in self.matrices())
+
+    def matrices(self):
+        return [(self.in_cols, self.hidden), (self.hidden, self.n_q * self.dv)]
 
     def scratch_bytes(self, max_tokens):
-        return max_tokens * (self.in_cols + self.n_q * self.dv) * self.rt.dtype.itemsize
+        return max_tokens * (self.in_cols + self.n_q * self.dv) * self.rt.dtype.itemsize + \
+            self.rt.token_scratch_bytes(max_tokens, self.hidden) + self.rt.token_scratch_bytes(max_tokens, self.n_q * self.dv)
 
     def load_transient_bytes(self):
         return self.in_cols * self.hidden * self.rt.dtype.itemsize       # q, k, v beside their stacked copy
 
     def cache_request(self):
+        if self.rt.cache_bits == 4:
+            if self.general:
+                raise ValueError("an attention layer of this form keeps its cache in the run dtype, not in 4 bits")
+            return PagedKV(self.n_kv, self.d, self.window, bits=4)
         return PagedKV(self.n_kv, self.d, self.window, value_head_dim=self.dv)
 
     def _out_proj(self, attn, hidden, then, fresh=False):

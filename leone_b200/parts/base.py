@@ -52,6 +52,8 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
+from ..cache import packed
+
 
 @dataclass(frozen=True)
 class WeightSpec:
@@ -93,6 +95,8 @@ class PagedKV:
     # summary whose last position is ``e`` lies in the page of ``e`` at ``(e % page_tokens) //
     # tokens_per_row``.
     tokens_per_row: int = 1
+    # 4: rows of ``head_dim`` (and as many value) elements in 4 bits (:mod:`leone_b200.cache.packed`); the pools hold bytes
+    bits: Optional[int] = None
 
     def resolved(self, run_dtype: torch.dtype) -> "PagedKV":
         lifetime = self.lifetime or ("window" if self.window else "full")
@@ -103,6 +107,14 @@ class PagedKV:
         vd = self.head_dim if self.value_head_dim is None else int(self.value_head_dim)
         if self.num_kv_heads <= 0 or self.head_dim <= 0 or vd < 0 or self.tokens_per_row <= 0:
             raise ValueError(f"a paged cache needs positive sizes, got {self}")
+        if self.bits is not None:
+            if self.bits != 4 or vd != self.head_dim or self.dtype is not None or self.tokens_per_row != 1 or \
+                    not packed.dim_ok(self.head_dim):
+                raise ValueError("a paged cache in 4 bits holds keys and values of one width, in groups of at most 64 that are "
+                                 f"multiples of 8, up to {packed.MAX_DIM}: not {self}")
+            width = packed.row_bytes(self.head_dim)
+            return PagedKV(self.num_kv_heads, width, self.window if lifetime == "window" else None, width, torch.uint8, lifetime,
+                           self.tag, 1, 4)
         return PagedKV(self.num_kv_heads, self.head_dim, self.window if lifetime == "window" else None,
                        vd, self.dtype or run_dtype, lifetime, self.tag, int(self.tokens_per_row))
 
@@ -193,13 +205,19 @@ class DeferredNorm:
 class Runtime:
     """What every part gets at construction: device, run dtype, kernels and scratch buffers."""
 
-    def __init__(self, device, dtype: torch.dtype, ops, max_tokens: int):
+    def __init__(self, device, dtype: torch.dtype, ops, max_tokens: int, cache_bits: Optional[int] = None,
+                 weight_bits: Optional[int] = None):
+        if cache_bits not in (None, 4) or weight_bits not in (None, 8):
+            raise ValueError(f"caches are held in the run dtype or in 4 bits, matrices in the run dtype or in 8 bits, "
+                             f"not in {cache_bits} and {weight_bits}")
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"run dtype must be float32 or bfloat16, got {dtype}")
         self.device = torch.device(device)
         self.dtype = dtype
         self.ops = ops
         self.max_tokens = max_tokens
+        self.cache_bits = cache_bits       # 4: mixers that can ask for their pages in 4 bits
+        self.weight_bits = weight_bits     # 8: parts that can keep their matrices in 8-bit integers
         self._buffers: Dict[str, torch.Tensor] = {}
         self._views: Dict[tuple, torch.Tensor] = {}
 
@@ -227,6 +245,27 @@ class Runtime:
         view = self._views[vkey] = buf[:rows]
         return view
 
+
+    def prepare_matrix(self, w: torch.Tensor, *bias):
+        """A part's matrix ``[out, in]`` (and bias) as its products take it: in the run dtype, or in 8 bits where the run asks for it."""
+        if self.weight_bits == 8:
+            from ..ops.int8 import quantize_matrix
+            return self.ops.prepare_matrix_int8(*quantize_matrix(w), *bias)
+        return self.ops.prepare_matrix(w, *bias)
+
+    def prepare_gate_up(self, gate: torch.Tensor, up: torch.Tensor, *biases):
+        if self.weight_bits == 8:
+            from ..ops.int8 import quantize_matrix
+            return self.ops.prepare_gate_up_int8(*quantize_matrix(gate), *quantize_matrix(up), *biases)
+        return self.ops.prepare_gate_up(gate, up, *biases)
+
+    def matrix_bytes(self, rows: int, cols: int) -> int:
+        """Bytes of a matrix that :meth:`prepare_matrix` keeps."""
+        return rows * cols + 4 * rows if self.weight_bits == 8 else rows * cols * self.dtype.itemsize
+
+    def token_scratch_bytes(self, max_tokens: int, width: int) -> int:
+        """Bytes of what the ops keep of a step's tokens for products with such matrices (codes and scales)."""
+        return max_tokens * (width + 4) if self.weight_bits == 8 else 0
 
     def flat_buffer(self, name: str, numel: int, dtype: torch.dtype, reserve: int = 0) -> torch.Tensor:
         """A scratch vector of at least ``numel`` elements under ``name`` (``reserve``: what to
@@ -263,6 +302,10 @@ class Part:
         """Bytes of scratch buffers this part asks the runtime for in a step of ``max_tokens``
         tokens (an estimate for the memory budget that is checked before anything is loaded)."""
         return 0
+
+    def matrices(self) -> List[Tuple[int, int]]:
+        """``(rows, cols)`` of the matrices that this part hands to :meth:`Runtime.prepare_matrix`, for the same budget."""
+        return []
 
     def load_transient_bytes(self) -> int:
         """Bytes ``load`` holds on top of the tensors it was given while it runs (a fused copy

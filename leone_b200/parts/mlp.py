@@ -28,14 +28,18 @@ class Mlp(FeedForward):
         return [WeightSpec(self.up_name, (self.inter, self.hidden)), WeightSpec(self.down_name, (self.hidden, self.inter))]
 
     def load(self, tensors):
-        self.w_up = self.rt.ops.prepare_matrix(tensors[self.up_name])
-        self.w_down = self.rt.ops.prepare_matrix(tensors[self.down_name])
+        self.w_up = self.rt.prepare_matrix(tensors[self.up_name])
+        self.w_down = self.rt.prepare_matrix(tensors[self.down_name])
 
     def weight_bytes(self):
-        return 2 * self.inter * self.hidden * self.rt.dtype.itemsize
+        return sum(self.rt.matrix_bytes(*shape) for shape in self.matrices())
+
+    def matrices(self):
+        return [(self.inter, self.hidden), (self.hidden, self.inter)]
 
     def scratch_bytes(self, max_tokens):
-        return max_tokens * self.inter * self.rt.dtype.itemsize
+        return max_tokens * self.inter * self.rt.dtype.itemsize + self.rt.token_scratch_bytes(max_tokens, self.hidden) + \
+            self.rt.token_scratch_bytes(max_tokens, self.inter)
 
     def forward(self, ctx, x, hidden):
         ops = self.rt.ops

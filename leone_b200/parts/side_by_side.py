@@ -68,6 +68,9 @@ class SideBySide(Mixer):
     def weight_bytes(self):
         return sum(part.weight_bytes() for _, part in self.branches if hasattr(part, "weight_bytes"))
 
+    def matrices(self):
+        return [shape for _, part in self.branches for shape in part.matrices()]
+
     def scratch_bytes(self, max_tokens):
         return sum(part.scratch_bytes(max_tokens) for _, part in self.branches)
 

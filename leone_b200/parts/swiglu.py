@@ -66,18 +66,22 @@ class SwiGLU(FeedForward):
     def load(self, tensors):
         if self.bias:
             gate_b, up_b, down_b = (tensors[self.bias_names[k]].float().contiguous() for k in ("gate", "up", "down"))
-            self.w_gate_up = self.rt.ops.prepare_gate_up(tensors[self.gate_name], tensors[self.up_name], gate_b, up_b)
-            self.w_down = self.rt.ops.prepare_matrix(tensors[self.down_name], down_b)
+            self.w_gate_up = self.rt.prepare_gate_up(tensors[self.gate_name], tensors[self.up_name], gate_b, up_b)
+            self.w_down = self.rt.prepare_matrix(tensors[self.down_name], down_b)
             return
-        self.w_gate_up = self.rt.ops.prepare_gate_up(tensors[self.gate_name], tensors[self.up_name])
-        self.w_down = self.rt.ops.prepare_matrix(tensors[self.down_name])
+        self.w_gate_up = self.rt.prepare_gate_up(tensors[self.gate_name], tensors[self.up_name])
+        self.w_down = self.rt.prepare_matrix(tensors[self.down_name])
 
     def weight_bytes(self):
-        return (2 * self.inter * self.hidden + self.hidden * self.inter) * self.rt.dtype.itemsize
+        return sum(self.rt.matrix_bytes(*shape) for shape in self.matrices())
+
+    def matrices(self):
+        return [(2 * self.inter, self.hidden), (self.hidden, self.inter)]
 
     def scratch_bytes(self, max_tokens):
         # the activation; a path without the fused epilogue also holds gate and up side by side
-        return max_tokens * 3 * self.inter * self.rt.dtype.itemsize
+        return max_tokens * 3 * self.inter * self.rt.dtype.itemsize + self.rt.token_scratch_bytes(max_tokens, self.hidden) + \
+            self.rt.token_scratch_bytes(max_tokens, self.inter)
 
     def load_transient_bytes(self):
         return 2 * self.inter * self.hidden * self.rt.dtype.itemsize       # gate and up beside their interleaved copy
