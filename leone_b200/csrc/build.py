@@ -42,7 +42,7 @@ MODULES: Dict[str, List[str]] = {
                "attention_mixed_heads.cu", "attention_mixed_heads_mma.cu", "gated_delta.cu", "gated_delta_mma.cu",
                "gated_linear_attention.cu", "gated_linear_attention_mma.cu", "ssd.cu", "ssd_mma.cu"],
     # pages in 4 bits (append, read, attention) and rows of tokens in 8 bits
-    "packed": ["cache4.cu", "quantize8.cu"],
+    "packed": ["cache4.cu", "attention4_decode.cu", "quantize8.cu"],
     # the entry point that allocates nothing (leone_static.h); it compiles attention_tiled.cu in
     "static": ["attention_decode_static.cu"],
     # the host side of the runtime (pages, block tables, step metadata, the scheduler's decisions,

@@ -597,10 +597,62 @@ class CudaOps:
         _need(n_q > 0 and n_q % n_kv == 0 and qkv.stride(1) == 1 and qkv.shape[1] >= n_q * d, "attention: query rows")
         if n == 0:
             return
+        # tokens [at, n) on the kernel of any size
+        at = self._attention4_tuned(ctx, qkv, out, n_q, n_kv, d, scale, window, cache)
+        if at < n:
+            self.launches += 1
+            _check(self.packed_calls.leone_attention4_any(
+                _dt(qkv.dtype), qkv[at:], qkv.stride(0), out[at:], out.stride(0), kp, vp, bt, width, ctx.seq_of_token[at:],
+                ctx.positions[at:], n - at, n_q, n_kv, d, float(scale), int(window or 0), page_tokens, pages, rows, ctx.status,
+                self._stream()), "attention (4 bits)")
+
+    def _attention4_tuned(self, ctx, qkv, out, n_q, n_kv, d, scale, window, cache) -> int:
+        """The bfloat16 kernels for head sizes 64 and 128: how many of the step's tokens they took (from the front)."""
+        bt = cache.block_table
+        if (qkv.dtype != torch.bfloat16 or d not in (64, 128) or getattr(ctx, "q_start", None) is None or qkv.stride(0) % 8
+                or any(t.data_ptr() % 16 for t in (qkv, out, cache.k_pool, cache.v_pool)) or ctx.n_seqs > 65535 or n_q > 65535):
+            return 0
+        order = getattr(ctx, "seq_order", None)
+        if ctx.decode_only:
+            self._attention4_decode(qkv, out, n_q, n_kv, d, scale, window, cache, ctx, ctx.n_seqs, int(ctx.max_ctx_len), order)
+            return qkv.shape[0]
+        lead = self._leading_single_rows(ctx)
+        if lead:
+            self._attention4_decode(qkv, out, n_q, n_kv, d, scale, window, cache, ctx, lead, int(ctx.ctx_lens[:lead].max()), order)
+        return lead
+
+    force_decode4_splits = 0               # > 0: every decode attention over pages in 4 bits splits its keys this many ways
+
+    @staticmethod
+    def choose_decode4_splits(n_seqs: int, n_kv: int, g: int, keys: int):
+        """``(splits, in a cluster)`` of a decode attention over pages in 4 bits: ``keys`` are the most that a sequence reads.  Two blocks an
+        SM, though an SM holds three: what a block costs before its first and after its last key is more than the third gives (one sequence,
+        8 cached heads of 128: 8,192 keys 16.5 us with 8 to 32 splits, 18.5 with 48; 40,960 keys 26.8 with 32, 28.7 with 48; 8
+        sequences of 2,048 16.5 with 4, 18.6 with 6; 24 of 3,000 with 2 heads of 64 14.4 with 8, 16.5 with 12).  A split keeps 128 keys.  Up
+        to 8 merge in a cluster; a few more than that are not worth scratch and a second kernel."""
+        s = max(1, min(64, 2 * 148 // (n_seqs * n_kv * -(-g // 16)), keys // 128))
+        if 8 < s < 12:
+            s = 8
+        return s, 1 < s <= 8
+
+    def _attention4_decode(self, qkv, out, n_q, n_kv, d, scale, window, cache, ctx, n_seqs, max_ctx, order) -> None:
+        """Sequences ``0 .. n_seqs - 1`` of the step, with one token each; ``order``: these, the longest first."""
+        calls, bt = self.packed_calls, cache.block_table
+        if order is not None and order.numel() != n_seqs:
+            raise KernelError(f"an order of {order.numel()} sequences for {n_seqs}")
+        splits, in_cluster = self.choose_decode4_splits(n_seqs, n_kv, n_q // n_kv, min(max_ctx, window) if window else max_ctx)
+        if self.force_decode4_splits:
+            splits = self.force_decode4_splits
+            in_cluster = 1 < splits <= 8
+        scratch = None
+        if splits > 1 and not in_cluster:
+            scratch = self._scratch("attention4", -(-n_seqs * n_q * splits * (d + 2) // 1024), 1024, torch.float32)
+            self.launches += 1
         self.launches += 1
-        _check(self.packed_calls.leone_attention4_any(
-            _dt(qkv.dtype), qkv, qkv.stride(0), out, out.stride(0), kp, vp, bt, width, ctx.seq_of_token, ctx.positions, n, n_q, n_kv, d,
-            float(scale), int(window or 0), page_tokens, pages, rows, ctx.status, self._stream()), "attention (4 bits)")
+        _check(calls.leone_attention4_decode(
+            qkv, qkv.stride(0), out, out.stride(0), cache.k_pool, cache.v_pool, bt, bt.shape[1], ctx.q_start, ctx.ctx_len, n_seqs,
+            n_q, n_kv, d, float(scale), int(window or 0), cache.page_tokens, cache.k_pool.shape[0], splits, 1 if in_cluster else 0,
+            order, scratch, ctx.status, self._stream()), "attention (4 bits, decode)")
 
     def can_fuse_decode(self, ctx, qkv, n_q, n_kv, d) -> bool:
         """True if the attention kernel can do the q/k norm, rotation and cache write itself

@@ -228,6 +228,63 @@ def test_attention_any_size(ops_of, dtype, n_q, n_kv, d, lens, page, window):
     assert ((out - want).abs() <= _bounds(dtype, step, d, n_q, want, top_s, top_v, False)).all()
 
 
+DECODE = [
+    # n_q, n_kv, d, lens, page, window
+    (16, 8, 128, [(1, 511)], 16, 0),
+    (32, 8, 128, [(1, 0), (1, 15), (1, 16), (1, 17), (1, 700)], 16, 0),
+    (14, 2, 64, [(1, 100), (1, 1100), (1, 3)], 16, 500),
+    (12, 1, 128, [(1, 300), (1, 64)], 48, 0),                                 # two tiles of heads
+    (40, 2, 64, [(1, 300), (1, 1)], 16, 0),                                   # two groups of heads
+    (5, 5, 128, [(1, 200)] * 40, 32, 33),
+    (3, 1, 64, [(1, 2047)], 16, 16),
+    (8, 1, 128, [(1, 9000)], 16, 0),
+    (64, 8, 128, [(1, 130 + 7 * i) for i in range(20)], 16, 0),
+]
+
+
+@pytest.mark.parametrize("splits", [0, 1, 2, 7, 8, 9, 33, 64])
+@pytest.mark.parametrize("n_q,n_kv,d,lens,page,window", DECODE)
+def test_attention_decode(ops_of, n_q, n_kv, d, lens, page, window, splits):
+    ops = ops_of(BF16)
+    ops.force_decode4_splits = splits
+    try:
+        step, qkv, pools, out, want, top_s, top_v = _attention_case(ops, BF16, n_q, n_kv, d, lens, page, window, seed=d + n_q)
+    finally:
+        ops.force_decode4_splits = 0
+    assert ((out - want).abs() <= _bounds(BF16, step, d, n_q, want, top_s, top_v, True)).all()
+
+
+def test_attention_decode_in_an_order_and_in_a_graph(ops_of):
+    ops = ops_of(BF16)
+    lens = [(1, 37 * i) for i in range(50)]
+    step, qkv, pools, out, want, top_s, top_v = _attention_case(ops, BF16, 16, 8, 128, lens, 16, 0)
+    view = step.view(*pools)
+    step.ctx.seq_order = torch.arange(49, -1, -1, dtype=torch.int32, device=DEV)
+    again = torch.zeros((50, 16 * 128), dtype=BF16, device=DEV)
+    ops.attention(step.ctx, qkv, again, 16, 8, 128, 128 ** -0.5, None, view)
+    assert torch.equal(again.double().view_as(out), out)
+    graph, got = torch.cuda.CUDAGraph(), torch.zeros_like(again)
+    with torch.cuda.graph(graph):
+        ops.attention(step.ctx, qkv, got, 16, 8, 128, 128 ** -0.5, None, view)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        assert torch.equal(got, again)
+    step.ctx.seq_order = step.ctx.seq_order[:3]
+    with pytest.raises(KernelError, match="order"):
+        ops.attention(step.ctx, qkv, again, 16, 8, 128, 128 ** -0.5, None, view)
+
+
+def test_attention_decode_reports_a_bad_page(ops_of):
+    ops = ops_of(BF16)
+    for bad in (-1, 10 ** 6):
+        step, qkv, pools, *_ = _attention_case(ops, BF16, 4, 2, 128, [(1, 200), (1, 90)], 16, 0)
+        step.table[0, 3] = bad
+        out = torch.zeros((2, 4 * 128), dtype=BF16, device=DEV)
+        ops.attention(step.ctx, qkv, out, 4, 2, 128, 0.1, None, step.view(*pools))
+        assert step.ctx.status.tolist() == [2, 0, bad if bad > 0 else -1, 48]
+
+
 def test_attention_refusals(ops_of):
     ops = ops_of(BF16)
     step = Step([(1, 20)], 16, DEV)
