@@ -43,6 +43,8 @@
 // is bounded; a wait that runs out sets the status word and the block leaves.  Tensor memory:
 // S_0 at column 0, S_1 at 128 (P_j over columns 0-31 and 64-95 of S_j), O_0 at 256, O_1 at 384
 // (all 512 columns: one block per SM).
+#include <cuda_fp16.h>
+#include "cache4.cuh"
 #include "tc_common.cuh"
 
 namespace leone {
@@ -57,8 +59,9 @@ constexpr int kTileThreads = kTileWarps * 32;
 constexpr int kMmaWarp = 2 * kTileWarps;
 constexpr int kLoadWarp0 = kMmaWarp + 1;   // two warps gather keys, the next two values
 constexpr int kStreamThreads = 64;         // threads that gather one kind of tile (a thread per two key rows)
-constexpr int kLoadThreads = 2 * kStreamThreads;
-constexpr int kBlockThreads = (kLoadWarp0 + 4) * 32;
+// Pages in 4 bits: twice as many, who also convert them (2,048 tokens behind 6,144 on 32 and 8 heads of 128: FIG us; 435 with 64 threads)
+constexpr int stream_threads(int form) { return form == 3 ? 128 : kStreamThreads; }
+constexpr int block_threads(int form) { return kLoadWarp0 * 32 + 2 * stream_threads(form); }
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleAt = 8.0f;         // the running maximum moves when a tile's exceeds it by this (log2)
 
@@ -195,21 +198,84 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <int D> constexpr int smem_bytes() {
+// Pages in 4 bits (cache4.cuh; kernel form 3, ordinary softmax).  A tile's keys, and its values, are eight units that the TMA copies
+// into shared memory as they lie in their pages, one tile ahead; the gathering warps turn them into the 16-bit operand tiles: a word of
+// codes is the 16-byte piece of its row, a pair of codes becomes an offset + c by AND-OR, c by a subtraction and z + s c by one FMA, which
+// rounds once.
+//
+// Values become bfloat16, and so do the weights, as in the other forms.  Keys become fp16, and queries are fp16 too, which is exact:
+// z + s c has 12 significant bits and more, and rounded to the 8 of bfloat16 its error in the scores was most of the output's (8,192
+// keys with a spread of scores of 3: 0.0075 of the output's norm, 0.0026 with the 11 of fp16).  For fp16's range a query's row is
+// multiplied by a power of two that brings its largest element to 2^7 .. 2^8, and a tile of keys by one that brings its largest value
+// below 2^15; the row's and the tile's power are taken out with the scale of the scores.
+//
+// A value that is NaN must not reach rows that do not see its key (the product has 0 x NaN for them): such a group is stored as zeros
+// and kept in a list of keys and groups, and at the end the rows that see one of them become NaN in that group's columns.  What does not
+// fit into the list widens a range of keys, which counts as a whole.
+constexpr int kTileUnits = kKeys / cache4::kUnit;
+constexpr int kOddKeys = 32;
+struct OddValues {
+  int count;
+  int key[kOddKeys];              // key * 2 + group
+  int lo[2], hi[2];               // the range of further keys, per group
+  unsigned units[2];              // of the tile that lands, keys and values: the units that have a page
+  int largest[4];                 // of the four warps that gather keys: the largest exponent of their rows
+  float key_power[4];             // 2^e of tile t % 4: its keys are stored times 2^-e
+  float query_power[2][kRows];    // the same of a row of queries
+};
+
+template <int D, bool kPacked> constexpr int smem_bytes() {
   // two Q tiles, two K and two V tiles, row sources [2 kinds][2 buffers][128], barriers; 1024 for alignment
-  return 2 * kRows * D * 2 + 4 * kKeys * D * 2 + 2 * 2 * kKeys * 8 + 16 * 8 + 1024;
+  return 2 * kRows * D * 2 + 4 * kKeys * D * 2 + 2 * 2 * kKeys * 8 + 18 * 8 + 1024 +
+         (kPacked ? 2 * kKeys * cache4::row_bytes(D) : 0);
+}
+
+// 2^e for e in -126 .. 127.
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+// The exponent of |v|, -126 at least (128: an infinity or NaN).
+__device__ __forceinline__ int exponent_of(float v) { return max((int)(__float_as_uint(v) >> 23 & 255u) - 127, -126); }
+
+// Four words of codes of a row (place q of its 16-byte pieces, at `raw`) become their chunks of the operand tile at `tile`; sz0, sz1:
+// the row's groups' scales (low half) and offsets, in bfloat16 for values and fp16 for keys.
+template <int D, bool kValues>
+__device__ __forceinline__ void unpack_quad(const uint8_t* raw, uint32_t tile, int row, int q, uint32_t sz0, uint32_t sz1) {
+  const uint4 raw4 = *reinterpret_cast<const uint4*>(raw);
+  const uint32_t w[4] = {raw4.x, raw4.y, raw4.z, raw4.w};
+  constexpr uint32_t kOffset = kValues ? 0x43004300u : 0x64006400u;        // 128 in bfloat16, 1024 in fp16: what follows is c
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // which word of the row stands in place 4 q + i (cache4.cuh)
+    const int g = D == 64 ? 0 : (kValues ? i & 1 : i >> 1);
+    const int chunk = D == 64 ? 4 * q + i : 8 * g + 2 * q + (kValues ? i >> 1 : i & 1);
+    const uint32_t sz = g == 0 ? sz0 : sz1;
+    const uint32_t s2 = __byte_perm(sz, sz, 0x1010), z2 = __byte_perm(sz, sz, 0x3232);
+    uint32_t out[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t c = ((w[i] >> (4 * j)) & 0x000f000fu) | kOffset;
+      uint32_t v;
+      if constexpr (kValues)
+        asm("{\n\t.reg .b32 t;\n\tsub.rn.bf16x2 t, %1, %2;\n\tfma.rn.bf16x2 %0, t, %3, %4;\n\t}" : "=r"(v) : "r"(c), "r"(kOffset), "r"(s2), "r"(z2));
+      else
+        asm("{\n\t.reg .b32 t;\n\tsub.rn.f16x2 t, %1, %2;\n\tfma.rn.f16x2 %0, t, %3, %4;\n\t}" : "=r"(v) : "r"(c), "r"(kOffset), "r"(s2), "r"(z2));
+      out[j] = v;
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + swizzled(row, chunk)), "r"(out[0]), "r"(out[1]), "r"(out[2]),
+                 "r"(out[3])
+                 : "memory");
+  }
 }
 
 // kForm 0: the reference's layer; the rules are then compile-time constants and the kernel is
 // the one it was before they became parameters.  1: the rules are run-time fields.  2: pooled blocks
-// before a window (ordinary softmax; `pooled` is read in this form only).
+// before a window (ordinary softmax; `pooled` is read in this form only).  3: pages in 4 bits.
 template <int D, int kForm>
-__global__ void __launch_bounds__(kBlockThreads)
+__global__ void __launch_bounds__(block_threads(kForm))
 attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row_stride,
                                   __nv_bfloat16* __restrict__ out, int out_stride, PagedArgs pa,
                                   const int* __restrict__ q_start, const int* __restrict__ ctx_len, int n_q,
                                   float scale, int window, Rules rules_in, Pooled pooled, int query_tiles, int* status) {
-  constexpr bool kRules = kForm == 1, kPooled = kForm == 2;
+  constexpr bool kRules = kForm == 1, kPooled = kForm == 2, kPacked = kForm == 3;
   struct {
     int weights, chunk;
     const float* bias;
@@ -232,6 +298,10 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
   // tensor core -> softmax: S_j is complete (and every product issued before it);
   // softmax -> tensor core: P_j is written; tensor core -> softmax: the last O_j is complete
   const uint32_t bar_s = bars + 72, bar_p = bars + 88, bar_o = bars + 104;
+  // pages in 4 bits: the units of a tile of keys, or values, have landed in raw_units
+  const uint32_t bar_raw = bars + 120;
+  uint8_t* raw_units = reinterpret_cast<uint8_t*>(row_src + 4 * kKeys) + 18 * 8;
+  __shared__ OddValues odd;
   __shared__ uint32_t tmem_holder;
   __shared__ int gave_up;
   __shared__ float halves[2][2][2][kRows];              // [query tile][tile parity][column half][row]: maxima, then sums
@@ -241,13 +311,19 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
     gave_up = 0;
     mbar_init(bar_q, 2 * kTileWarps);                   // every softmax warp brings its share of its query tile
     for (int b = 0; b < 2; ++b) {
-      mbar_init(bar_k_full + 8 * b, kStreamThreads / 32);
-      mbar_init(bar_v_full + 8 * b, kStreamThreads / 32);
+      mbar_init(bar_k_full + 8 * b, stream_threads(kForm) / 32);
+      mbar_init(bar_v_full + 8 * b, stream_threads(kForm) / 32);
       mbar_init(bar_k_free + 8 * b, 1);
       mbar_init(bar_v_free + 8 * b, 1);
       mbar_init(bar_s + 8 * b, 1);
       mbar_init(bar_p + 8 * b, kTileWarps);
       mbar_init(bar_o + 8 * b, 1);
+      if constexpr (kPacked) mbar_init(bar_raw + 8 * b, 1);
+    }
+    if constexpr (kPacked) {
+      odd.count = 0;
+      odd.lo[0] = odd.lo[1] = 0x7fffffff;
+      odd.hi[0] = odd.hi[1] = -1;
     }
     mbar_fence_init();
   }
@@ -290,7 +366,8 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
     if (warp == kMmaWarp) {
       // ---------------- the warp that issues the tensor-core work ----------------
       if (elect_one()) {
-        constexpr uint32_t idesc_s = instr_desc_bf16(kRows, kKeys);
+        // (without the two bits that say bfloat16: fp16 operands)
+        constexpr uint32_t idesc_s = instr_desc_bf16(kRows, kKeys) & (kPacked ? ~((1u << 7) | (1u << 10)) : ~0u);
         constexpr uint32_t idesc_o = instr_desc_bf16_b_mn(kRows, D);
         auto issue_s = [&](int j, int t) {     // S_j = Q_j . K(t)^T
           const uint32_t q_s = q_t + j * kTileBytes, k_s = k_t + (t & 1) * kTileBytes;
@@ -338,6 +415,123 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
           umma_commit(bar_v_free + 8 * (t & 1));
           if (next) umma_commit(bar_k_free + 8 * ((t + 1) & 1));
         }
+      }
+    } else if (kPacked && warp >= kLoadWarp0) {
+      // ---------------- the warps that gather the tiles from pages in 4 bits ----------------
+      constexpr int kUnitBytes = cache4::kUnit * cache4::row_bytes(D), kQuads = D / 32, G = D / 64, kStream = stream_threads(3);
+      const int lt = tid - kLoadWarp0 * 32;
+      const bool values = lt >= kStream;
+      const int st = lt & (kStream - 1);
+      const uint8_t* pool = reinterpret_cast<const uint8_t*>(values ? pa.v_pool : pa.k_pool);
+      const uint32_t tiles = values ? v_t : k_t;
+      const uint32_t bar_full = values ? bar_v_full : bar_k_full, bar_free = values ? bar_v_free : bar_k_free;
+      const uint32_t landed = bar_raw + (values ? 8 : 0);
+      uint8_t* raw = raw_units + (values ? kTileUnits * kUnitBytes : 0);
+      const int bar_id = values ? 3 : 2;
+      // The stream's first warp asks for tile t's units that hold a key of [k_lo, k_hi); called when nobody reads the tile before any more.
+      auto request = [&](int t) {
+        const int key = tile0 + t * kKeys + lane * cache4::kUnit;
+        long long at = -1;
+        if (t < n_tiles && lane < kTileUnits && key < k_hi && key + cache4::kUnit > k_lo) {
+          const int blk = key / pa.page_tokens;
+          const int page = blk < pa.table_width ? pa.block_table[(size_t)seq * pa.table_width + blk] : -1;
+          if (page < 0 || page >= pa.num_pages) set_status(status, kBadPage, q0 + tok0, page, key);
+          else at = cache4::unit_at(page, pa.n_kv, kvh, pa.page_tokens, key - blk * pa.page_tokens, D);
+        }
+        const unsigned have = __ballot_sync(0xffffffffu, at >= 0);
+        if (t >= n_tiles) return;
+        if (lane == 0) {
+          odd.units[values] = have;
+          mbar_expect_tx(landed, __popc(have) * kUnitBytes);
+        }
+        __syncwarp();
+        if (at >= 0) bulk_load(smem_u32(raw) + lane * kUnitBytes, pool + at, kUnitBytes, landed);
+      };
+      if (st < 32) request(0);
+      bool ok_all = true;
+      for (int t = 0; t < n_tiles; ++t) {
+        if (ok_all && !mbar_wait_long(landed, t & 1, giveup)) ok_all = false;
+        if (t >= 2 && ok_all && !mbar_wait_long(bar_free + 8 * (t & 1), ((t >> 1) - 1) & 1, giveup)) ok_all = false;
+        ok_all = __all_sync(0xffffffffu, ok_all);
+        const unsigned have = ok_all ? odd.units[values] : 0u;
+        const uint32_t tile = tiles + (t & 1) * kTileBytes;
+        const int key0 = tile0 + t * kKeys;
+        // every row of the tile is a key to be read: the same for all threads
+        const bool clean = have == (1u << kTileUnits) - 1 && key0 >= k_lo && key0 + kKeys <= k_hi;
+        float down = 1.f;
+        if (!values) {
+          // the tile's largest |z|, |z + 15 s|, a row a thread; a NaN does not count
+          int top = -126;
+          if ((have >> (st / cache4::kUnit) & 1) && key0 + st >= k_lo && key0 + st < k_hi) {
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const uint32_t sz = *reinterpret_cast<const uint32_t*>(raw + st / cache4::kUnit * kUnitBytes +
+                                                                     cache4::scale_at(st % cache4::kUnit, g, D));
+              const float z = cache4::offset_of(sz), most = fmaxf(fabsf(z), fabsf(fmaf(15.f, cache4::scale_of(sz), z)));
+              if (most < INFINITY) top = max(top, exponent_of(most));
+            }
+          }
+          top = __reduce_max_sync(0xffffffffu, top);
+          if (lane == 0) odd.largest[st >> 5] = top;
+          named_barrier_sync(bar_id, kStream);
+          top = max(max(odd.largest[0], odd.largest[1]), max(odd.largest[2], odd.largest[3]));
+          const int e = min(max(top - 13, -126), 126);     // below 2^15, with what rounding adds
+          down = power_of_two(-e);
+          if (st == 0) odd.key_power[t & 3] = power_of_two(e);
+        }
+        // thread st takes piece st % kQuads of rows st / kQuads, + kStream / kQuads, ..: always the same row of a unit
+        constexpr int kStep = kStream / kQuads;
+        static_assert(kStep % cache4::kUnit == 0, "a thread's rows are the same row of units");
+        const int q = st % kQuads, row0 = st / kQuads, tt = row0 % cache4::kUnit, vr = cache4::value_row(tt);
+        const int piece = values ? vr * (D / 2) + (G == 2 ? q ^ (vr & 2) : q) * 16 : tt * (D / 2) + q * 16;
+        const uint8_t* unit = raw + row0 / cache4::kUnit * kUnitBytes;
+#pragma unroll 2
+        for (int row = row0; row < kKeys; row += kStep, unit += kStep / cache4::kUnit * kUnitBytes) {
+          bool zero0 = false, zero1 = false;
+          if (!clean) zero0 = zero1 = !(have >> (row / cache4::kUnit) & 1) || key0 + row < k_lo || key0 + row >= k_hi;
+          uint32_t sz0, sz1 = 0;
+          if constexpr (G == 2) {
+            const uint2 both = *reinterpret_cast<const uint2*>(unit + cache4::scale_at(tt, 0, D));
+            sz0 = both.x;
+            sz1 = both.y;
+          } else {
+            sz0 = *reinterpret_cast<const uint32_t*>(unit + cache4::scale_at(tt, 0, D));
+          }
+          if (values) {
+            // (z + 15 s is the largest value; what would not be a bfloat16 number counts with the NaN)
+            const bool odd0 = !(fabsf(fmaf(15.f, cache4::scale_of(sz0), cache4::offset_of(sz0))) <= 3.3895e38f);
+            const bool odd1 = G == 2 && !(fabsf(fmaf(15.f, cache4::scale_of(sz1), cache4::offset_of(sz1))) <= 3.3895e38f);
+            if ((odd0 || odd1) && !zero0) {
+              if (q == 0) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                  if (!(g == 0 ? odd0 : odd1)) continue;
+                  const int at = atomicAdd(&odd.count, 1);
+                  if (at < kOddKeys) {
+                    odd.key[at] = (key0 + row) * 2 + g;
+                  } else {
+                    atomicMin(&odd.lo[g], key0 + row);
+                    atomicMax(&odd.hi[g], key0 + row);
+                  }
+                }
+              }
+              zero0 |= odd0;
+              zero1 |= odd1;
+            }
+            // a zero group: codes, scale and offset 0
+            unpack_quad<D, true>(unit + piece, tile, row, q, zero0 ? 0u : sz0, zero1 ? 0u : sz1);
+          } else {
+            auto as_fp16 = [&](uint32_t sz) {
+              const __half2 v = __floats2half2_rn(cache4::scale_of(sz) * down, cache4::offset_of(sz) * down);
+              return *reinterpret_cast<const uint32_t*>(&v);
+            };
+            unpack_quad<D, false>(unit + piece, tile, row, q, zero0 ? 0u : as_fp16(sz0), G == 1 || zero1 ? 0u : as_fp16(sz1));
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        named_barrier_sync(bar_id, kStream);             // the landed units are read; the next tile's may take their place
+        if (lane == 0) mbar_arrive(bar_full + 8 * (t & 1));
+        if (st < 32 && ok_all) request(t + 1);
       }
     } else if (warp >= kLoadWarp0) {
       // ---------------- the warps that gather the tiles ----------------
@@ -451,14 +645,41 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
           const bool ok = tl < tq && token < q_len;
           const __nv_bfloat16* src =
               qkv + (size_t)(q0 + (ok ? token : 0)) * row_stride + (size_t)(kvh * g + hh) * D + ch * 8;
-          cp_async16(q_t + j * kTileBytes + swizzled(r, ch), src, ok);
+          if constexpr (kPacked) {
+            // as fp16, the row's largest element in 2^7 .. 2^8; the row's chunks are in neighbouring lanes
+            uint4 raw4 = make_uint4(0, 0, 0, 0);
+            if (ok) raw4 = *reinterpret_cast<const uint4*>(src);
+            const uint32_t w[4] = {raw4.x, raw4.y, raw4.z, raw4.w};
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+#pragma unroll
+            for (int o = 1; o < kChunks; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int e = top > 0.f && top < INFINITY ? min(max(exponent_of(top) - 7, -126), 126) : 0;
+            const float by = power_of_two(-e);
+            if (ch == 0) odd.query_power[j][r] = power_of_two(e);
+            uint32_t out4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const __half2 v = __floats2half2_rn(__uint_as_float(w[i] << 16) * by, __uint_as_float(w[i] & 0xffff0000u) * by);
+              out4[i] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(q_t + j * kTileBytes + swizzled(r, ch)), "r"(out4[0]),
+                         "r"(out4[1]), "r"(out4[2]), "r"(out4[3])
+                         : "memory");
+          } else {
+            cp_async16(q_t + j * kTileBytes + swizzled(r, ch), src, ok);
+          }
         }
+        if constexpr (kPacked) named_barrier_sync(bar_id, kTileThreads);      // the rows' powers are there
         cp_async_commit();
         cp_async_wait<0>();
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_q);
       }
+      const float row_sl2 = kPacked && nj > 0 ? sl2 * odd.query_power[j][row] : sl2;
       for (int t = 0; t < nj; ++t) {
         const bool block_tile = kPooled && t < nbt;
         const int tk = t - nbt;                                   // the tile's number among the token tiles
@@ -467,6 +688,7 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
         // S_j(t) is complete, and so is PV_j(t - 1): O_j is at rest until this tile's go-ahead
         if (ok_all && !mbar_wait_long(bar_s + 8 * j, t & 1, giveup)) ok_all = false;
         tc_fence_after();
+        const float tile_sl2 = kPacked ? row_sl2 * odd.key_power[t & 3] : row_sl2;
         // A tile that every row of this query tile sees whole needs no masking (the same for all
         // threads, so the branch is uniform; rows that stand for no token compute on zeros and
         // are never stored).
@@ -510,7 +732,7 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
             }
           }
         }
-        float tile_max = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sl2;    // the scale is positive; -inf stays -inf
+        float tile_max = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * tile_sl2;    // the scale is positive; -inf stays -inf
         halves[j][t & 1][half][row] = tile_max;
         named_barrier_sync(bar_id, kTileThreads);        // the two halves of every row's maximum
         tile_max = fmaxf(tile_max, halves[j][t & 1][half ^ 1][row]);
@@ -548,7 +770,7 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
         auto to_p = [&](const uint32_t* r, int c) {
           float x[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = fmaf(__uint_as_float(r[i]), sl2, shift);
+          for (int i = 0; i < 16; ++i) x[i] = fmaf(__uint_as_float(r[i]), tile_sl2, shift);
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] = ex2(x[i]);
           if (rules.weights == 2) {                      // uniform: 1 / (1 + 2^-(score + bias))
@@ -601,7 +823,19 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
         if (rules.weights == 1) l_row += ex2(m_run == -INFINITY ? 0.f : -m_run);      // the silent member's share
         if (ok_all && !mbar_wait_long(bar_o + 8 * j, 0, giveup)) ok_all = false;
         tc_fence_after();
-        const float inv = (rules.weights == 2 ? 1.f : (l_row > 0.f ? 1.f / l_row : 0.f)) * (kPooled ? pooled.out_scale : 1.f);
+        float inv = (rules.weights == 2 ? 1.f : (l_row > 0.f ? 1.f / l_row : 0.f)) * (kPooled ? pooled.out_scale : 1.f);
+        if constexpr (kPacked) {
+          const int count = odd.count;                     // (almost always 0)
+          if (count > 0 && my_pos >= 0) {
+            const int g = D == 64 ? 0 : half, from = window > 0 ? max(0, my_pos - window + 1) : 0;
+            bool sees = from <= odd.hi[g] && my_pos >= odd.lo[g];
+            for (int i = 0; i < min(count, kOddKeys); ++i) {
+              const int key = odd.key[i] >> 1;
+              sees |= (odd.key[i] & 1) == g && key <= my_pos && key >= from;
+            }
+            if (sees) inv = NAN;
+          }
+        }
         const bool store = ok_all && my_pos >= 0;
         const int hh = row - my_tl * g;
         __nv_bfloat16* dst = out + (size_t)(q0 + lo + (store ? my_tl : 0)) * out_stride + (size_t)(kvh * g + hh) * D +
@@ -633,6 +867,11 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
   tc_fence_before();
   __syncthreads();
   if (gave_up && tid == 0) set_status(status, kWaitTimeout, blockIdx.x, 2);
+  if (kPacked && gave_up) {                               // units that are still on their way land before the block's memory goes away
+    const long long since = clock64();
+    while (clock64() - since < 200000) {}
+    __syncthreads();
+  }
   if (warp == kMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tmem_base, kTmemCols);
@@ -646,7 +885,7 @@ int launch_form(const __nv_bfloat16* qkv, int row_stride, __nv_bfloat16* out, in
   static bool configured = false;
   if (!configured) {
     cudaError_t e = cudaFuncSetAttribute(attention_prefill_pingpong_kernel<D, kForm>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D>());
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D, kForm == 3>());
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
@@ -664,7 +903,7 @@ int launch_form(const __nv_bfloat16* qkv, int row_stride, __nv_bfloat16* out, in
   const long long tiles = (long long)((max_q_len + tq - 1) / tq) * pa.n_kv * n_seqs;
   const int query_tiles = tiles <= sms ? 1 : 2;
   dim3 grid(((max_q_len + query_tiles * tq - 1) / (query_tiles * tq)) * pa.n_kv, 1, n_seqs);
-  return launch_kernel(attention_prefill_pingpong_kernel<D, kForm>, grid, dim3(kBlockThreads), smem_bytes<D>(), stream,
+  return launch_kernel(attention_prefill_pingpong_kernel<D, kForm>, grid, dim3(block_threads(kForm)), smem_bytes<D, kForm == 3>(), stream,
                        qkv, row_stride, out, out_stride, pa, q_start, ctx_len, n_q, scale, window, rules, pooled, query_tiles,
                        status);
 }
@@ -758,4 +997,26 @@ extern "C" int leone_attention_prefill_pingpong(const void* qkv, int row_stride,
   return leone_attention_prefill_pingpong_rules(qkv, row_stride, out, out_stride, k_pool, v_pool, block_table,
                                                 table_width, q_start, ctx_len, n_seqs, max_q_len, n_q, n_kv, d, scale,
                                                 window, 0, 0, nullptr, page_tokens, num_pages, status, stream);
+}
+
+// The same over pages in 4 bits (cache4.cuh; page_tokens a multiple of 16).
+extern "C" int leone_attention4_prefill(const void* qkv, int row_stride, void* out, int out_stride, const void* k_pool,
+                                        const void* v_pool, const int* block_table, int table_width, const int* q_start,
+                                        const int* ctx_len, int n_seqs, int max_q_len, int n_q, int n_kv, int d, float scale, int window,
+                                        int page_tokens, int num_pages, int* status, cudaStream_t stream) {
+  if (n_seqs <= 0 || max_q_len <= 0) return 0;
+  if ((d != 64 && d != 128) || !(scale > 0.f) || window < 0) return kRefusedSize;
+  if (n_q <= 0 || n_kv <= 0 || n_q % n_kv != 0 || n_q / n_kv > pingpong::kRows) return kRefusedSize;
+  if (page_tokens <= 0 || page_tokens % cache4::kUnit != 0 || table_width <= 0 || n_seqs > 65535) return kRefusedSize;
+  if (row_stride % 8 != 0 || out_stride % 8 != 0) return kRefusedAlignment;
+  if (((uintptr_t)qkv | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return kRefusedAlignment;
+  const pingpong::PagedArgs pa{(const __nv_bfloat16*)k_pool, (const __nv_bfloat16*)v_pool, block_table, table_width,
+                               page_tokens, num_pages, n_kv};
+  const pingpong::Rules rules{0, 0, nullptr};
+  const pingpong::Pooled none{nullptr, nullptr, nullptr, 0, 0, 0, 0, 1.f};
+  if (d == 64)
+    return pingpong::launch_form<64, 3>((const __nv_bfloat16*)qkv, row_stride, (__nv_bfloat16*)out, out_stride, pa, q_start, ctx_len,
+                                        n_seqs, n_q, max_q_len, scale, window, rules, none, status, stream);
+  return pingpong::launch_form<128, 3>((const __nv_bfloat16*)qkv, row_stride, (__nv_bfloat16*)out, out_stride, pa, q_start, ctx_len,
+                                       n_seqs, n_q, max_q_len, scale, window, rules, none, status, stream);
 }

@@ -609,7 +609,7 @@ class CudaOps:
     def _attention4_tuned(self, ctx, qkv, out, n_q, n_kv, d, scale, window, cache) -> int:
         """The bfloat16 kernels for head sizes 64 and 128: how many of the step's tokens they took (from the front)."""
         bt = cache.block_table
-        if (qkv.dtype != torch.bfloat16 or d not in (64, 128) or getattr(ctx, "q_start", None) is None or qkv.stride(0) % 8
+        if (self.fast is None or qkv.dtype != torch.bfloat16 or d not in (64, 128) or getattr(ctx, "q_start", None) is None or qkv.stride(0) % 8
                 or any(t.data_ptr() % 16 for t in (qkv, out, cache.k_pool, cache.v_pool)) or ctx.n_seqs > 65535 or n_q > 65535):
             return 0
         order = getattr(ctx, "seq_order", None)
@@ -619,7 +619,15 @@ class CudaOps:
         lead = self._leading_single_rows(ctx)
         if lead:
             self._attention4_decode(qkv, out, n_q, n_kv, d, scale, window, cache, ctx, lead, int(ctx.ctx_lens[:lead].max()), order)
-        return lead
+        if n_q // n_kv > 128 or not scale > 0:
+            return lead
+        q_len = int(ctx.q_lens[lead:].max()) if lead else int(ctx.max_q_len)
+        self.launches += 1
+        _check(self.fast.calls.leone_attention4_prefill(
+            qkv, qkv.stride(0), out, out.stride(0), cache.k_pool, cache.v_pool, bt[lead:], bt.shape[1], ctx.q_start[lead:],
+            ctx.ctx_len[lead:], ctx.n_seqs - lead, q_len, n_q, n_kv, d, float(scale), int(window or 0), cache.page_tokens,
+            cache.k_pool.shape[0], ctx.status, self._stream()), "attention (4 bits, prompt)")
+        return qkv.shape[0]
 
     force_decode4_splits = 0               # > 0: every decode attention over pages in 4 bits splits its keys this many ways
 

@@ -285,6 +285,82 @@ def test_attention_decode_reports_a_bad_page(ops_of):
         assert step.ctx.status.tolist() == [2, 0, bad if bad > 0 else -1, 48]
 
 
+PROMPT = [
+    # n_q, n_kv, d, lens, page, window
+    (16, 8, 128, [(2, 0)], 16, 0),
+    (32, 8, 128, [(300, 0), (77, 500), (2, 129)], 16, 0),
+    (14, 2, 64, [(1, 100), (1, 700), (333, 1100)], 16, 500),                  # a mixed step
+    (4, 4, 128, [(129, 127), (128, 128), (1, 0), (130, 0)], 32, 0),           # (a single row that does not lead)
+    (40, 2, 64, [(65, 300), (3, 1)], 16, 0),
+    (128, 1, 128, [(9, 200)], 16, 0),                                         # a query tile of one token
+    (8, 2, 64, [(500, 30)], 48, 33),
+    (6, 2, 128, [(40, 1000), (700, 0)], 16, 128),
+    (5, 1, 128, [(31, 2000)], 16, 16),
+]
+
+
+@pytest.mark.parametrize("n_q,n_kv,d,lens,page,window", PROMPT)
+def test_attention_prompt(ops_of, n_q, n_kv, d, lens, page, window):
+    step, qkv, pools, out, want, top_s, top_v = _attention_case(ops_of(BF16), BF16, n_q, n_kv, d, lens, page, window, seed=d + n_q,
+                                                                stride=8)
+    # keys and values stand as bfloat16 operands: a half step of each, the keys' in the scores (twice: the sum too)
+    half = 2.0 ** -8
+    extra = top_v * (2 * half * top_s + half)
+    assert ((out - want).abs() <= _bounds(BF16, step, d, n_q, want, top_s, top_v, True) + extra[..., None]).all()
+
+
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("many", [False, True])
+def test_values_and_keys_that_are_nan(ops_of, d, window, many):
+    """A group of a cached value that is NaN makes the group's columns NaN for the rows that see it, and nothing else; a key that is NaN
+    makes every row NaN that sees it."""
+    ops = ops_of(BF16)
+    n_q, n_kv, lens = 4, 2, [(150, 60), (1, 90)]
+    step = Step(lens, 16, DEV, window=window)
+    bad_v = [(0, 70 + i) for i in range(45)] if many else [(0, 100), (0, 203), (1, 90)]
+    bad_k = [(0, 140)]
+    pools, plain = [], []
+    for values in (False, True):
+        x = torch.randn((step.pages, n_kv, 16, d), generator=_gen(7 + values), device=DEV).double()
+        codes, s, z = quantize4(x)
+        for seq, key in bad_v if values else bad_k:
+            page = int(step.table[seq, key // 16])
+            if page >= 0:
+                s[page, 1, key % 16, -1] = z[page, 1, key % 16, -1] = math.nan
+        pools.append(packed.pack_pages(codes, s, z, values))
+        plain.append(values4(codes, s, z))
+    qkv = torch.randn((151, (n_q + 2 * n_kv) * d), generator=_gen(9), device=DEV).to(BF16)
+    out = torch.zeros((151, n_q * d), dtype=BF16, device=DEV)
+    ops.attention(step.ctx, qkv, out, n_q, n_kv, d, d ** -0.5, window or None, step.view(*pools))
+    got = out.view(151, n_q, d).isnan()
+    want = torch.zeros_like(got)
+    for seq, first, count, past in ((0, 0, 150, 60), (1, 150, 1, 90)):
+        for t in range(count):
+            p = past + t
+            sees = lambda key: key <= p and (not window or key > p - window)  # noqa: E731
+            if any(s == seq and sees(key) for s, key in bad_v):
+                want[first + t, 2:, d - 64 if d > 64 else 0:] = True
+            if any(s == seq and sees(key) for s, key in bad_k):
+                want[first + t, 2:] = True
+    if many and window:
+        # (more than fit into the kernel's list: the keys behind it count as one range)
+        assert (got | ~want).all() and not got[:, :2].any()
+    else:
+        assert torch.equal(got, want)
+    assert step.ctx.status.tolist() == [0, 0, 0, 0]
+
+
+def test_attention_prompt_reports_a_bad_page(ops_of):
+    ops = ops_of(BF16)
+    for bad in (-1, 10 ** 6):
+        step, qkv, pools, *_ = _attention_case(ops, BF16, 4, 2, 128, [(20, 200), (30, 90)], 16, 0)
+        step.table[0, 3] = bad
+        out = torch.zeros((50, 4 * 128), dtype=BF16, device=DEV)
+        ops.attention(step.ctx, qkv, out, 4, 2, 128, 0.1, None, step.view(*pools))
+        assert step.ctx.status.tolist()[0] == 2 and step.ctx.status.tolist()[3] == 48
+
+
 def test_attention_refusals(ops_of):
     ops = ops_of(BF16)
     step = Step([(1, 20)], 16, DEV)
