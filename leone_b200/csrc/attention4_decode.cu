@@ -526,15 +526,16 @@ attention4_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int row_stride, 
   }
 }
 
-// The splits' partial results of more splits than a cluster holds.  grid = (heads, sequences), a thread for two columns.
+// The parts of more splits than a cluster holds, and those of prompt portions.  grid = (sequences or tokens, heads), a thread for two
+// columns; rows: where a sequence's row of the output is, or null for token i in row i.
 __global__ void attention4_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
-                                        __nv_bfloat16* __restrict__ out, int out_stride, const int* __restrict__ q_start, int n_q,
-                                        int d, int splits) {
+                                        __nv_bfloat16* __restrict__ out, int out_stride, const int* __restrict__ rows, int n_q, int d,
+                                        int splits) {
   __shared__ float f_s[64];
   __shared__ float l_s;
   pdl_trigger();
   pdl_wait();
-  const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
+  const int head = blockIdx.y, seq = blockIdx.x, tid = threadIdx.x;
   const size_t base = ((size_t)seq * n_q + head) * splits;
   if (tid < 32) {
     float m[2], l[2];
@@ -549,7 +550,8 @@ __global__ void attention4_merge_kernel(const float* __restrict__ part_o, const 
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float f = m[i] == -INFINITY ? 1.f : ex2(m[i] - top);
+      // a part without a key has no outputs (perhaps none were written); one whose scores are all NaN has a sum that is
+      const float f = m[i] == -INFINITY ? (l[i] == 0.f ? 0.f : 1.f) : ex2(m[i] - top);
       f_s[tid + 32 * i] = f;
       sum = fmaf(f, l[i], sum);
     }
@@ -561,12 +563,13 @@ __global__ void attention4_merge_kernel(const float* __restrict__ part_o, const 
   float o0 = 0.f, o1 = 0.f;
 #pragma unroll 8
   for (int s = 0; s < splits; ++s) {
+    if (f_s[s] == 0.f) continue;
     const float2 v = *reinterpret_cast<const float2*>(part_o + (base + s) * d + c);
     o0 = fmaf(f_s[s], v.x, o0);
     o1 = fmaf(f_s[s], v.y, o1);
   }
   const float inv = l_s == 0.f ? 0.f : 1.f / l_s;
-  *reinterpret_cast<__nv_bfloat162*>(out + (size_t)q_start[seq] * out_stride + (size_t)head * d + c) =
+  *reinterpret_cast<__nv_bfloat162*>(out + (size_t)(rows == nullptr ? seq : rows[seq]) * out_stride + (size_t)head * d + c) =
       __floats2bfloat162_rn(o0 * inv, o1 * inv);
 }
 
@@ -596,7 +599,7 @@ int launch_decode(const __nv_bfloat16* qkv, int row_stride, __nv_bfloat16* out, 
                               row_stride, out, out_stride, pa, q_start, ctx_len, n_q, scale, window, splits, 0, order, scratch,
                               part_ml, status);
   if (e != 0 || splits == 1) return e;
-  return launch_kernel(attention4_merge_kernel, dim3(n_q, n_seqs), dim3(D / 2), 0, stream, (const float*)scratch,
+  return launch_kernel(attention4_merge_kernel, dim3(n_seqs, n_q), dim3(D / 2), 0, stream, (const float*)scratch,
                        (const float*)part_ml, out, out_stride, q_start, n_q, D, splits);
 }
 
@@ -636,4 +639,14 @@ extern "C" int leone_attention4_decode(const void* qkv, int row_stride, void* ou
   if (wide) LAUNCH(128, 2);
   LAUNCH(128, 1);
 #undef LAUNCH
+}
+
+// What leone_attention4_prefill left in scratch becomes the output's rows 0 .. n_tokens - 1.
+extern "C" int leone_attention4_merge(const float* part_o, const float* part_ml, void* out, int out_stride, int n_tokens, int n_q, int d,
+                                      int splits, cudaStream_t stream) {
+  if (n_tokens <= 0) return 0;
+  if ((d != 64 && d != 128) || n_q <= 0 || n_q > 65535 || splits < 1 || splits > 64) return kRefusedSize;
+  if (out_stride % 2 != 0 || ((uintptr_t)out & 3) || ((uintptr_t)part_o | (uintptr_t)part_ml) & 15) return kRefusedAlignment;
+  return launch_kernel(cache4::attention4_merge_kernel, dim3(n_tokens, n_q), dim3(d / 2), 0, stream, part_o, part_ml,
+                       (__nv_bfloat16*)out, out_stride, (const int*)nullptr, n_q, d, splits);
 }

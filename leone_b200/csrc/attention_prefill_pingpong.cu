@@ -59,7 +59,7 @@ constexpr int kTileThreads = kTileWarps * 32;
 constexpr int kMmaWarp = 2 * kTileWarps;
 constexpr int kLoadWarp0 = kMmaWarp + 1;   // two warps gather keys, the next two values
 constexpr int kStreamThreads = 64;         // threads that gather one kind of tile (a thread per two key rows)
-// Pages in 4 bits: twice as many, who also convert them (2,048 tokens behind 6,144 on 32 and 8 heads of 128: FIG us; 435 with 64 threads)
+// Pages in 4 bits: twice as many, who also convert them (2,048 tokens behind 6,144 on 32 and 8 heads of 128: 383 us; 447 with 64 threads)
 constexpr int stream_threads(int form) { return form == 3 ? 128 : kStreamThreads; }
 constexpr int block_threads(int form) { return kLoadWarp0 * 32 + 2 * stream_threads(form); }
 constexpr float kLog2e = 1.4426950408889634f;
@@ -224,6 +224,14 @@ struct OddValues {
   float query_power[2][kRows];    // the same of a row of queries
 };
 
+// Pages in 4 bits: the keys of a block's queries may be split over gridDim.y blocks, each with a share of the key tiles, where there are too
+// few query tiles for the SMs.  A split leaves its rows' (maximum, sum, unnormalised output) in scratch, [token][query head][split],
+// for a kernel that merges them (attention4_decode.cu).
+struct Split {
+  float* part_o;                  // null: not split
+  float* part_ml;
+};
+
 template <int D, bool kPacked> constexpr int smem_bytes() {
   // two Q tiles, two K and two V tiles, row sources [2 kinds][2 buffers][128], barriers; 1024 for alignment
   return 2 * kRows * D * 2 + 4 * kKeys * D * 2 + 2 * 2 * kKeys * 8 + 18 * 8 + 1024 +
@@ -274,7 +282,7 @@ __global__ void __launch_bounds__(block_threads(kForm))
 attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row_stride,
                                   __nv_bfloat16* __restrict__ out, int out_stride, PagedArgs pa,
                                   const int* __restrict__ q_start, const int* __restrict__ ctx_len, int n_q,
-                                  float scale, int window, Rules rules_in, Pooled pooled, int query_tiles, int* status) {
+                                  float scale, int window, Rules rules_in, Pooled pooled, Split parts, int query_tiles, int* status) {
   constexpr bool kRules = kForm == 1, kPooled = kForm == 2, kPacked = kForm == 3;
   struct {
     int weights, chunk;
@@ -351,21 +359,29 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
     int k_lo = 0;
     if (window > 0) k_lo = max(0, start + tok0 - window + 1);
     if (rules.chunk > 0) k_lo = ((start + tok0) / rules.chunk) * rules.chunk;
-    const int tile0 = (k_lo / kKeys) * kKeys;
-    const int k_hi = start + max(hi0, hi1);             // one past the last key any row reads
+    int tile0 = (k_lo / kKeys) * kKeys;
+    int k_hi = start + max(hi0, hi1);                   // one past the last key any row reads
     // pooled form: the row at position p sees the blocks 0 .. blocks_seen(p) - 1; nb_max of them are seen by
     // the block's last row, in nbt tiles that run before the token tiles (tile t < nbt holds blocks, tile
     // t >= nbt the keys from tile0 + (t - nbt) * kKeys on)
     auto blocks_seen = [&](int p) { return kPooled && p >= window - 1 ? (p - window + 1) / pooled.pool : 0; };
     const int nb_max = blocks_seen(k_hi - 1);
     const int nbt = kPooled ? (nb_max + kKeys - 1) / kKeys : 0;
-    const int n0 = nbt + (start + hi0 - tile0 + kKeys - 1) / kKeys;
-    const int n1 = hi1 > lo1 ? nbt + (start + hi1 - tile0 + kKeys - 1) / kKeys : 0;
+    int n0 = nbt + (start + hi0 - tile0 + kKeys - 1) / kKeys;
+    int n1 = hi1 > lo1 ? nbt + (start + hi1 - tile0 + kKeys - 1) / kKeys : 0;
+    if (kPacked && gridDim.y > 1) {                     // this block's share of the key tiles (perhaps none)
+      const int all = max(n0, n1), share = (all + gridDim.y - 1) / gridDim.y, from = min(all, (int)blockIdx.y * share);
+      tile0 += from * kKeys;
+      k_lo = max(k_lo, tile0);
+      k_hi = min(k_hi, tile0 + share * kKeys);
+      n0 = min(max(n0 - from, 0), share);
+      n1 = min(max(n1 - from, 0), share);
+    }
     const int n_tiles = max(n0, n1);
 
     if (warp == kMmaWarp) {
       // ---------------- the warp that issues the tensor-core work ----------------
-      if (elect_one()) {
+      if ((!kPacked || n_tiles > 0) && elect_one()) {
         // (without the two bits that say bfloat16: fp16 operands)
         constexpr uint32_t idesc_s = instr_desc_bf16(kRows, kKeys) & (kPacked ? ~((1u << 7) | (1u << 10)) : ~0u);
         constexpr uint32_t idesc_o = instr_desc_bf16_b_mn(kRows, D);
@@ -815,6 +831,10 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_p + 8 * j);       // PV_j(t) may go
       }
+      const size_t part_row = kPacked && parts.part_o != nullptr && my_pos >= 0
+                                  ? ((size_t)(q0 + lo + my_tl) * n_q + kvh * g + (row - my_tl * g)) * gridDim.y + blockIdx.y : 0;
+      if (kPacked && parts.part_o != nullptr && nj == 0 && my_pos >= 0 && half == 0)
+        *reinterpret_cast<float2*>(parts.part_ml + part_row * 2) = make_float2(-INFINITY, 0.f);
       // the last O_j, divided by the row's sum (its two halves meet like the maxima)
       if (nj > 0) {
         halves[j][nj & 1][half][row] = l_run;
@@ -835,7 +855,25 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
             }
             if (sees) inv = NAN;
           }
+          if (parts.part_o != nullptr) {                   // this split's part, as it is
+            const float as_is = isnan(inv) && !isnan(l_row) ? inv : 1.f;
+            const bool store = ok_all && my_pos >= 0;
+            if (store && half == 0) *reinterpret_cast<float2*>(parts.part_ml + part_row * 2) = make_float2(m_run, l_row);
+            float4* dst = reinterpret_cast<float4*>(parts.part_o + part_row * D + half * (D / 2));
+#pragma unroll
+            for (int c = 0; c < D / 2; c += 16) {
+              uint32_t r[16];
+              tmem_ld16_issue(t_o + c, r);
+              tmem_ld_wait();
+              if (!store) continue;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                dst[c / 4 + i] = make_float4(__uint_as_float(r[4 * i]) * as_is, __uint_as_float(r[4 * i + 1]) * as_is,
+                                             __uint_as_float(r[4 * i + 2]) * as_is, __uint_as_float(r[4 * i + 3]) * as_is);
+            }
+          }
         }
+        if (!kPacked || parts.part_o == nullptr) {
         const bool store = ok_all && my_pos >= 0;
         const int hh = row - my_tl * g;
         __nv_bfloat16* dst = out + (size_t)(q0 + lo + (store ? my_tl : 0)) * out_stride + (size_t)(kvh * g + hh) * D +
@@ -859,6 +897,7 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
             }
           }
         }
+        }
       }
     }
   }
@@ -881,7 +920,8 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
 template <int D, int kForm>
 int launch_form(const __nv_bfloat16* qkv, int row_stride, __nv_bfloat16* out, int out_stride, const PagedArgs& pa,
                 const int* q_start, const int* ctx_len, int n_seqs, int n_q, int max_q_len, float scale, int window,
-                const Rules& rules, const Pooled& pooled, int* status, cudaStream_t stream) {
+                const Rules& rules, const Pooled& pooled, int* status, cudaStream_t stream, int splits = 1,
+                const Split& parts = Split{nullptr, nullptr}) {
   static bool configured = false;
   if (!configured) {
     cudaError_t e = cudaFuncSetAttribute(attention_prefill_pingpong_kernel<D, kForm>,
@@ -902,10 +942,10 @@ int launch_form(const __nv_bfloat16* qkv, int row_stride, __nv_bfloat16* out, in
   }();
   const long long tiles = (long long)((max_q_len + tq - 1) / tq) * pa.n_kv * n_seqs;
   const int query_tiles = tiles <= sms ? 1 : 2;
-  dim3 grid(((max_q_len + query_tiles * tq - 1) / (query_tiles * tq)) * pa.n_kv, 1, n_seqs);
+  dim3 grid(((max_q_len + query_tiles * tq - 1) / (query_tiles * tq)) * pa.n_kv, splits, n_seqs);
   return launch_kernel(attention_prefill_pingpong_kernel<D, kForm>, grid, dim3(block_threads(kForm)), smem_bytes<D, kForm == 3>(), stream,
-                       qkv, row_stride, out, out_stride, pa, q_start, ctx_len, n_q, scale, window, rules, pooled, query_tiles,
-                       status);
+                       qkv, row_stride, out, out_stride, pa, q_start, ctx_len, n_q, scale, window, rules, pooled, parts,
+                       query_tiles, status);
 }
 
 template <int D>
@@ -999,24 +1039,30 @@ extern "C" int leone_attention_prefill_pingpong(const void* qkv, int row_stride,
                                                 window, 0, 0, nullptr, page_tokens, num_pages, status, stream);
 }
 
-// The same over pages in 4 bits (cache4.cuh; page_tokens a multiple of 16).
+// The same over pages in 4 bits (cache4.cuh; page_tokens a multiple of 16).  `splits` > 1: the keys of every query tile are split over
+// that many blocks, whose parts go to `scratch`: (D + 2) floats for each (token, query head, split) of the qkv rows, outputs
+// first, then (maximum, sum); leone_attention4_merge makes the output of them.
 extern "C" int leone_attention4_prefill(const void* qkv, int row_stride, void* out, int out_stride, const void* k_pool,
                                         const void* v_pool, const int* block_table, int table_width, const int* q_start,
                                         const int* ctx_len, int n_seqs, int max_q_len, int n_q, int n_kv, int d, float scale, int window,
-                                        int page_tokens, int num_pages, int* status, cudaStream_t stream) {
+                                        int page_tokens, int num_pages, int splits, float* part_o, float* part_ml, int* status,
+                                        cudaStream_t stream) {
   if (n_seqs <= 0 || max_q_len <= 0) return 0;
   if ((d != 64 && d != 128) || !(scale > 0.f) || window < 0) return kRefusedSize;
   if (n_q <= 0 || n_kv <= 0 || n_q % n_kv != 0 || n_q / n_kv > pingpong::kRows) return kRefusedSize;
   if (page_tokens <= 0 || page_tokens % cache4::kUnit != 0 || table_width <= 0 || n_seqs > 65535) return kRefusedSize;
+  if (splits < 1 || splits > 64 || (splits > 1) != (part_o != nullptr) || (part_o == nullptr) != (part_ml == nullptr)) return kRefusedSize;
   if (row_stride % 8 != 0 || out_stride % 8 != 0) return kRefusedAlignment;
-  if (((uintptr_t)qkv | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return kRefusedAlignment;
+  if (((uintptr_t)qkv | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)part_o | (uintptr_t)part_ml) & 15)
+    return kRefusedAlignment;
   const pingpong::PagedArgs pa{(const __nv_bfloat16*)k_pool, (const __nv_bfloat16*)v_pool, block_table, table_width,
                                page_tokens, num_pages, n_kv};
   const pingpong::Rules rules{0, 0, nullptr};
   const pingpong::Pooled none{nullptr, nullptr, nullptr, 0, 0, 0, 0, 1.f};
+  const pingpong::Split parts{part_o, part_ml};
   if (d == 64)
     return pingpong::launch_form<64, 3>((const __nv_bfloat16*)qkv, row_stride, (__nv_bfloat16*)out, out_stride, pa, q_start, ctx_len,
-                                        n_seqs, n_q, max_q_len, scale, window, rules, none, status, stream);
+                                        n_seqs, n_q, max_q_len, scale, window, rules, none, status, stream, splits, parts);
   return pingpong::launch_form<128, 3>((const __nv_bfloat16*)qkv, row_stride, (__nv_bfloat16*)out, out_stride, pa, q_start, ctx_len,
-                                       n_seqs, n_q, max_q_len, scale, window, rules, none, status, stream);
+                                       n_seqs, n_q, max_q_len, scale, window, rules, none, status, stream, splits, parts);
 }

@@ -622,12 +622,35 @@ class CudaOps:
         if n_q // n_kv > 128 or not scale > 0:
             return lead
         q_len = int(ctx.q_lens[lead:].max()) if lead else int(ctx.max_q_len)
+        n, n_seqs, group = qkv.shape[0], ctx.n_seqs - lead, n_q // n_kv
+        keys = int(ctx.ctx_lens[lead:].max()) if lead else int(ctx.max_ctx_len)
+        splits = self.choose_prompt4_splits(n_seqs, n_kv, group, q_len, min(keys, window + q_len) if window else keys)
+        part_o = part_ml = None
+        if splits > 1:
+            # (rows of the step's tokens: the leading decode rows' stay unused)
+            part_o = self._scratch("attention4_parts", n * n_q * splits, d, torch.float32)
+            part_ml = self._scratch("attention4_sums", n * n_q * splits, 2, torch.float32)
         self.launches += 1
         _check(self.fast.calls.leone_attention4_prefill(
             qkv, qkv.stride(0), out, out.stride(0), cache.k_pool, cache.v_pool, bt[lead:], bt.shape[1], ctx.q_start[lead:],
-            ctx.ctx_len[lead:], ctx.n_seqs - lead, q_len, n_q, n_kv, d, float(scale), int(window or 0), cache.page_tokens,
-            cache.k_pool.shape[0], ctx.status, self._stream()), "attention (4 bits, prompt)")
-        return qkv.shape[0]
+            ctx.ctx_len[lead:], n_seqs, q_len, n_q, n_kv, d, float(scale), int(window or 0), cache.page_tokens,
+            cache.k_pool.shape[0], splits, part_o, part_ml, ctx.status, self._stream()), "attention (4 bits, prompt)")
+        if splits > 1:
+            self.launches += 1
+            _check(self.packed_calls.leone_attention4_merge(
+                part_o[lead * n_q * splits:], part_ml[lead * n_q * splits:], out[lead:], out.stride(0), n - lead, n_q, d, splits,
+                self._stream()), "attention (4 bits, merge)")
+        return n
+
+    force_prompt4_splits = 0               # > 0: the same for prompt portions
+
+    def choose_prompt4_splits(self, n_seqs: int, n_kv: int, group: int, q_len: int, keys: int) -> int:
+        """How many blocks share the keys of a query tile (128 rows of tokens and heads) of prompt portions over pages in 4 bits."""
+        if self.force_prompt4_splits:
+            return self.force_prompt4_splits
+        tokens = 128 // group
+        blocks = -(-q_len // tokens) * n_kv * n_seqs
+        return max(1, min(64, 148 // blocks, -(-keys // 128) // 3))
 
     force_decode4_splits = 0               # > 0: every decode attention over pages in 4 bits splits its keys this many ways
 

@@ -299,10 +299,15 @@ PROMPT = [
 ]
 
 
+@pytest.mark.parametrize("splits", [0, 1, 2, 5, 64])
 @pytest.mark.parametrize("n_q,n_kv,d,lens,page,window", PROMPT)
-def test_attention_prompt(ops_of, n_q, n_kv, d, lens, page, window):
-    step, qkv, pools, out, want, top_s, top_v = _attention_case(ops_of(BF16), BF16, n_q, n_kv, d, lens, page, window, seed=d + n_q,
-                                                                stride=8)
+def test_attention_prompt(ops_of, n_q, n_kv, d, lens, page, window, splits):
+    ops = ops_of(BF16)
+    ops.force_prompt4_splits = splits
+    try:
+        step, qkv, pools, out, want, top_s, top_v = _attention_case(ops, BF16, n_q, n_kv, d, lens, page, window, seed=d + n_q, stride=8)
+    finally:
+        ops.force_prompt4_splits = 0
     # keys and values stand as bfloat16 operands: a half step of each, the keys' in the scores (twice: the sum too)
     half = 2.0 ** -8
     extra = top_v * (2 * half * top_s + half)
@@ -312,7 +317,8 @@ def test_attention_prompt(ops_of, n_q, n_kv, d, lens, page, window):
 @pytest.mark.parametrize("window", [0, 40])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("many", [False, True])
-def test_values_and_keys_that_are_nan(ops_of, d, window, many):
+@pytest.mark.parametrize("splits", [1, 2])
+def test_values_and_keys_that_are_nan(ops_of, d, window, many, splits):
     """A group of a cached value that is NaN makes the group's columns NaN for the rows that see it, and nothing else; a key that is NaN
     makes every row NaN that sees it."""
     ops = ops_of(BF16)
@@ -332,7 +338,11 @@ def test_values_and_keys_that_are_nan(ops_of, d, window, many):
         plain.append(values4(codes, s, z))
     qkv = torch.randn((151, (n_q + 2 * n_kv) * d), generator=_gen(9), device=DEV).to(BF16)
     out = torch.zeros((151, n_q * d), dtype=BF16, device=DEV)
-    ops.attention(step.ctx, qkv, out, n_q, n_kv, d, d ** -0.5, window or None, step.view(*pools))
+    ops.force_prompt4_splits = splits
+    try:
+        ops.attention(step.ctx, qkv, out, n_q, n_kv, d, d ** -0.5, window or None, step.view(*pools))
+    finally:
+        ops.force_prompt4_splits = 0
     got = out.view(151, n_q, d).isnan()
     want = torch.zeros_like(got)
     for seq, first, count, past in ((0, 0, 150, 60), (1, 150, 1, 90)):
