@@ -62,6 +62,9 @@ inline int pair_blocks(int bn) { return bn <= 96 ? 2 : 1; }
 __device__ __forceinline__ void umma2_k64(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(LEONE_UMMA_BLOCK("2", "f16") ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh) : "memory");
 }
+__device__ __forceinline__ void umma2_k128_i8(uint32_t tmem_d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(LEONE_UMMA_BLOCK("2", "i8") ::"r"(tmem_d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh) : "memory");
+}
 // One arrival on the barrier at this offset in both blocks of the pair when every MMA issued so
 // far by this thread is done.
 __device__ __forceinline__ void umma2_commit_both(uint32_t bar, uint32_t lead) {
@@ -129,9 +132,13 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
 // finishes a chunk copies its S pieces into the (now free) stages with the copy engine, adds
 // them in split order on top of the residual values and runs the epilogue (no folded norm).  The caller's rule takes
 // this form only where its unsplit pairs are switched off.
+//
+// kInt8: both operands are 8-bit integers (128 of them a k-block), the sums int32 (see GemmParams::row_scale); unsplit only.
+template <bool kInt8>
 __global__ void __launch_bounds__(kPairThreads, 1)
 gemm_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                  const GemmParams p, const int BN, const int blocks) {
+  constexpr int kElems = kInt8 ? 2 * kTileK : kTileK;  // elements of K in a k-block
   const PairShape cfg = pair_shape(BN, blocks);
   const int kStages = cfg.stages;
   constexpr int kABytes = kTileW * kTileK * 2;
@@ -153,14 +160,14 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   const uint32_t crank = cluster_ctarank();            // 0 .. 2 S - 1
   const uint32_t rank = crank & 1u;                    // within the pair
   const uint32_t lead = crank & ~1u;                   // the pair's first block, by rank in the cluster
-  const int S = p.splits, split = (int)(crank >> 1);
+  const int S = kInt8 ? 1 : p.splits, split = kInt8 ? 0 : (int)(crank >> 1);
   const int n_tiles = (p.N + BN - 1) / BN;
   const int m_tiles = (p.M + kTileW - 1) / kTileW;
   const int m_pairs = (m_tiles + 1) / 2;
   const int total = n_tiles * m_pairs;
   // unsplit: pair q of the grid walks tiles q, q + pairs, ..; split: cluster q has tile q only
   const int pair = blockIdx.x / (2 * S), pairs = S == 1 ? gridDim.x >> 1 : total;
-  const int all_k_blocks = (p.K + kTileK - 1) / kTileK;
+  const int all_k_blocks = (p.K + kElems - 1) / kElems;
   const int k_share = (all_k_blocks + S - 1) / S;
   const int kb_lo = split * k_share, kb_hi = min(all_k_blocks, kb_lo + k_share);
 
@@ -213,12 +220,12 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
       auto load_w = [&](const Cursor& c, uint32_t dst, uint32_t bar_here, uint32_t bar) {
         const int here = min(blocks, kb_hi - c.kb);
         if (rank == 0) mbar_expect_tx(bar_here, (uint32_t)(2 * here * (kABytes + cfg.half * kTileK * 2)));
-        tma_load_2d_pair(dst + blocks * kABytes, &map_w, bar, c.kb * kTileK, c.n);
-        if (here == 2) tma_load_2d_pair(dst + 2 * kABytes + cfg.b_bytes, &map_w, bar, (c.kb + 1) * kTileK, c.n);
+        tma_load_2d_pair(dst + blocks * kABytes, &map_w, bar, c.kb * kElems, c.n);
+        if (here == 2) tma_load_2d_pair(dst + 2 * kABytes + cfg.b_bytes, &map_w, bar, (c.kb + 1) * kElems, c.n);
       };
       auto load_x = [&](const Cursor& c, uint32_t dst, uint32_t bar) {
-        tma_load_2d_pair(dst, &map_x, bar, c.kb * kTileK, c.m);
-        if (min(blocks, kb_hi - c.kb) == 2) tma_load_2d_pair(dst + kABytes, &map_x, bar, (c.kb + 1) * kTileK, c.m);
+        tma_load_2d_pair(dst, &map_x, bar, c.kb * kElems, c.m);
+        if (min(blocks, kb_hi - c.kb) == 2) tma_load_2d_pair(dst + kABytes, &map_x, bar, (c.kb + 1) * kElems, c.m);
       };
       const uint32_t lead_full0 = cluster_map(full0, lead);
       Cursor c{pair, kb_lo, 0, 0};
@@ -249,7 +256,11 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   } else if (warp == 1) {
     // ---------------- MMA issuer (the first block) ----------------
     if (elect_one()) {
-      const uint32_t idesc = instr_desc_bf16(2 * kTileW, BN);
+      const uint32_t idesc = kInt8 ? instr_desc_i8(2 * kTileW, BN) : instr_desc_bf16(2 * kTileW, BN);
+      auto issue = [&](uint32_t d, uint32_t x, uint32_t w, uint32_t add) {
+        if constexpr (kInt8) umma2_k128_i8(d, x, w, idesc, add);
+        else umma2_k64(d, x, w, idesc, add);
+      };
       const uint32_t first = desc_low(tiles_base), step = cfg.stage_bytes >> 4;
       const uint32_t b_step = cfg.b_bytes >> 4, b_at = blocks * (kABytes >> 4);
       uint32_t a = first, bar = full0, phase = 0;
@@ -263,9 +274,9 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         int left = kb_hi - kb_lo;
         for (; left > 0; left -= blocks) {
           if (!mbar_wait_cluster(bar, phase, giveup)) break;
-          umma2_k64(tmem_d, a, a + b_at, idesc, sum);
+          issue(tmem_d, a, a + b_at, sum);
           sum = 1;
-          if (blocks == 2 && left > 1) umma2_k64(tmem_d, a + (kABytes >> 4), a + b_at + b_step, idesc, 1);
+          if (blocks == 2 && left > 1) issue(tmem_d, a + (kABytes >> 4), a + b_at + b_step, 1);
           umma2_commit_both(bar + 8 * kStages, lead);
           bar += 8;
           a += step;
@@ -336,7 +347,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         __threadfence();
         break;
       }
-      if (!finish_rows<false>(p, taddr, m_tile * kTileW + quarter * 32, n_tile * BN, c_lo, c_hi, box, complete, squares)) break;
+      if (!finish_rows<kInt8>(p, taddr, m_tile * kTileW + quarter * 32, n_tile * BN, c_lo, c_hi, box, complete, squares)) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -411,10 +422,10 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
   }
 }
 
-static int configure_pair() {
+template <bool kInt8> static int configure_pair() {
   static bool configured = false;
   if (!configured) {
-    cudaError_t e = cudaFuncSetAttribute(gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemLimit);
+    cudaError_t e = cudaFuncSetAttribute(gemm_pair_kernel<kInt8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmemLimit);
     if (e != cudaSuccess) return (int)e;
     configured = true;
   }
@@ -423,7 +434,7 @@ static int configure_pair() {
 
 // Clusters of 2 * splits blocks that can be resident at once for tiles of bn weight rows (0: none).
 int pair_cluster_capacity(int bn, int splits) {
-  if (configure_pair() != 0) return 0;
+  if (configure_pair<false>() != 0) return 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2u * (unsigned)splits * 64u);
   cfg.blockDim = dim3(kPairThreads);
@@ -436,27 +447,28 @@ int pair_cluster_capacity(int bn, int splits) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int clusters = 0;
-  if (cudaOccupancyMaxActiveClusters(&clusters, gemm_pair_kernel, &cfg) != cudaSuccess) {
+  if (cudaOccupancyMaxActiveClusters(&clusters, gemm_pair_kernel<false>, &cfg) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
   return clusters;
 }
 
+template <bool kInt8>
 int launch_pair(const CUtensorMap& mw, const CUtensorMap& mx, const GemmParams& p, int bn, int sm_count,
                 cudaStream_t stream) {
-  int r = configure_pair();
+  int r = configure_pair<kInt8>();
   if (r != 0) return r;
   const int n_tiles = (p.N + bn - 1) / bn, m_pairs = ((p.M + kTileW - 1) / kTileW + 1) / 2;
   const long long total = (long long)n_tiles * m_pairs;
   if (p.splits > 1) {
     // one tile per cluster of 2 * splits blocks, all clusters resident at once
     if (total > pair_cluster_capacity(bn, p.splits)) return kRefusedSize;
-    return launch_kernel_cluster(gemm_pair_kernel, dim3((unsigned)(total * 2 * p.splits)), dim3(kPairThreads),
+    return launch_kernel_cluster(gemm_pair_kernel<kInt8>, dim3((unsigned)(total * 2 * p.splits)), dim3(kPairThreads),
                                  (size_t)pair_shape(bn, pair_blocks(bn)).smem_bytes, stream, dim3(2u * (unsigned)p.splits), mw, mx, p, bn, pair_blocks(bn));
   }
   const int pairs = (int)(total < sm_count / 2 ? total : sm_count / 2);
-  return launch_kernel_cluster(gemm_pair_kernel, dim3(2u * (unsigned)pairs), dim3(kPairThreads),
+  return launch_kernel_cluster(gemm_pair_kernel<kInt8>, dim3(2u * (unsigned)pairs), dim3(kPairThreads),
                                (size_t)pair_shape(bn, pair_blocks(bn)).smem_bytes, stream, dim3(2), mw, mx, p, bn, pair_blocks(bn));
 }
 
@@ -503,7 +515,31 @@ extern "C" int leone_gemm_pair(const void* x, const void* w, void* out, const fl
   set_gate_shape(p, gate_shape);
   if ((uintptr_t)bias & 15) return kRefusedAlignment;
   p.bias = bias;
-  return launch_pair(mw, mx, p, width, sm_count, stream);
+  return launch_pair<false>(mw, mx, p, width, sm_count, stream);
+}
+
+// The unsplit product of 8-bit integers on pairs of SMs, arguments as leone_gemm_narrow_i8 (gemm_narrow.cu); `width` a multiple of 32.
+extern "C" int leone_gemm_pair_i8(const void* x, const float* x_scale, const void* w, const float* w_scale, void* out,
+                                  const float* residual, int m, int n, int k, int ldx, int ldw, int ldc, int epilogue, int width,
+                                  int* status, int sm_count, const float* gate_shape, const float* bias, cudaStream_t stream) {
+  if (m <= 0 || n <= 0) return 0;
+  if (k <= 0 || (k % 16) != 0 || (ldx % 16) != 0 || (ldw % 16) != 0) return kRefusedAlignment;
+  if (epilogue < 0 || epilogue > 3 || sm_count < 2 || width < 32 || width > 256 || (width % 32) != 0) return kRefusedSize;
+  if ((epilogue == 2 && residual == nullptr) || (epilogue == 3 && (n % 32) != 0) || x_scale == nullptr || w_scale == nullptr)
+    return kRefusedSize;
+  if (((uintptr_t)bias | (uintptr_t)w_scale) & 15) return kRefusedAlignment;
+  CUtensorMap mw, mx;
+  int r = make_tensor_map_2d_i8(&mw, w, (uint64_t)n, (uint64_t)k, (uint64_t)ldw, (uint32_t)(width / 2));
+  if (r != 0) return r;
+  r = make_tensor_map_2d_i8(&mx, x, (uint64_t)m, (uint64_t)k, (uint64_t)ldx, kTileW);
+  if (r != 0) return r;
+  GemmParams p{out, residual, m, n, k, ldc, epilogue, 1, 0, nullptr, nullptr, status, nullptr,
+               nullptr, nullptr, nullptr, 0, nullptr, 0, 0.f, 0};
+  set_gate_shape(p, gate_shape);
+  p.bias = bias;
+  p.row_scale = x_scale;
+  p.col_scale = w_scale;
+  return launch_pair<true>(mw, mx, p, width, sm_count, stream);
 }
 
 // Tiles of `width` weight rows whose clusters of 2 * splits blocks can be resident at once, and the

@@ -66,6 +66,14 @@ class Int8Products:
         self.calls = EntryPoints(self.lib)
         self.sm_count = torch.cuda.get_device_properties(ops.device).multi_processor_count
 
+    force = None               # (on pairs of SMs, tile width) of every product, whatever the rule says (tests set it)
+
+    def choose(self, m: int, n: int, k: int, gated: bool):
+        """``(on pairs of SMs, weight rows per tile)``."""
+        if m > 128:
+            return True, 256
+        return False, 32 * max(1, min(8, -(-n // (32 * self.sm_count))))
+
     def run(self, x, w: Int8Matrix, out, epilogue, residual, gate_shape) -> int:
         """A product of ``x`` with ``w``; returns the number of launches."""
         from .cuda import _check, _dt
@@ -77,7 +85,8 @@ class Int8Products:
         _check(self.ops.packed_calls.leone_quantize_rows(_dt(x.dtype), x, m, k, x.stride(0), codes, scales, stream), "quantize_rows")
         shape = None if gate_shape is None else (c_float * 4)(*[float(v) for v in gate_shape])
         gs = None if shape is None else addressof(shape)
-        width = 32 * max(1, min(8, -(-n // (32 * self.sm_count))))
-        _check(self.calls.leone_gemm_narrow_i8(codes, scales, w.weight, w.scales, out, residual, m, n, k, k, k, out.stride(0),
-                                               epilogue, width, self.ops.status, self.sm_count, gs, w.bias, stream), "gemm_int8")
+        pairs, width = self.force or self.choose(m, n, k, epilogue == 3)
+        entry = self.calls.leone_gemm_pair_i8 if pairs else self.calls.leone_gemm_narrow_i8
+        _check(entry(codes, scales, w.weight, w.scales, out, residual, m, n, k, k, k, out.stride(0), epilogue, width, self.ops.status,
+                     self.sm_count, gs, w.bias, stream), "gemm_int8")
         return 2

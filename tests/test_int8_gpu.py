@@ -78,6 +78,25 @@ def test_linear(ops_of, m, n, k, dtype, bias):
     _check(stream, want + zero + residual.double(), residual.double().abs() + zero.abs(), FP32)
 
 
+@pytest.mark.parametrize("form", [(pairs, width) for pairs in (False, True) for width in (32, 64, 96, 128, 192, 224, 256)])
+def test_forms(ops_of, form):
+    """Every tile width on single SMs and on pairs, whatever the rule would take."""
+    ops = ops_of(BF16)
+    for m, n, k in [(1, 400, 272), (130, 1056, 1040), (257, 96, 4096)]:
+        x, codes, scales = _inputs(m, n, k, BF16, m)
+        w = ops.prepare_matrix_int8(codes, scales)
+        out, wide = torch.empty((m, n), dtype=BF16, device=DEV), torch.empty((m, n), device=DEV)
+        ops.int8.force = form
+        try:
+            ops.linear(x, w, out)
+            ops.linear(x, w, wide)
+        finally:
+            ops.int8.force = None
+        want = _want(x, codes, scales)
+        _check(out, want, want * 0, BF16)
+        _check(wide, want, want * 0, FP32)
+
+
 GATES = [None, (1.0, 7.0, 1.0, 0.0), (1.595769, math.inf, 0.0, 0.044715)]
 
 
