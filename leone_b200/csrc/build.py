@@ -31,7 +31,8 @@ MODULES: Dict[str, List[str]] = {
     # every run needs these: both dtypes, every size
     "core": ["elementwise.cu", "gemm_simt.cu", "gemm_f32_tc.cu", "attention_generic.cu", "attention_f32.cu", "sampling_pipeline.cu", "random_weights.cu"],
     # the bfloat16 serving path: tensor-core products and tiled attention
-    "bf16": ["gemm_tc.cu", "gemm_pair.cu", "gemm_narrow.cu", "attention_tiled.cu", "attention_prefill_pingpong.cu"],
+    "bf16": ["gemm_tc.cu", "gemm_pair.cu", "gemm_narrow.cu", "attention_tiled.cu", "attention_prefill_pingpong.cu",
+             "quantize8.cu", "gemm_int8.cu"],
     # mixers and feed-forwards beyond softmax attention over K/V pages and the dense gated layer:
     # linear attention with a decaying state, attention through a cached latent, attention with a choice
     # of mask and weight rule, routed experts, short convolutions with state, the minGRU recurrence, attention
@@ -41,8 +42,8 @@ MODULES: Dict[str, List[str]] = {
                "attention_masked_mma.cu", "experts.cu", "experts_tc.cu", "norm_act.cu", "short_conv.cu", "attention_pooled.cu",
                "attention_mixed_heads.cu", "attention_mixed_heads_mma.cu", "gated_delta.cu", "gated_delta_mma.cu",
                "gated_linear_attention.cu", "gated_linear_attention_mma.cu", "ssd.cu", "ssd_mma.cu"],
-    # pages in 4 bits (append, read, attention) and rows of tokens in 8 bits
-    "packed": ["cache4.cu", "attention4_decode.cu", "quantize8.cu"],
+    # pages in 4 bits: append, read, decode attention, attention of any size
+    "packed": ["cache4.cu", "attention4_decode.cu"],
     # the entry point that allocates nothing (leone_static.h); it compiles attention_tiled.cu in
     "static": ["attention_decode_static.cu"],
     # the host side of the runtime (pages, block tables, step metadata, the scheduler's decisions,

@@ -188,7 +188,13 @@ class CudaOps:
     def _stream(self):
         if self._pinned_stream is not None:        # (a handle of 0, the default stream, is a valid pin)
             return self._pinned_stream
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return self._current_stream()
+
+    def _current_stream(self):
+        """The handle of this device's current stream (through torch's own lookup of the handle: 0.2 us, where the Stream object that
+        ``torch.cuda.current_stream`` makes takes 3)."""
+        index = self.device.index
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
     def pin_stream(self, on: bool) -> None:
         """Between ``pin_stream(True)`` and ``pin_stream(False)`` every launch goes to the stream
@@ -568,16 +574,18 @@ class CudaOps:
 
     def _pool4(self, cache, n_kv, d):
         """The arguments of a cache in 4 bits, checked."""
-        kp, vp, bt = cache.k_pool, cache.v_pool, cache.block_table
+        kp, vp, bt, page_tokens = cache.k_pool, cache.v_pool, cache.block_table, cache.page_tokens
         if not packed.dim_ok(d):
             raise KernelError(f"rows of {d} elements cannot be held in 4 bits")
-        if vp is None or kp.dtype != torch.uint8 or vp.dtype != torch.uint8 or kp.dim() != 4 or vp.shape != kp.shape \
-                or kp.shape[1:] != (n_kv, cache.page_tokens, packed.row_bytes(d)) or cache.page_tokens % packed.UNIT \
+        shape = kp.shape
+        if vp is None or kp.dtype != torch.uint8 or vp.dtype != torch.uint8 or len(shape) != 4 or vp.shape != shape \
+                or shape[1] != n_kv or shape[2] != page_tokens or shape[3] != packed.row_bytes(d) or page_tokens % packed.UNIT \
                 or not kp.is_contiguous() or not vp.is_contiguous() or cache.tokens_per_row != 1:
             raise KernelError("cache pool layout (4 bits)")
-        if bt.dtype != torch.int32 or bt.dim() != 2 or not bt.is_contiguous():
+        table = bt.shape
+        if bt.dtype != torch.int32 or len(table) != 2 or not bt.is_contiguous():
             raise KernelError("block table")
-        return bt, bt.shape[1], bt.shape[0], kp, vp, kp.shape[0], cache.page_tokens
+        return bt, table[1], table[0], kp, vp, shape[0], page_tokens
 
     def read_packed_rows(self, ctx, cache, n_kv, d, k_out, v_out):
         """What a cache in 4 bits holds for the step's tokens: ``k_out`` and ``v_out`` ``[tokens, n_kv * d]``, fp32 or bfloat16.  A
@@ -591,56 +599,70 @@ class CudaOps:
                                              *self._pool4(cache, n_kv, d), ctx.status, self._stream()), "read_packed_rows")
 
     def _attention4(self, ctx, qkv, out, n_q, n_kv, d, scale, window, cache) -> None:
-        """:meth:`attention` over a cache in 4 bits."""
-        bt, width, rows, kp, vp, pages, page_tokens = self._pool4(cache, n_kv, d)
-        n = qkv.shape[0]
+        """:meth:`attention` over a cache in 4 bits: bfloat16 queries and head sizes 64 and 128 on tensor cores (decode rows and prompt
+        portions each have their kernel), everything else on the kernel of any size."""
+        bt, width, rows, kp, vp, pages, page_tokens = pool = self._pool4(cache, n_kv, d)
+        n, row_stride = qkv.shape[0], qkv.stride(0)
         _need(n_q > 0 and n_q % n_kv == 0 and qkv.stride(1) == 1 and qkv.shape[1] >= n_q * d, "attention: query rows")
         if n == 0:
             return
-        # tokens [at, n) on the kernel of any size
-        at = self._attention4_tuned(ctx, qkv, out, n_q, n_kv, d, scale, window, cache)
+        q, o, out_stride, window, scale = qkv.data_ptr(), out.data_ptr(), out.stride(0), int(window or 0), float(scale)
+        at = 0                                     # tokens that a tuned kernel has taken, from the front
+        if (qkv.dtype == torch.bfloat16 and (d == 128 or d == 64) and self.fast is not None and ctx.q_start is not None
+                and not (row_stride % 8 or (q | o | kp.data_ptr() | vp.data_ptr()) & 15) and ctx.n_seqs <= 65535 and n_q <= 65535):
+            lead, lead_ctx, q_len, keys = self._parts4(ctx)
+            if lead:
+                self._attention4_decode(q, row_stride, o, out_stride, n_q, n_kv, d, scale, window, pool, ctx, lead, lead_ctx)
+                at = n if ctx.decode_only else lead
+            if at < n and n_q // n_kv <= 128 and scale > 0:
+                self._attention4_prompt(q, row_stride, o, out_stride, n, n_q, n_kv, d, scale, window, pool, ctx, lead, q_len, keys)
+                at = n
         if at < n:
             self.launches += 1
+            item = qkv.element_size()
             _check(self.packed_calls.leone_attention4_any(
-                _dt(qkv.dtype), qkv[at:], qkv.stride(0), out[at:], out.stride(0), kp, vp, bt, width, ctx.seq_of_token[at:],
-                ctx.positions[at:], n - at, n_q, n_kv, d, float(scale), int(window or 0), page_tokens, pages, rows, ctx.status,
-                self._stream()), "attention (4 bits)")
+                _dt(qkv.dtype), q + at * row_stride * item, row_stride, o + at * out_stride * item, out_stride, kp, vp, bt, width,
+                ctx.seq_of_token.data_ptr() + 4 * at, ctx.positions.data_ptr() + 4 * at, n - at, n_q, n_kv, d, scale, window, page_tokens,
+                pages, rows, ctx.status, self._stream()), "attention (4 bits)")
 
-    def _attention4_tuned(self, ctx, qkv, out, n_q, n_kv, d, scale, window, cache) -> int:
-        """The bfloat16 kernels for head sizes 64 and 128: how many of the step's tokens they took (from the front)."""
-        bt = cache.block_table
-        if (self.fast is None or qkv.dtype != torch.bfloat16 or d not in (64, 128) or getattr(ctx, "q_start", None) is None or qkv.stride(0) % 8
-                or any(t.data_ptr() % 16 for t in (qkv, out, cache.k_pool, cache.v_pool)) or ctx.n_seqs > 65535 or n_q > 65535):
-            return 0
-        order = getattr(ctx, "seq_order", None)
+    def _parts4(self, ctx):
+        """``(sequences of one token in front, the longest of them, the longest portion behind them, the most keys of one)``; looked up
+        once a step."""
         if ctx.decode_only:
-            self._attention4_decode(qkv, out, n_q, n_kv, d, scale, window, cache, ctx, ctx.n_seqs, int(ctx.max_ctx_len), order)
-            return qkv.shape[0]
-        lead = self._leading_single_rows(ctx)
-        if lead:
-            self._attention4_decode(qkv, out, n_q, n_kv, d, scale, window, cache, ctx, lead, int(ctx.ctx_lens[:lead].max()), order)
-        if n_q // n_kv > 128 or not scale > 0:
-            return lead
-        q_len = int(ctx.q_lens[lead:].max()) if lead else int(ctx.max_q_len)
-        n, n_seqs, group = qkv.shape[0], ctx.n_seqs - lead, n_q // n_kv
-        keys = int(ctx.ctx_lens[lead:].max()) if lead else int(ctx.max_ctx_len)
-        splits = self.choose_prompt4_splits(n_seqs, n_kv, group, q_len, min(keys, window + q_len) if window else keys)
+            return ctx.n_seqs, int(ctx.max_ctx_len), 0, 0
+        parts = getattr(ctx, "parts4", None)
+        if parts is None:
+            lead = self._leading_single_rows(ctx)
+            if lead:
+                parts = lead, int(ctx.ctx_lens[:lead].max()), int(ctx.q_lens[lead:].max()), int(ctx.ctx_lens[lead:].max())
+            else:
+                parts = 0, 0, int(ctx.max_q_len), int(ctx.max_ctx_len)
+            ctx.parts4 = parts
+        return parts
+
+    def _attention4_prompt(self, q, row_stride, o, out_stride, n, n_q, n_kv, d, scale, window, pool, ctx, lead, q_len, keys) -> None:
+        """Sequences ``lead ..`` of the step, with any number of tokens each (rows ``lead ..`` of the ``n``)."""
+        bt, width, rows, kp, vp, pages, page_tokens = pool
+        n_seqs, stream = ctx.n_seqs - lead, self._stream()
+        splits = self.force_prompt4_splits or \
+            self.choose_prompt4_splits(n_seqs, n_kv, n_q // n_kv, q_len, min(keys, window + q_len) if window else keys)
         part_o = part_ml = None
         if splits > 1:
-            # (rows of the step's tokens: the leading decode rows' stay unused)
-            part_o = self._scratch("attention4_parts", n * n_q * splits, d, torch.float32)
-            part_ml = self._scratch("attention4_sums", n * n_q * splits, 2, torch.float32)
+            # outputs [token][head][split][d], then (maximum, sum) [token][head][split]; the leading decode rows' stay unused
+            count = n * n_q * splits
+            part_o = self._scratch("attention4_parts", -(-count * (d + 2) // 1024), 1024, torch.float32).data_ptr()
+            part_ml = part_o + 4 * count * d
+            self.launches += 1
         self.launches += 1
         _check(self.fast.calls.leone_attention4_prefill(
-            qkv, qkv.stride(0), out, out.stride(0), cache.k_pool, cache.v_pool, bt[lead:], bt.shape[1], ctx.q_start[lead:],
-            ctx.ctx_len[lead:], n_seqs, q_len, n_q, n_kv, d, float(scale), int(window or 0), cache.page_tokens,
-            cache.k_pool.shape[0], splits, part_o, part_ml, ctx.status, self._stream()), "attention (4 bits, prompt)")
+            q, row_stride, o, out_stride, kp, vp, bt.data_ptr() + 4 * lead * width, width, ctx.q_start.data_ptr() + 4 * lead,
+            ctx.ctx_len.data_ptr() + 4 * lead, n_seqs, q_len, n_q, n_kv, d, scale, window, page_tokens, pages, splits, part_o, part_ml,
+            ctx.status, stream), "attention (4 bits, prompt)")
         if splits > 1:
-            self.launches += 1
+            first = lead * n_q * splits
             _check(self.packed_calls.leone_attention4_merge(
-                part_o[lead * n_q * splits:], part_ml[lead * n_q * splits:], out[lead:], out.stride(0), n - lead, n_q, d, splits,
-                self._stream()), "attention (4 bits, merge)")
-        return n
+                part_o + 4 * first * d, part_ml + 8 * first, o + 2 * lead * out_stride, out_stride, n - lead, n_q, d, splits, stream),
+                "attention (4 bits, merge)")
 
     force_prompt4_splits = 0               # > 0: the same for prompt portions
 
@@ -666,9 +688,10 @@ class CudaOps:
             s = 8
         return s, 1 < s <= 8
 
-    def _attention4_decode(self, qkv, out, n_q, n_kv, d, scale, window, cache, ctx, n_seqs, max_ctx, order) -> None:
-        """Sequences ``0 .. n_seqs - 1`` of the step, with one token each; ``order``: these, the longest first."""
-        calls, bt = self.packed_calls, cache.block_table
+    def _attention4_decode(self, q, row_stride, o, out_stride, n_q, n_kv, d, scale, window, pool, ctx, n_seqs, max_ctx) -> None:
+        """Sequences ``0 .. n_seqs - 1`` of the step, with one token each."""
+        bt, width, rows, kp, vp, pages, page_tokens = pool
+        calls, order = self.packed_calls, getattr(ctx, "seq_order", None)          # these sequences, the longest first
         if order is not None and order.numel() != n_seqs:
             raise KernelError(f"an order of {order.numel()} sequences for {n_seqs}")
         splits, in_cluster = self.choose_decode4_splits(n_seqs, n_kv, n_q // n_kv, min(max_ctx, window) if window else max_ctx)
@@ -681,9 +704,8 @@ class CudaOps:
             self.launches += 1
         self.launches += 1
         _check(calls.leone_attention4_decode(
-            qkv, qkv.stride(0), out, out.stride(0), cache.k_pool, cache.v_pool, bt, bt.shape[1], ctx.q_start, ctx.ctx_len, n_seqs,
-            n_q, n_kv, d, float(scale), int(window or 0), cache.page_tokens, cache.k_pool.shape[0], splits, 1 if in_cluster else 0,
-            order, scratch, ctx.status, self._stream()), "attention (4 bits, decode)")
+            q, row_stride, o, out_stride, kp, vp, bt, width, ctx.q_start, ctx.ctx_len, n_seqs, n_q, n_kv, d, scale, window, page_tokens,
+            pages, splits, 1 if in_cluster else 0, order, scratch, ctx.status, self._stream()), "attention (4 bits, decode)")
 
     def can_fuse_decode(self, ctx, qkv, n_q, n_kv, d) -> bool:
         """True if the attention kernel can do the q/k norm, rotation and cache write itself

@@ -16,6 +16,8 @@ import torch
 from ..csrc.build import ensure_built
 from .entry_points import EntryPoints
 
+# the forms of a product: a stream over the weights for few tokens (gemm_int8.cu), single SMs (gemm_narrow.cu), pairs (gemm_pair.cu)
+STREAM, NARROW, PAIRS = 0, 1, 2
 MAX_K = 1 << 17            # sums of 127 * 127 * MAX_K stay in 32 bits
 
 
@@ -65,28 +67,70 @@ class Int8Products:
             self.lib.leone_bf16_set_pdl(1 if ops._pdl else 0)
         self.calls = EntryPoints(self.lib)
         self.sm_count = torch.cuda.get_device_properties(ops.device).multi_processor_count
+        self.plans, self.buffers, self.retired = {}, {}, []
 
-    force = None               # (on pairs of SMs, tile width) of every product, whatever the rule says (tests set it)
+    force = None               # (form, splits or tile width) of every product, whatever the rule says (tests set it)
 
-    def choose(self, m: int, n: int, k: int, gated: bool):
-        """``(on pairs of SMs, weight rows per tile)``."""
-        if m > 128:
-            return True, 256
-        return False, 32 * max(1, min(8, -(-n // (32 * self.sm_count))))
+    def choose(self, m: int, n: int, k: int):
+        """The form of a product: ``(STREAM, splits)``, ``(NARROW, tile width)`` or ``(PAIRS, tile width)``.  Times below with the rounding of
+        the tokens, from cold caches.
+
+        Up to 32 tokens the stream: 8 tokens 24576 x 4096 30.9 us (33.2 on narrow tiles), 4096 x 12288 21.2 (24.8).  Its splits of K until nine
+        tenths of the SMs' places (two each) are taken, which clusters of up to 8 find.
+        From there to 128 narrow tiles of the width of the lowest estimate, in us: 3.2, 0.012 for every tile past 64, for every
+        round of tiles over the SMs and k-block 0.12 + 0.0007 a weight row (no less than the weights at 6 MB a us), and 0.02 a weight
+        row for the last tile's epilogue.  64 tokens 24576 x 4096: 34.9 us with 64 rows, 35.0 with 96, 39.1 with 192, 41 with 32.
+        From 129 on pairs, the width likewise: 2.3 + 0.016 a weight row and for every round over the pairs and k-block the longest of
+        0.18, 0.0013 a weight row and the operands at 18 MB a us.  512 tokens 2048 x 6144: 30.9 us with 128 rows, 41.0 with 256;
+        2,048 tokens 24576 x 4096: 133 with 224, 136 with 192 and 256, 152 with 128."""
+        k_blocks, best = -(-k // 128), None
+        if m <= 32:
+            return STREAM, max(1, min(8, 2 * self.sm_count * 9 // 10 // -(-n // 128), k_blocks // 2))
+        for w in range(256, 31, -32):
+            tiles = -(-n // w)
+            if m <= 128:
+                cost = max(3.2 + 0.012 * max(0, min(tiles, self.sm_count) - 64) + -(-tiles // self.sm_count) * k_blocks * (0.12 + 0.0007 * w),
+                           n * k / 6e6) + 0.02 * w
+            else:
+                pairs, tiles = self.sm_count // 2, tiles * -(-m // 256)
+                block = max(0.18, 0.0013 * w, min(tiles, pairs) * (256 + w) * 128 / 18e6)
+                cost = 2.3 + 0.016 * w + -(-tiles // pairs) * k_blocks * block
+            if best is None or cost < 0.99 * best[0]:
+                best = (cost, w)
+        return (NARROW if m <= 128 else PAIRS), best[1]
 
     def run(self, x, w: Int8Matrix, out, epilogue, residual, gate_shape) -> int:
         """A product of ``x`` with ``w``; returns the number of launches."""
-        from .cuda import _check, _dt
+        ops = self.ops
         m, k = x.shape
         n = w.out_features
-        stream = self.ops._stream()
-        codes = self.ops._scratch("int8_codes", m, k, torch.int8)
-        scales = self.ops._scratch("int8_scales", m, 1, torch.float32)
-        _check(self.ops.packed_calls.leone_quantize_rows(_dt(x.dtype), x, m, k, x.stride(0), codes, scales, stream), "quantize_rows")
-        shape = None if gate_shape is None else (c_float * 4)(*[float(v) for v in gate_shape])
-        gs = None if shape is None else addressof(shape)
-        pairs, width = self.force or self.choose(m, n, k, epilogue == 3)
-        entry = self.calls.leone_gemm_pair_i8 if pairs else self.calls.leone_gemm_narrow_i8
-        _check(entry(codes, scales, w.weight, w.scales, out, residual, m, n, k, k, k, out.stride(0), epilogue, width, self.ops.status,
-                     self.sm_count, gs, w.bias, stream), "gemm_int8")
+        plan = self.plans.get((m, n, k))
+        if plan is None:
+            plan = self.plans[m, n, k] = self.choose(m, n, k)
+        form, width = self.force or plan
+        stream = ops._stream()
+        codes, scales = self.tokens(m, k, stream)
+        gs = None
+        if gate_shape is not None:
+            shape = (c_float * 4)(*[float(v) for v in gate_shape])
+            gs = addressof(shape)
+        code = self.calls.leone_linear_i8(1 if x.dtype == torch.bfloat16 else 0, x, x.stride(0), codes, scales, w.weight, w.scales, out,
+                                          residual, m, n, k, out.stride(0), epilogue, form, width, ops.status, self.sm_count, gs, w.bias,
+                                          stream)
+        if code != 0:
+            from .cuda import _check
+            _check(code, "linear (8 bits)")
         return 2
+
+    def tokens(self, m: int, k: int, stream):
+        """Codes and scales of ``m`` tokens: one buffer for each width and stream, which only grows; an outgrown one stays for captured graphs
+        that use it."""
+        key = (k, stream)
+        held = self.buffers.get(key)
+        if held is None or held[0].shape[0] < m:
+            if held is not None:
+                self.retired.append(held)
+            rows = max(m, 64 if held is None else 2 * held[0].shape[0])
+            held = self.buffers[key] = (torch.empty((rows, k), dtype=torch.int8, device=self.ops.device),
+                                        torch.empty(rows, dtype=torch.float32, device=self.ops.device))
+        return held

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from leone_b200.ops.cuda import KernelError
-from leone_b200.ops.int8 import quantize_matrix
+from leone_b200.ops.int8 import NARROW, PAIRS, STREAM, quantize_matrix
 from tests.fewer_bits import quantize8
 
 pytestmark = pytest.mark.gpu
@@ -78,23 +78,30 @@ def test_linear(ops_of, m, n, k, dtype, bias):
     _check(stream, want + zero + residual.double(), residual.double().abs() + zero.abs(), FP32)
 
 
-@pytest.mark.parametrize("form", [(pairs, width) for pairs in (False, True) for width in (32, 64, 96, 128, 192, 224, 256)])
+@pytest.mark.parametrize("form", [(form, width) for form in (NARROW, PAIRS) for width in (32, 64, 96, 128, 192, 224, 256)]
+                         + [(STREAM, splits) for splits in range(1, 9)])
 def test_forms(ops_of, form):
-    """Every tile width on single SMs and on pairs, whatever the rule would take."""
+    """Every tile width on single SMs and on pairs and every split of the stream, whatever the rule would take."""
     ops = ops_of(BF16)
-    for m, n, k in [(1, 400, 272), (130, 1056, 1040), (257, 96, 4096)]:
+    sizes = [(1, 400, 272), (17, 1056, 1040), (32, 96, 4096), (7, 4000, 128)] if form[0] == STREAM else \
+        [(1, 400, 272), (130, 1056, 1040), (257, 96, 4096)]
+    for m, n, k in sizes:
         x, codes, scales = _inputs(m, n, k, BF16, m)
         w = ops.prepare_matrix_int8(codes, scales)
         out, wide = torch.empty((m, n), dtype=BF16, device=DEV), torch.empty((m, n), device=DEV)
+        residual = torch.randn((m, n), generator=_gen(8), device=DEV)
+        stream = residual.clone()
         ops.int8.force = form
         try:
             ops.linear(x, w, out)
             ops.linear(x, w, wide)
+            ops.linear(x, w, stream, residual=stream)
         finally:
             ops.int8.force = None
         want = _want(x, codes, scales)
         _check(out, want, want * 0, BF16)
         _check(wide, want, want * 0, FP32)
+        _check(stream, want + residual.double(), residual.double(), FP32)
 
 
 GATES = [None, (1.0, 7.0, 1.0, 0.0), (1.595769, math.inf, 0.0, 0.044715)]
@@ -164,6 +171,18 @@ def test_codes_at_the_border_of_two(ops_of):
     out = torch.empty((3, k), device=DEV)
     ops.linear(x, w, out)
     assert torch.equal(out.double(), torch.round(x.double()))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("k,lead", [(16, 0), (2048, 0), (2048, 1), (4112, 8), (16384, 0), (16400, 0), (20000, 0)])
+def test_codes_of_tokens(ops_of, dtype, k, lead):
+    """Rows as the kernels round them, for every form that the rounding has."""
+    ops = ops_of(dtype)
+    x = torch.randn((5, k + 16), generator=_gen(k), device=DEV).to(dtype)[:, lead:lead + k]
+    codes, scales = torch.empty((5, k), dtype=torch.int8, device=DEV), torch.empty(5, device=DEV)
+    assert ops.int8.calls.leone_quantize_rows(0 if dtype == FP32 else 1, x, 5, k, x.stride(0), codes, scales, ops._stream()) == 0
+    want, s = quantize8(x.double())
+    assert torch.equal(codes.double(), want) and torch.equal(scales, s[:, 0].float())
 
 
 def test_strided_inputs_and_outputs(ops_of):
