@@ -133,7 +133,209 @@ __global__ void append_kernel(T* __restrict__ qkv, int n_tokens, int n_q, int n_
   }
 }
 
-// What the pages hold for the step's tokens: rows [n_tokens][n_kv * d] of keys and of values.  One warp per (token, cached head).
+// The same for heads of 64 and 128 elements that rotate whole or not at all.  grid = (tokens, blocks of heads); a warp takes `per` heads
+// one after the other, with its token's place, rotation and norm weights at hand; lane l has elements E l .. E l + E - 1.
+//
+// Codes are still those of 64 bits, but computed in 32 where that is certain.  The factor of the norm is formed in 64 bits and
+// rounded once; then a key is off by at most kKeyError (|a| + |b|) (|cos| + |sin|) of its pair's elements before the rotation (three
+// roundings to each of them, a product's and a sum's), so the group's minimum and maximum are known to within the largest such error, and where both
+// ends of that range give the same z and the same s, those are right.  A quotient (x - z) / s is off by its key's error over s
+// and three roundings; where it comes no nearer than that to a border of two codes, so is its code.  Where anything is in doubt, or not
+// finite, the warp computes the row again in 64 bits (one row in a thousand).  2,048 tokens of 48 heads: FIG us, the form above FIG.
+constexpr float kKeyError = 4.2e-7f;            // 7 x 2^-24: factor, two products, a product and a sum, and what follows from them
+constexpr int kAppendWarps = 4;
+
+template <typename T, typename TW, int E>
+__global__ void __launch_bounds__(32 * kAppendWarps)
+append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__ q_w, const TW* __restrict__ k_w, float eps,
+                  const float2* __restrict__ rope, int max_positions, const int* __restrict__ positions,
+                  const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int table_width, int n_seqs,
+                  uint8_t* __restrict__ k_pool, uint8_t* __restrict__ v_pool, int num_pages, int page_tokens, int adjacent, int per,
+                  int* status) {
+  constexpr int D = 32 * E, G = D / 64, kGroupLanes = 32 / G;
+  pdl_trigger();
+  pdl_wait();
+  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int heads = n_q + 2 * n_kv;
+  const int h0 = (blockIdx.y * kAppendWarps + warp) * per, h1 = min(heads, h0 + per);
+  if (h0 >= h1) return;
+  T* tok = qkv + (size_t)t * heads * D + lane * E;
+  auto fetch = [&](int h, float (&v)[E]) {
+    __align__(16) T raw[E];
+    if constexpr (sizeof(T) * E == 16) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(tok + (size_t)h * D);
+    else if constexpr (sizeof(T) * E == 8) *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(tok + (size_t)h * D);
+    else *reinterpret_cast<uint32_t*>(raw) = *reinterpret_cast<const uint32_t*>(tok + (size_t)h * D);
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = to_float<T>(raw[i]);
+  };
+  float next[E];
+  fetch(h0, next);
+  const int pos = positions[t];
+  const bool rotate = rope != nullptr;
+  const bool in_table = !rotate || (pos >= 0 && pos < max_positions);
+  if (!in_table && lane == 0) set_status(status, kBadPosition, t, pos);
+  Place place;
+  const bool placed = h1 <= n_q || find_place(place, t, pos, seq_of_token, n_seqs, block_table, table_width, num_pages, page_tokens, status,
+                                              lane == 0);
+  // the lane's pairs: elements (i, i + D / 2) share cs[i] between lanes l and l ^ 16, elements (2 i, 2 i + 1) cs[2 i] in the lane
+  float2 cs[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int pair = adjacent ? (lane * E + i) >> 1 : (lane & 15) * E + i;
+    cs[i] = rotate && in_table ? rope[(size_t)pos * (D / 2) + pair] : make_float2(1.f, 0.f);
+  }
+  for (int h = h0; h < h1; ++h) {
+    float x[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = next[i];
+    if (h + 1 < h1) fetch(h + 1, next);
+    const bool is_q = h < n_q, is_k = !is_q && h < n_q + n_kv, turns = rotate && (is_q || is_k);
+    if ((turns && !in_table) || (!is_q && !placed)) continue;
+    const TW* w = is_q ? q_w : (is_k ? k_w : nullptr);
+    double factor = 1.0;
+    float y[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) y[i] = x[i];
+    if (w != nullptr) {
+      double ss = 0.0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) ss = fma((double)x[i], (double)x[i], ss);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      factor = rsqrt(ss / D + (double)eps);
+      const float f = (float)factor;
+#pragma unroll
+      for (int i = 0; i < E; ++i) y[i] = x[i] * to_float<TW>(w[lane * E + i]) * f;
+    }
+    float err = 0.f;                                       // the largest that an element of this lane may be off
+    float off[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) off[i] = 0.f;
+    if (is_k) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) off[i] = w != nullptr ? fabsf(y[i]) * kKeyError : 0.f;
+    }
+    if (turns) {
+      if (adjacent) {
+#pragma unroll
+        for (int i = 0; i < E; i += 2) {
+          const float a = y[i], b = y[i + 1];
+          off[i] = off[i + 1] = (fabsf(a) + fabsf(b)) * ((fabsf(cs[i].x) + fabsf(cs[i].y)) * kKeyError);
+          y[i] = a * cs[i].x - b * cs[i].y;
+          y[i + 1] = a * cs[i].y + b * cs[i].x;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          const float other = __shfl_xor_sync(0xffffffffu, y[i], 16);
+          off[i] = (fabsf(y[i]) + fabsf(other)) * ((fabsf(cs[i].x) + fabsf(cs[i].y)) * kKeyError);
+          y[i] = lane >= 16 ? other * cs[i].y + y[i] * cs[i].x : y[i] * cs[i].x - other * cs[i].y;
+        }
+      }
+    }
+    if (is_q) {
+      __align__(16) T out[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) out[i] = from_float<T>(y[i]);
+      T* dst = tok + (size_t)h * D;
+      if constexpr (sizeof(T) * E == 16) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(out);
+      else if constexpr (sizeof(T) * E == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(out);
+      else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(out);
+      continue;
+    }
+    // the group's range, and the largest error in it
+    float lo = y[0], hi = y[0];
+    bool doubt = false;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      doubt |= !(fabsf(y[i]) < INFINITY);
+      lo = fminf(lo, y[i]);
+      hi = fmaxf(hi, y[i]);
+      err = fmaxf(err, off[i]);
+    }
+#pragma unroll
+    for (int o = kGroupLanes / 2; o > 0; o >>= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, o));
+    }
+    float z = __bfloat162float(__float2bfloat16_rd(lo - err));
+    doubt |= z != __bfloat162float(__float2bfloat16_rd(lo + err));
+    // (hi - z) / 15 with what its ends and its own five roundings leave open
+    float s = __bfloat162float(__float2bfloat16_ru((hi - z - err) * (1.f / 15.f) * (1.f - 6e-7f)));
+    doubt |= s != __bfloat162float(__float2bfloat16_ru((hi - z + err) * (1.f / 15.f) * (1.f + 6e-7f)));
+    doubt |= (s != 0.f && !(s > 1e-37f && s < 1e37f)) || !(fabsf(z) < 3e38f);
+    const float inv = s > 0.f ? 1.f / s : 0.f;
+    uint32_t code[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float q = (y[i] - z) * inv, r = rintf(q);
+      doubt |= fabsf(fabsf(q - r) - 0.5f) <= fmaf(off[i], inv * 1.01f, fabsf(q) * 2.5e-7f) && s > 0.f;
+      code[i] = (uint32_t)fminf(fmaxf(r, 0.f), 15.f);
+    }
+    uint32_t sz = __float_as_uint(s) >> 16 | (__float_as_uint(z) & 0xffff0000u);
+    if (__any_sync(0xffffffffu, doubt)) {
+      // again in 64 bits, as the form above
+      double d[E], most = -INFINITY, least = INFINITY;
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < E; ++i) d[i] = w != nullptr ? (double)x[i] * ((double)to_float<TW>(w[lane * E + i]) * factor) : (double)x[i];
+      if (turns) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          if (adjacent) {
+            if (i & 1) continue;
+            const double a = d[i], b = d[i + 1];
+            d[i] = a * cs[i].x - b * cs[i].y;
+            d[i + 1] = a * cs[i].y + b * cs[i].x;
+          } else {
+            const double other = __shfl_xor_sync(0xffffffffu, d[i], 16);
+            d[i] = lane >= 16 ? other * cs[i].y + d[i] * cs[i].x : d[i] * cs[i].x - other * cs[i].y;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        odd |= !isfinite(d[i]);
+        least = fmin(least, d[i]);
+        most = fmax(most, d[i]);
+      }
+#pragma unroll
+      for (int o = kGroupLanes / 2; o > 0; o >>= 1) {
+        least = fmin(least, __shfl_xor_sync(0xffffffffu, least, o));
+        most = fmax(most, __shfl_xor_sync(0xffffffffu, most, o));
+        odd |= __shfl_xor_sync(0xffffffffu, (int)odd, o) != 0;
+      }
+      __nv_bfloat16 z16 = bf16_down(least);
+      const double z64 = __bfloat162float(z16);
+      __nv_bfloat16 s16 = bf16_up((most - z64) / 15.0);
+      if (__bfloat162float(s16) < 1.17549435e-38f) s16 = __float2bfloat16_rn(0.f);
+      odd |= !isfinite(z64) || !isfinite(__bfloat162float(s16));
+      if (odd) z16 = s16 = __ushort_as_bfloat16(0x7fc0);
+      const double s64 = __bfloat162float(s16);
+#pragma unroll
+      for (int i = 0; i < E; ++i) code[i] = !odd && s64 > 0.0 ? (uint32_t)fmin(fmax(rint((d[i] - z64) / s64), 0.0), 15.0) : 0u;
+      sz = (uint32_t)__bfloat16_as_ushort(s16) | (uint32_t)__bfloat16_as_ushort(z16) << 16;
+    }
+    // the word's lanes put their nibbles together (element 2 j in nibble j, 2 j + 1 in nibble j + 4), the first of them stores it
+    constexpr int kWordLanes = 8 / E;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < E; i += 2) word |= (code[i] | code[i + 1] << 16) << (4 * (i >> 1));
+    word <<= 4 * (E / 2) * (lane % kWordLanes);
+#pragma unroll
+    for (int o = 1; o < kWordLanes; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+    uint8_t* unit = (is_k ? k_pool : v_pool) +
+                    unit_at(place.page, n_kv, is_k ? h - n_q : h - n_q - n_kv, page_tokens, place.slot / kUnit * kUnit, D);
+    const int slot = place.slot % kUnit, w_at = lane / kWordLanes;
+    if (lane % kWordLanes == 0)
+      *reinterpret_cast<uint32_t*>(unit + (is_k ? key_word_at(slot, w_at, D) : value_word_at(slot, w_at, D))) = word;
+    if (lane % kGroupLanes == 0) *reinterpret_cast<uint32_t*>(unit + scale_at(slot, lane / kGroupLanes, D)) = sz;
+  }
+}
+
+// What the pages hold for the step's tokens: rows [n_tokens][n_kv * d] of keys and of values.  One warp per (token, cached head), a
+// lane a word of a key, then of a value.
 template <typename T>
 __global__ void read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, int n_tokens, int n_kv, int d,
                             const int* __restrict__ positions, const int* __restrict__ seq_of_token,
@@ -149,20 +351,19 @@ __global__ void read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, int n_
   if (!find_place(place, t, positions[t], seq_of_token, n_seqs, block_table, table_width, num_pages, page_tokens, status, lane == 0))
     return;
   const long long unit = unit_at(place.page, n_kv, h, page_tokens, place.slot / kUnit * kUnit, d);
-  const int slot = place.slot % kUnit, size = d / groups(d);
-  for (int w = lane; w < d / 8; w += 32) {
-    const uint32_t kw = *reinterpret_cast<const uint32_t*>(k_pool + unit + key_word_at(slot, w, d));
-    const uint32_t vw = *reinterpret_cast<const uint32_t*>(v_pool + unit + value_word_at(slot, w, d));
-    const int at = scale_at(slot, 8 * w / size, d);
-    const uint32_t ks = *reinterpret_cast<const uint32_t*>(k_pool + unit + at);
-    const uint32_t vs = *reinterpret_cast<const uint32_t*>(v_pool + unit + at);
-    T* k = k_out + item * d + 8 * w;
-    T* v = v_out + item * d + 8 * w;
+  const int slot = place.slot % kUnit, size = d / groups(d), words = d / 8;
+  for (int i = lane; i < 2 * words; i += 32) {
+    const bool key = i < words;
+    const int w = key ? i : i - words;
+    const uint8_t* from = (key ? k_pool : v_pool) + unit;
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(from + (key ? key_word_at(slot, w, d) : value_word_at(slot, w, d)));
+    const uint32_t sz = *reinterpret_cast<const uint32_t*>(from + scale_at(slot, 8 * w / size, d));
+    __align__(16) T out[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      k[e] = from_float<T>(fmaf(scale_of(ks), (float)code_of(kw, e), offset_of(ks)));
-      v[e] = from_float<T>(fmaf(scale_of(vs), (float)code_of(vw, e), offset_of(vs)));
-    }
+    for (int e = 0; e < 8; ++e) out[e] = from_float<T>(fmaf(scale_of(sz), (float)code_of(word, e), offset_of(sz)));
+    uint4* dst = reinterpret_cast<uint4*>((key ? k_out : v_out) + item * d + 8 * w);       // (d is a multiple of 8)
+#pragma unroll
+    for (int e = 0; e < (int)sizeof(T) / 2; ++e) dst[e] = reinterpret_cast<const uint4*>(out)[e];
   }
 }
 
@@ -315,6 +516,29 @@ extern "C" int leone_append4(int dtype, void* qkv, int n_tokens, int n_q, int n_
   if (n_q <= 0 || !pool_ok(d, n_kv, page_tokens, table_width, k_pool, v_pool)) return kRefusedSize;
   if (rope != nullptr && (rotary_dim <= 0 || rotary_dim > d || (rotary_dim & 1))) return kRefusedSize;
   if (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return kRefusedAlignment;
+  // Heads that rotate whole or not at all: a warp for each head of few tokens; of many, four heads a warp.
+  if ((d == 64 || d == 128) && (rope == nullptr || rotary_dim == d) && (q_w == nullptr) == (k_w == nullptr) && ((uintptr_t)qkv & 15) == 0 &&
+      (n_q + 2 * n_kv + cache4::kAppendWarps - 1) / cache4::kAppendWarps <= 65535) {
+    const int heads = n_q + 2 * n_kv, per = n_tokens <= 128 ? 1 : 4;
+    const dim3 grid(n_tokens, (heads + per * cache4::kAppendWarps - 1) / (per * cache4::kAppendWarps));
+#define LAUNCH_VEC(T, TW, E)                                                                                                     \
+  return launch_kernel(cache4::append_vec_kernel<T, TW, E>, grid, dim3(32 * cache4::kAppendWarps), 0, stream, (T*)qkv, n_q, n_kv, \
+                       (const TW*)q_w, (const TW*)k_w, eps, (const float2*)rope, max_positions, positions, seq_of_token,          \
+                       block_table, table_width, n_seqs, (uint8_t*)k_pool, (uint8_t*)v_pool, num_pages, page_tokens, adjacent, per, \
+                       status)
+    if (d == 64) {
+      if (dtype == 0 && w_dtype == 0) LAUNCH_VEC(float, float, 2);
+      if (dtype == 1 && w_dtype == 0) LAUNCH_VEC(__nv_bfloat16, float, 2);
+      if (dtype == 0 && w_dtype == 1) LAUNCH_VEC(float, __nv_bfloat16, 2);
+      if (dtype == 1 && w_dtype == 1) LAUNCH_VEC(__nv_bfloat16, __nv_bfloat16, 2);
+    } else {
+      if (dtype == 0 && w_dtype == 0) LAUNCH_VEC(float, float, 4);
+      if (dtype == 1 && w_dtype == 0) LAUNCH_VEC(__nv_bfloat16, float, 4);
+      if (dtype == 0 && w_dtype == 1) LAUNCH_VEC(float, __nv_bfloat16, 4);
+      if (dtype == 1 && w_dtype == 1) LAUNCH_VEC(__nv_bfloat16, __nv_bfloat16, 4);
+    }
+#undef LAUNCH_VEC
+  }
   const int warps = 4;
   const long long blocks = ((long long)n_tokens * (n_q + 2 * n_kv) + warps - 1) / warps;
   if (blocks > 0x7fffffff) return kRefusedSize;
@@ -337,7 +561,7 @@ extern "C" int leone_read4(int dtype, void* k_out, void* v_out, int n_tokens, in
                            const void* v_pool, int num_pages, int page_tokens, int* status, cudaStream_t stream) {
   if (n_tokens <= 0) return 0;
   if (!pool_ok(d, n_kv, page_tokens, table_width, k_pool, v_pool)) return kRefusedSize;
-  if (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return kRefusedAlignment;
+  if (((uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_out | (uintptr_t)v_out) & 15) return kRefusedAlignment;
   const int warps = 4;
   const long long blocks = ((long long)n_tokens * n_kv + warps - 1) / warps;
   if (blocks > 0x7fffffff) return kRefusedSize;

@@ -38,6 +38,9 @@ _REFUSALS = {
 }
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 class KernelError(RuntimeError):
     pass
 
@@ -193,8 +196,10 @@ class CudaOps:
     def _current_stream(self):
         """The handle of this device's current stream (through torch's own lookup of the handle: 0.2 us, where the Stream object that
         ``torch.cuda.current_stream`` makes takes 3)."""
+        if _raw_stream is None:
+            return torch.cuda.current_stream(self.device).cuda_stream
         index = self.device.index
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+        return _raw_stream(torch.cuda.current_device() if index is None else index)
 
     def pin_stream(self, on: bool) -> None:
         """Between ``pin_stream(True)`` and ``pin_stream(False)`` every launch goes to the stream

@@ -79,11 +79,19 @@ def test_append_and_read(ops_of, dtype, d, n_q, n_kv, norm, pairing, rot, page, 
     q, k, v = rows.double().unflatten(1, (n_q + 2 * n_kv, d)).split([n_q, n_kv, n_kv], 1)
     if norm:
         q, k = (x * w.double() * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) for x, w in ((q, weights[0]), (k, weights[1])))
+    partner = torch.zeros_like(q)
+    if rot:
+        turned = q[..., :rot]
+        partner[..., :rot] = torch.cat([turned[..., rot // 2:], turned[..., :rot // 2]], -1) if pairing == "half_split" else \
+            turned.unflatten(-1, (-1, 2)).flip(-1).flatten(-2)
+    pair = (q.abs() + partner.abs()).flatten(1)
     if rot:
         q, k = (rotate(x, step.pos, 10000.0, pairing, rot) for x in (q, k))
-    # queries: one rounding to the type of a 64-bit value (in two steps over fp32 for bfloat16)
+    # Queries: the norm's factor is rounded once, an element before the rotation so off by three roundings (factor, two products), and
+    # an element after it by a product's and a sum's more, of its pair's two elements: 6 x 2^-24 (|a| + |b|) with all of them, and
+    # one rounding to the type.
     want = q.flatten(1)
-    bound = want.abs() * (_half_step(dtype) + 2.0 ** -23) + 1e-30
+    bound = want.abs() * _half_step(dtype) + pair * 6 * 2.0 ** -24 + 1e-30
     assert ((got[:, :n_q * d].double() - want).abs() <= bound).all()
     assert torch.equal(got[:, n_q * d:], rows[:, n_q * d:])                    # keys and values are not written back
     held = []
