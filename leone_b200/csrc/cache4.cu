@@ -133,50 +133,48 @@ __global__ void append_kernel(T* __restrict__ qkv, int n_tokens, int n_q, int n_
   }
 }
 
-// The same for heads of 64 and 128 elements that rotate whole or not at all.  grid = (tokens, blocks of heads); a warp takes `per` heads
-// one after the other, with its token's place, rotation and norm weights at hand; lane l has elements E l .. E l + E - 1.
+// The same for heads of 64 and 128 elements that rotate whole or not at all.  grid = (tokens, blocks of `per` heads); a block brings its
+// rows into shared memory at once, then its eight warps take a head each in turn, with the token's place, rotation and norm
+// weights at hand; lane l has elements E l .. E l + E - 1.  (Rows read one ahead of their use, four heads a warp: 49 us for 2,048 tokens of 48
+// heads, most of it waiting for them.)
 //
-// Codes are still those of 64 bits, but computed in 32 where that is certain.  The factor of the norm is formed in 64 bits and
-// rounded once; then a key is off by at most kKeyError (|a| + |b|) (|cos| + |sin|) of its pair's elements before the rotation (three
-// roundings to each of them, a product's and a sum's), so the group's minimum and maximum are known to within the largest such error, and where both
-// ends of that range give the same z and the same s, those are right.  A quotient (x - z) / s is off by its key's error over s
-// and three roundings; where it comes no nearer than that to a border of two codes, so is its code.  Where anything is in doubt, or not
-// finite, the warp computes the row again in 64 bits (one row in a thousand).  2,048 tokens of 48 heads: FIG us, the form above FIG.
-constexpr float kKeyError = 4.2e-7f;            // 7 x 2^-24: factor, two products, a product and a sum, and what follows from them
-constexpr int kAppendWarps = 4;
+// Codes are still those of 64 bits, but computed in 32 where that is certain.  A key is off by at most kKeyError (|a| + |b|) (|cos| +
+// |sin|) of its pair's elements before the rotation: of 2^-24, half of the sum's nine roundings, four for the reciprocal root
+// and its argument, two products, a product and a sum.  So the group's minimum and maximum are known to within the largest such error,
+// and where both ends of that range give the same z and the same s, those are right.  A quotient (x - z) / s is off by its key's error
+// over s and three roundings; where it comes no nearer than that to a border of two codes, so is its code.  Where anything is in doubt,
+// or not finite, the warp computes the row again in 64 bits (one row of keys in two hundred).
+// 2,048 tokens of 48 heads 29 us (floor 5); the form above takes 90.
+constexpr float kKeyError = 16.f / 16777216.f;
+constexpr int kAppendWarps = 8;
+constexpr int kAppendHeads = 48;                   // of a block, at most
 
 template <typename T, typename TW, int E>
-__global__ void __launch_bounds__(32 * kAppendWarps)
+__global__ void __launch_bounds__(32 * kAppendWarps, 4)
 append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__ q_w, const TW* __restrict__ k_w, float eps,
                   const float2* __restrict__ rope, int max_positions, const int* __restrict__ positions,
                   const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int table_width, int n_seqs,
                   uint8_t* __restrict__ k_pool, uint8_t* __restrict__ v_pool, int num_pages, int page_tokens, int adjacent, int per,
                   int* status) {
-  constexpr int D = 32 * E, G = D / 64, kGroupLanes = 32 / G;
+  constexpr int D = 32 * E, G = D / 64, kGroupLanes = 32 / G, kWordLanes = 8 / E;
   pdl_trigger();
   pdl_wait();
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = n_q + 2 * n_kv;
-  const int h0 = (blockIdx.y * kAppendWarps + warp) * per, h1 = min(heads, h0 + per);
-  if (h0 >= h1) return;
-  T* tok = qkv + (size_t)t * heads * D + lane * E;
-  auto fetch = [&](int h, float (&v)[E]) {
-    __align__(16) T raw[E];
-    if constexpr (sizeof(T) * E == 16) *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(tok + (size_t)h * D);
-    else if constexpr (sizeof(T) * E == 8) *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(tok + (size_t)h * D);
-    else *reinterpret_cast<uint32_t*>(raw) = *reinterpret_cast<const uint32_t*>(tok + (size_t)h * D);
-#pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = to_float<T>(raw[i]);
-  };
-  float next[E];
-  fetch(h0, next);
+  const int h0 = blockIdx.y * per, h1 = min(heads, h0 + per);
+  struct __align__(sizeof(T) * E) Row { T e[E]; };         // a lane's elements of a head
+  extern __shared__ __align__(16) uint8_t rows_s[];
+  T* tok = qkv + (size_t)t * heads * D;
+  for (int i = threadIdx.x; i < (h1 - h0) * D * (int)sizeof(T) / 16; i += 32 * kAppendWarps) {
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(rows_s) + 16 * i;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(reinterpret_cast<const uint4*>(tok + (size_t)h0 * D) + i)
+                 : "memory");
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
   const int pos = positions[t];
   const bool rotate = rope != nullptr;
   const bool in_table = !rotate || (pos >= 0 && pos < max_positions);
   if (!in_table && lane == 0) set_status(status, kBadPosition, t, pos);
-  Place place;
-  const bool placed = h1 <= n_q || find_place(place, t, pos, seq_of_token, n_seqs, block_table, table_width, num_pages, page_tokens, status,
-                                              lane == 0);
   // the lane's pairs: elements (i, i + D / 2) share cs[i] between lanes l and l ^ 16, elements (2 i, 2 i + 1) cs[2 i] in the lane
   float2 cs[E];
 #pragma unroll
@@ -184,66 +182,83 @@ append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__
     const int pair = adjacent ? (lane * E + i) >> 1 : (lane & 15) * E + i;
     cs[i] = rotate && in_table ? rope[(size_t)pos * (D / 2) + pair] : make_float2(1.f, 0.f);
   }
-  for (int h = h0; h < h1; ++h) {
-    float x[E];
+  float w[E];
+  auto weights = [&](const TW* from) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = next[i];
-    if (h + 1 < h1) fetch(h + 1, next);
-    const bool is_q = h < n_q, is_k = !is_q && h < n_q + n_kv, turns = rotate && (is_q || is_k);
-    if ((turns && !in_table) || (!is_q && !placed)) continue;
-    const TW* w = is_q ? q_w : (is_k ? k_w : nullptr);
-    double factor = 1.0;
-    float y[E];
+    for (int i = 0; i < E; ++i) w[i] = from != nullptr ? to_float<TW>(from[lane * E + i]) : 1.f;
+  };
+  auto normed = [&](const float (&x)[E], float (&y)[E]) {
+    float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) y[i] = x[i];
-    if (w != nullptr) {
-      double ss = 0.0;
+    for (int i = 0; i < E; ++i) ss = fmaf(x[i], x[i], ss);
+    ss = warp_sum(ss);
+    const float f = rsqrtf(ss * (1.f / D) + eps);
 #pragma unroll
-      for (int i = 0; i < E; ++i) ss = fma((double)x[i], (double)x[i], ss);
+    for (int i = 0; i < E; ++i) y[i] = x[i] * w[i] * f;
+  };
+  // off[i]: how far element i may be off
+  auto turned = [&](float (&y)[E], float (&off)[E]) {
+    if (adjacent) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      factor = rsqrt(ss / D + (double)eps);
-      const float f = (float)factor;
+      for (int i = 0; i < E; i += 2) {
+        const float a = y[i], b = y[i + 1];
+        off[i] = off[i + 1] = (fabsf(a) + fabsf(b)) * ((fabsf(cs[i].x) + fabsf(cs[i].y)) * kKeyError);
+        y[i] = a * cs[i].x - b * cs[i].y;
+        y[i + 1] = a * cs[i].y + b * cs[i].x;
+      }
+    } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i) y[i] = x[i] * to_float<TW>(w[lane * E + i]) * f;
-    }
-    float err = 0.f;                                       // the largest that an element of this lane may be off
-    float off[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) off[i] = 0.f;
-    if (is_k) {
-#pragma unroll
-      for (int i = 0; i < E; ++i) off[i] = w != nullptr ? fabsf(y[i]) * kKeyError : 0.f;
-    }
-    if (turns) {
-      if (adjacent) {
-#pragma unroll
-        for (int i = 0; i < E; i += 2) {
-          const float a = y[i], b = y[i + 1];
-          off[i] = off[i + 1] = (fabsf(a) + fabsf(b)) * ((fabsf(cs[i].x) + fabsf(cs[i].y)) * kKeyError);
-          y[i] = a * cs[i].x - b * cs[i].y;
-          y[i + 1] = a * cs[i].y + b * cs[i].x;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          const float other = __shfl_xor_sync(0xffffffffu, y[i], 16);
-          off[i] = (fabsf(y[i]) + fabsf(other)) * ((fabsf(cs[i].x) + fabsf(cs[i].y)) * kKeyError);
-          y[i] = lane >= 16 ? other * cs[i].y + y[i] * cs[i].x : y[i] * cs[i].x - other * cs[i].y;
-        }
+      for (int i = 0; i < E; ++i) {
+        const float other = __shfl_xor_sync(0xffffffffu, y[i], 16);
+        off[i] = (fabsf(y[i]) + fabsf(other)) * ((fabsf(cs[i].x) + fabsf(cs[i].y)) * kKeyError);
+        y[i] = lane >= 16 ? other * cs[i].y + y[i] * cs[i].x : y[i] * cs[i].x - other * cs[i].y;
       }
     }
-    if (is_q) {
-      __align__(16) T out[E];
+  };
+  int h = h0 + warp;
+  if (h < n_q && q_w != nullptr) weights(q_w);
+  Place place;
+  const bool placed = h1 <= n_q || find_place(place, t, pos, seq_of_token, n_seqs, block_table, table_width, num_pages, page_tokens,
+                                              status, threadIdx.x == 0);
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  const Row* mine = reinterpret_cast<const Row*>(rows_s) + lane - h0 * 32;       // + 32 for every head
+  if (h < n_q) {
+    for (const int end = min(h1, n_q); h < end; h += kAppendWarps) {
+      float x[E], y[E], off[E];
+      const Row row = mine[h * 32];
 #pragma unroll
-      for (int i = 0; i < E; ++i) out[i] = from_float<T>(y[i]);
-      T* dst = tok + (size_t)h * D;
-      if constexpr (sizeof(T) * E == 16) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(out);
-      else if constexpr (sizeof(T) * E == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(out);
-      else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(out);
-      continue;
+      for (int i = 0; i < E; ++i) y[i] = x[i] = to_float<T>(row.e[i]);
+      if (q_w != nullptr) normed(x, y);
+      if (rotate) turned(y, off);
+      Row out;
+#pragma unroll
+      for (int i = 0; i < E; ++i) out.e[i] = from_float<T>(y[i]);
+      if (in_table) reinterpret_cast<Row*>(tok + (size_t)h * D)[lane] = out;
     }
-    // the group's range, and the largest error in it
+  }
+  if (h >= h1 || !placed) return;
+  if (k_w != nullptr) weights(k_w);
+  const long long unit = unit_at(place.page, n_kv, 0, page_tokens, place.slot / kUnit * kUnit, D);
+  const int slot = place.slot % kUnit, head_bytes = page_tokens * row_bytes(D);
+  const int key_at = key_word_at(slot, lane / kWordLanes, D), value_at = value_word_at(slot, lane / kWordLanes, D);
+  for (; h < h1; h += kAppendWarps) {
+    float x[E], y[E], off[E];
+    const Row row = mine[h * 32];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      y[i] = x[i] = to_float<T>(row.e[i]);
+      off[i] = 0.f;
+    }
+    const bool is_k = h < n_q + n_kv, norms = is_k && k_w != nullptr, turns = is_k && rotate;
+    if (turns && !in_table) continue;
+    float err = 0.f;                                       // the largest of off in the group
+    if (norms) {
+      normed(x, y);
+#pragma unroll
+      for (int i = 0; i < E; ++i) off[i] = fabsf(y[i]) * kKeyError;
+    }
+    if (turns) turned(y, off);
     float lo = y[0], hi = y[0];
     bool doubt = false;
 #pragma unroll
@@ -251,13 +266,17 @@ append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__
       doubt |= !(fabsf(y[i]) < INFINITY);
       lo = fminf(lo, y[i]);
       hi = fmaxf(hi, y[i]);
-      err = fmaxf(err, off[i]);
+    }
+    if (is_k) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) err = fmaxf(err, off[i]);
+#pragma unroll
+      for (int o = kGroupLanes / 2; o > 0; o >>= 1) err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, o));
     }
 #pragma unroll
     for (int o = kGroupLanes / 2; o > 0; o >>= 1) {
       lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
       hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, o));
     }
     float z = __bfloat162float(__float2bfloat16_rd(lo - err));
     doubt |= z != __bfloat162float(__float2bfloat16_rd(lo + err));
@@ -265,21 +284,36 @@ append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__
     float s = __bfloat162float(__float2bfloat16_ru((hi - z - err) * (1.f / 15.f) * (1.f - 6e-7f)));
     doubt |= s != __bfloat162float(__float2bfloat16_ru((hi - z + err) * (1.f / 15.f) * (1.f + 6e-7f)));
     doubt |= (s != 0.f && !(s > 1e-37f && s < 1e37f)) || !(fabsf(z) < 3e38f);
-    const float inv = s > 0.f ? 1.f / s : 0.f;
+    const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
     uint32_t code[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const float q = (y[i] - z) * inv, r = rintf(q);
-      doubt |= fabsf(fabsf(q - r) - 0.5f) <= fmaf(off[i], inv * 1.01f, fabsf(q) * 2.5e-7f) && s > 0.f;
+      const float gap = y[i] - z, q = gap * inv;
+      float r = rintf(q);
+      if (fabsf(fabsf(q - r) - 0.5f) <= fmaf(off[i], inv * 1.01f, fabsf(q) * 2.5e-7f) && s > 0.f) {
+        // An element that is known exactly (a value) and an exact difference: the sign of gap - (k + 1/2) s is exact too, and a tie
+        // goes to the even code.  (Values in bfloat16 lie on a border more often than not in a row.)
+        const float low = floorf(q), back = y[i] - gap, side = fmaf(-(low + 0.5f), s, gap);
+        doubt |= off[i] != 0.f || (y[i] - (gap + back)) + (back - z) != 0.f;
+        r = side > 0.f || (side == 0.f && ((int)low & 1)) ? low + 1.f : low;
+      }
       code[i] = (uint32_t)fminf(fmaxf(r, 0.f), 15.f);
     }
     uint32_t sz = __float_as_uint(s) >> 16 | (__float_as_uint(z) & 0xffff0000u);
     if (__any_sync(0xffffffffu, doubt)) {
       // again in 64 bits, as the form above
-      double d[E], most = -INFINITY, least = INFINITY;
+      double d[E], most = -INFINITY, least = INFINITY, factor = 1.0;
       bool odd = false;
+      if (norms) {
+        double ss = 0.0;
 #pragma unroll
-      for (int i = 0; i < E; ++i) d[i] = w != nullptr ? (double)x[i] * ((double)to_float<TW>(w[lane * E + i]) * factor) : (double)x[i];
+        for (int i = 0; i < E; ++i) ss = fma((double)x[i], (double)x[i], ss);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        factor = rsqrt(ss / D + (double)eps);
+      }
+#pragma unroll
+      for (int i = 0; i < E; ++i) d[i] = norms ? (double)x[i] * ((double)w[i] * factor) : (double)x[i];
       if (turns) {
 #pragma unroll
         for (int i = 0; i < E; ++i) {
@@ -318,52 +352,50 @@ append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__
       sz = (uint32_t)__bfloat16_as_ushort(s16) | (uint32_t)__bfloat16_as_ushort(z16) << 16;
     }
     // the word's lanes put their nibbles together (element 2 j in nibble j, 2 j + 1 in nibble j + 4), the first of them stores it
-    constexpr int kWordLanes = 8 / E;
     uint32_t word = 0;
 #pragma unroll
     for (int i = 0; i < E; i += 2) word |= (code[i] | code[i + 1] << 16) << (4 * (i >> 1));
     word <<= 4 * (E / 2) * (lane % kWordLanes);
 #pragma unroll
     for (int o = 1; o < kWordLanes; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-    uint8_t* unit = (is_k ? k_pool : v_pool) +
-                    unit_at(place.page, n_kv, is_k ? h - n_q : h - n_q - n_kv, page_tokens, place.slot / kUnit * kUnit, D);
-    const int slot = place.slot % kUnit, w_at = lane / kWordLanes;
-    if (lane % kWordLanes == 0)
-      *reinterpret_cast<uint32_t*>(unit + (is_k ? key_word_at(slot, w_at, D) : value_word_at(slot, w_at, D))) = word;
-    if (lane % kGroupLanes == 0) *reinterpret_cast<uint32_t*>(unit + scale_at(slot, lane / kGroupLanes, D)) = sz;
+    uint8_t* to = (is_k ? k_pool + (size_t)(h - n_q) * head_bytes : v_pool + (size_t)(h - n_q - n_kv) * head_bytes) + unit;
+    if (lane % kWordLanes == 0) *reinterpret_cast<uint32_t*>(to + (is_k ? key_at : value_at)) = word;
+    if (lane % kGroupLanes == 0) *reinterpret_cast<uint32_t*>(to + scale_at(slot, lane / kGroupLanes, D)) = sz;
   }
 }
 
-// What the pages hold for the step's tokens: rows [n_tokens][n_kv * d] of keys and of values.  One warp per (token, cached head), a
-// lane a word of a key, then of a value.
+// What the pages hold for the step's tokens: rows [n_tokens][n_kv * d] of keys and of values.  grid = (tokens, blocks of heads); a warp takes
+// a cached head at a time, a lane a word of its key, then of its value.
+constexpr int kReadWarps = 8;
 template <typename T>
-__global__ void read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, int n_tokens, int n_kv, int d,
-                            const int* __restrict__ positions, const int* __restrict__ seq_of_token,
-                            const int* __restrict__ block_table, int table_width, int n_seqs, const uint8_t* __restrict__ k_pool,
-                            const uint8_t* __restrict__ v_pool, int num_pages, int page_tokens, int* status) {
+__global__ void __launch_bounds__(32 * kReadWarps)
+read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, int n_kv, int d, const int* __restrict__ positions,
+            const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int table_width, int n_seqs,
+            const uint8_t* __restrict__ k_pool, const uint8_t* __restrict__ v_pool, int num_pages, int page_tokens, int* status) {
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (item >= (long long)n_tokens * n_kv) return;
-  const int t = (int)(item / n_kv), h = (int)(item - (long long)t * n_kv);
+  const int lane = threadIdx.x & 31, t = blockIdx.x;
   Place place;
-  if (!find_place(place, t, positions[t], seq_of_token, n_seqs, block_table, table_width, num_pages, page_tokens, status, lane == 0))
+  if (!find_place(place, t, positions[t], seq_of_token, n_seqs, block_table, table_width, num_pages, page_tokens, status,
+                  threadIdx.x == 0))
     return;
-  const long long unit = unit_at(place.page, n_kv, h, page_tokens, place.slot / kUnit * kUnit, d);
   const int slot = place.slot % kUnit, size = d / groups(d), words = d / 8;
-  for (int i = lane; i < 2 * words; i += 32) {
-    const bool key = i < words;
-    const int w = key ? i : i - words;
-    const uint8_t* from = (key ? k_pool : v_pool) + unit;
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(from + (key ? key_word_at(slot, w, d) : value_word_at(slot, w, d)));
-    const uint32_t sz = *reinterpret_cast<const uint32_t*>(from + scale_at(slot, 8 * w / size, d));
-    __align__(16) T out[8];
+  for (int h = blockIdx.y * kReadWarps + (threadIdx.x >> 5); h < n_kv; h += gridDim.y * kReadWarps) {
+    const long long item = (long long)t * n_kv + h;
+    const long long unit = unit_at(place.page, n_kv, h, page_tokens, place.slot / kUnit * kUnit, d);
+    for (int i = lane; i < 2 * words; i += 32) {
+      const bool key = i < words;
+      const int w = key ? i : i - words;
+      const uint8_t* from = (key ? k_pool : v_pool) + unit;
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(from + (key ? key_word_at(slot, w, d) : value_word_at(slot, w, d)));
+      const uint32_t sz = *reinterpret_cast<const uint32_t*>(from + scale_at(slot, 8 * w / size, d));
+      __align__(16) T out[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = from_float<T>(fmaf(scale_of(sz), (float)code_of(word, e), offset_of(sz)));
-    uint4* dst = reinterpret_cast<uint4*>((key ? k_out : v_out) + item * d + 8 * w);       // (d is a multiple of 8)
+      for (int e = 0; e < 8; ++e) out[e] = from_float<T>(fmaf(scale_of(sz), (float)code_of(word, e), offset_of(sz)));
+      uint4* dst = reinterpret_cast<uint4*>((key ? k_out : v_out) + item * d + 8 * w);       // (d is a multiple of 8)
 #pragma unroll
-    for (int e = 0; e < (int)sizeof(T) / 2; ++e) dst[e] = reinterpret_cast<const uint4*>(out)[e];
+      for (int e = 0; e < (int)sizeof(T) / 2; ++e) dst[e] = reinterpret_cast<const uint4*>(out)[e];
+    }
   }
 }
 
@@ -516,13 +548,15 @@ extern "C" int leone_append4(int dtype, void* qkv, int n_tokens, int n_q, int n_
   if (n_q <= 0 || !pool_ok(d, n_kv, page_tokens, table_width, k_pool, v_pool)) return kRefusedSize;
   if (rope != nullptr && (rotary_dim <= 0 || rotary_dim > d || (rotary_dim & 1))) return kRefusedSize;
   if (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return kRefusedAlignment;
-  // Heads that rotate whole or not at all: a warp for each head of few tokens; of many, four heads a warp.
+  // Heads that rotate whole or not at all.  A block has a head a warp for few tokens, all of a token's heads (up to 48) for many.
   if ((d == 64 || d == 128) && (rope == nullptr || rotary_dim == d) && (q_w == nullptr) == (k_w == nullptr) && ((uintptr_t)qkv & 15) == 0 &&
-      (n_q + 2 * n_kv + cache4::kAppendWarps - 1) / cache4::kAppendWarps <= 65535) {
-    const int heads = n_q + 2 * n_kv, per = n_tokens <= 128 ? 1 : 4;
-    const dim3 grid(n_tokens, (heads + per * cache4::kAppendWarps - 1) / (per * cache4::kAppendWarps));
+      n_q + 2 * n_kv <= 65535) {
+    const int heads = n_q + 2 * n_kv, most = n_tokens <= 96 ? cache4::kAppendWarps : cache4::kAppendHeads;
+    const int blocks_of = (heads + most - 1) / most, per = (heads + blocks_of - 1) / blocks_of;
+    const dim3 grid(n_tokens, blocks_of);
+    const size_t row_bytes = (size_t)per * d * (dtype == 0 ? 4 : 2);
 #define LAUNCH_VEC(T, TW, E)                                                                                                     \
-  return launch_kernel(cache4::append_vec_kernel<T, TW, E>, grid, dim3(32 * cache4::kAppendWarps), 0, stream, (T*)qkv, n_q, n_kv, \
+  return launch_kernel(cache4::append_vec_kernel<T, TW, E>, grid, dim3(32 * cache4::kAppendWarps), row_bytes, stream, (T*)qkv, n_q, n_kv, \
                        (const TW*)q_w, (const TW*)k_w, eps, (const float2*)rope, max_positions, positions, seq_of_token,          \
                        block_table, table_width, n_seqs, (uint8_t*)k_pool, (uint8_t*)v_pool, num_pages, page_tokens, adjacent, per, \
                        status)
@@ -562,12 +596,11 @@ extern "C" int leone_read4(int dtype, void* k_out, void* v_out, int n_tokens, in
   if (n_tokens <= 0) return 0;
   if (!pool_ok(d, n_kv, page_tokens, table_width, k_pool, v_pool)) return kRefusedSize;
   if (((uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)k_out | (uintptr_t)v_out) & 15) return kRefusedAlignment;
-  const int warps = 4;
-  const long long blocks = ((long long)n_tokens * n_kv + warps - 1) / warps;
-  if (blocks > 0x7fffffff) return kRefusedSize;
+  const int blocks = (n_kv + cache4::kReadWarps - 1) / cache4::kReadWarps;
+  const dim3 grid(n_tokens, blocks < 65535 ? blocks : 65535);
 #define LAUNCH(T)                                                                                                            \
-  return launch_kernel(cache4::read_kernel<T>, dim3((unsigned)blocks), dim3(warps * 32), 0, stream, (T*)k_out, (T*)v_out,    \
-                       n_tokens, n_kv, d, positions, seq_of_token, block_table, table_width, n_seqs, (const uint8_t*)k_pool, \
+  return launch_kernel(cache4::read_kernel<T>, grid, dim3(32 * cache4::kReadWarps), 0, stream, (T*)k_out, (T*)v_out,         \
+                       n_kv, d, positions, seq_of_token, block_table, table_width, n_seqs, (const uint8_t*)k_pool, \
                        (const uint8_t*)v_pool, num_pages, page_tokens, status)
   if (dtype == 0) LAUNCH(float);
   if (dtype == 1) LAUNCH(__nv_bfloat16);
