@@ -11,7 +11,7 @@
 // the smallest exponent have one step), so of a word a code in bits 0-3 is c 2^-133, one in bits 4-7 is 16 c 2^-133.  Queries
 // and weights are multiplied by 2^48 before (the queries that meet bits 4-7 by 2^44), so that the sums lie in the middle of fp32's range,
 // and the sums by 2^85 after; both are exact while queries stay below 2^79 and scales below 2^40.  (128 + c by AND-OR, which needs
-// a shift for every code but a word's first and the 128 taken out again, took 425 instructions for 16 keys where this takes 330.)
+// a shift for every code but a word's first and the 128 taken out again, took 425 instructions for 16 keys of 128 where this takes 311.)
 //
 // Keys ride the MMA's M side and up to 8 query heads its N side (NT tiles of them), as in attention_tiled.cu.  The pages' layout is
 // made so that a thread's operands are words that lie side by side: 16 keys are one piece of 1,152 bytes (576 with 64 elements) for

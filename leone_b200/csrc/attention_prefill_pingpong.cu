@@ -59,7 +59,7 @@ constexpr int kTileThreads = kTileWarps * 32;
 constexpr int kMmaWarp = 2 * kTileWarps;
 constexpr int kLoadWarp0 = kMmaWarp + 1;   // two warps gather keys, the next two values
 constexpr int kStreamThreads = 64;         // threads that gather one kind of tile (a thread per two key rows)
-// Pages in 4 bits: twice as many, who also convert them (2,048 tokens behind 6,144 on 32 and 8 heads of 128: 383 us; 447 with 64 threads)
+// Pages in 4 bits: twice as many, who also convert them (383 us where 64 threads for each kind took 447)
 constexpr int stream_threads(int form) { return form == 3 ? 128 : kStreamThreads; }
 constexpr int block_threads(int form) { return kLoadWarp0 * 32 + 2 * stream_threads(form); }
 constexpr float kLog2e = 1.4426950408889634f;
@@ -200,14 +200,18 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 
 // Pages in 4 bits (cache4.cuh; kernel form 3, ordinary softmax).  A tile's keys, and its values, are eight units that the TMA copies
 // into shared memory as they lie in their pages, one tile ahead; the gathering warps turn them into the 16-bit operand tiles: a word of
-// codes is the 16-byte piece of its row, a pair of codes becomes an offset + c by AND-OR, c by a subtraction and z + s c by one FMA, which
-// rounds once.
+// codes is the 16-byte piece of its row, and a pair of its codes becomes z + s c by an AND and an FMA, which rounds once.  For as a bit
+// pattern a code in bits 0-3 is the subnormal number c 2^-24 of fp16, or c 2^-133 of bfloat16, and one in bits 4-7 is 16 times that (for
+// bfloat16 the eighth bit is the exponent's lowest, and the numbers up to there have one step); s is multiplied by the other power
+// of two before.  A tile is taken into registers whole, so that the next one can be asked for before it is converted (2,048 tokens behind
+// 6,144 on 32 and 8 heads of 128: 348 us, 381 where it was asked for after that).
 //
 // Values become bfloat16, and so do the weights, as in the other forms.  Keys become fp16, and queries are fp16 too, which is exact:
 // z + s c has 12 significant bits and more, and rounded to the 8 of bfloat16 its error in the scores was most of the output's (8,192
 // keys with a spread of scores of 3: 0.0075 of the output's norm, 0.0026 with the 11 of fp16).  For fp16's range a query's row is
 // multiplied by a power of two that brings its largest element to 2^7 .. 2^8, and a tile of keys by one that brings its largest value
-// below 2^15; the row's and the tile's power are taken out with the scale of the scores.
+// to 2^-8 .. 2^-7 (s 2^24 is then a number of fp16 too); the row's and the tile's power are taken out with the scale of the scores.  Values
+// are stored times 2^-64 (for s 2^133; scales up to 2^57 fit), which the outputs are multiplied with at the end.
 //
 // A value that is NaN must not reach rows that do not see its key (the product has 0 x NaN for them): such a group is stored as zeros
 // and kept in a list of keys and groups, and at the end the rows that see one of them become NaN in that group's columns.  What does not
@@ -219,7 +223,7 @@ struct OddValues {
   int key[kOddKeys];              // key * 2 + group
   int lo[2], hi[2];               // the range of further keys, per group
   unsigned units[2];              // of the tile that lands, keys and values: the units that have a page
-  int largest[4];                 // of the four warps that gather keys: the largest exponent of their rows
+  int largest[2][4];              // of the four warps that gather keys: the largest exponent of their rows of tile t % 2
   float key_power[4];             // 2^e of tile t % 4: its keys are stored times 2^-e
   float query_power[2][kRows];    // the same of a row of queries
 };
@@ -243,33 +247,27 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e 
 // The exponent of |v|, -126 at least (128: an infinity or NaN).
 __device__ __forceinline__ int exponent_of(float v) { return max((int)(__float_as_uint(v) >> 23 & 255u) - 127, -126); }
 
-// Four words of codes of a row (place q of its 16-byte pieces, at `raw`) become their chunks of the operand tile at `tile`; sz0, sz1:
-// the row's groups' scales (low half) and offsets, in bfloat16 for values and fp16 for keys.
+// Four words of codes of a row (place q of its 16-byte pieces) become their chunks of the operand tile at `tile`.  lo, hi, z: by
+// group, twice in a register: the scale that a code in bits 0-3 is multiplied with, that for bits 4-7, and the offset.
 template <int D, bool kValues>
-__device__ __forceinline__ void unpack_quad(const uint8_t* raw, uint32_t tile, int row, int q, uint32_t sz0, uint32_t sz1) {
-  const uint4 raw4 = *reinterpret_cast<const uint4*>(raw);
-  const uint32_t w[4] = {raw4.x, raw4.y, raw4.z, raw4.w};
-  constexpr uint32_t kOffset = kValues ? 0x43004300u : 0x64006400u;        // 128 in bfloat16, 1024 in fp16: what follows is c
+__device__ __forceinline__ void unpack_quad(const uint4& words, uint32_t tile, int row, int q, const uint32_t (&lo)[D / 64],
+                                            const uint32_t (&hi)[D / 64], const uint32_t (&z)[D / 64]) {
+  const uint32_t w[4] = {words.x, words.y, words.z, words.w};
+  auto value = [](uint32_t c, uint32_t s, uint32_t z) {
+    uint32_t v;
+    if constexpr (kValues) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(c), "r"(s), "r"(z));
+    else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(c), "r"(s), "r"(z));
+    return v;
+  };
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     // which word of the row stands in place 4 q + i (cache4.cuh)
     const int g = D == 64 ? 0 : (kValues ? i & 1 : i >> 1);
     const int chunk = D == 64 ? 4 * q + i : 8 * g + 2 * q + (kValues ? i >> 1 : i & 1);
-    const uint32_t sz = g == 0 ? sz0 : sz1;
-    const uint32_t s2 = __byte_perm(sz, sz, 0x1010), z2 = __byte_perm(sz, sz, 0x3232);
-    uint32_t out[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t c = ((w[i] >> (4 * j)) & 0x000f000fu) | kOffset;
-      uint32_t v;
-      if constexpr (kValues)
-        asm("{\n\t.reg .b32 t;\n\tsub.rn.bf16x2 t, %1, %2;\n\tfma.rn.bf16x2 %0, t, %3, %4;\n\t}" : "=r"(v) : "r"(c), "r"(kOffset), "r"(s2), "r"(z2));
-      else
-        asm("{\n\t.reg .b32 t;\n\tsub.rn.f16x2 t, %1, %2;\n\tfma.rn.f16x2 %0, t, %3, %4;\n\t}" : "=r"(v) : "r"(c), "r"(kOffset), "r"(s2), "r"(z2));
-      out[j] = v;
-    }
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + swizzled(row, chunk)), "r"(out[0]), "r"(out[1]), "r"(out[2]),
-                 "r"(out[3])
+    const uint32_t x = w[i], y = x >> 8;
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + swizzled(row, chunk)),
+                 "r"(value(x & 0x000f000fu, lo[g], z[g])), "r"(value(x & 0x00f000f0u, hi[g], z[g])),
+                 "r"(value(y & 0x000f000fu, lo[g], z[g])), "r"(value(y & 0x00f000f0u, hi[g], z[g]))
                  : "memory");
   }
 }
@@ -465,89 +463,116 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
       };
       if (st < 32) request(0);
       bool ok_all = true;
+      // thread st takes piece st % kQuads of rows st / kQuads, + kStep, ..: always the same row of a unit
+      constexpr int kStep = kStream / kQuads, kMine = kKeys / kStep;
+      static_assert(kStep % cache4::kUnit == 0, "a thread's rows are the same row of units");
+      const int q = st % kQuads, row0 = st / kQuads, tt = row0 % cache4::kUnit, vr = cache4::value_row(tt);
+      const uint8_t* first = raw + row0 / cache4::kUnit * kUnitBytes;
+      const uint8_t* piece = first + (values ? vr * (D / 2) + (G == 2 ? q ^ (vr & 2) : q) * 16 : tt * (D / 2) + q * 16);
+      first += cache4::scale_at(tt, 0, D);
       for (int t = 0; t < n_tiles; ++t) {
         if (ok_all && !mbar_wait_long(landed, t & 1, giveup)) ok_all = false;
-        if (t >= 2 && ok_all && !mbar_wait_long(bar_free + 8 * (t & 1), ((t >> 1) - 1) & 1, giveup)) ok_all = false;
         ok_all = __all_sync(0xffffffffu, ok_all);
         const unsigned have = ok_all ? odd.units[values] : 0u;
-        const uint32_t tile = tiles + (t & 1) * kTileBytes;
+        // What landed is taken into registers, so that the next tile's units can be asked for before this one's are converted.
+        uint4 words[kMine];
+        uint32_t sz[kMine][G];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int at = i * (kStep / cache4::kUnit) * kUnitBytes;
+          words[i] = *reinterpret_cast<const uint4*>(piece + at);
+          if constexpr (G == 2) {
+            const uint2 both = *reinterpret_cast<const uint2*>(first + at);
+            sz[i][0] = both.x;
+            sz[i][G - 1] = both.y;
+          } else {
+            sz[i][0] = *reinterpret_cast<const uint32_t*>(first + at);
+          }
+        }
         const int key0 = tile0 + t * kKeys;
         // every row of the tile is a key to be read: the same for all threads
-        const bool clean = have == (1u << kTileUnits) - 1 && key0 >= k_lo && key0 + kKeys <= k_hi;
-        float down = 1.f;
-        if (!values) {
-          // the tile's largest |z|, |z + 15 s|, a row a thread; a NaN does not count
-          int top = -126;
-          if ((have >> (st / cache4::kUnit) & 1) && key0 + st >= k_lo && key0 + st < k_hi) {
+        if (have != (1u << kTileUnits) - 1 || key0 < k_lo || key0 + kKeys > k_hi) {
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-              const uint32_t sz = *reinterpret_cast<const uint32_t*>(raw + st / cache4::kUnit * kUnitBytes +
-                                                                     cache4::scale_at(st % cache4::kUnit, g, D));
-              const float z = cache4::offset_of(sz), most = fmaxf(fabsf(z), fabsf(fmaf(15.f, cache4::scale_of(sz), z)));
-              if (most < INFINITY) top = max(top, exponent_of(most));
+          for (int i = 0; i < kMine; ++i) {
+            const int row = row0 + i * kStep;
+            if (!(have >> (row / cache4::kUnit) & 1) || key0 + row < k_lo || key0 + row >= k_hi) {
+#pragma unroll
+              for (int g = 0; g < G; ++g) sz[i][g] = 0;    // a row that is not to be read: scales and offsets 0, so all of it 0
             }
           }
+        }
+        if (values) {
+          // (z + 15 s is the largest value; what would not be a bfloat16 number, or a scale too large, counts with the NaN)
+#pragma unroll
+          for (int i = 0; i < kMine; ++i)
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const float s = cache4::scale_of(sz[i][g]);
+              if (fabsf(fmaf(15.f, s, cache4::offset_of(sz[i][g]))) <= 3.3895e38f && s <= 144115188075855872.f) continue;      // 2^57
+              sz[i][g] = 0;
+              if (q != 0) continue;
+              const int key = key0 + row0 + i * kStep, at = atomicAdd(&odd.count, 1);
+              if (at < kOddKeys) {
+                odd.key[at] = key * 2 + g;
+              } else {
+                atomicMin(&odd.lo[g], key);
+                atomicMax(&odd.hi[g], key);
+              }
+            }
+        } else {
+          // the tile's largest |z|, |z + 15 s|; a NaN does not count
+          int top = -126;
+#pragma unroll
+          for (int i = 0; i < kMine; ++i)
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const float z = cache4::offset_of(sz[i][g]), most = fmaxf(fabsf(z), fabsf(fmaf(15.f, cache4::scale_of(sz[i][g]), z)));
+              if (most < INFINITY) top = max(top, exponent_of(most));
+            }
           top = __reduce_max_sync(0xffffffffu, top);
-          if (lane == 0) odd.largest[st >> 5] = top;
-          named_barrier_sync(bar_id, kStream);
-          top = max(max(odd.largest[0], odd.largest[1]), max(odd.largest[2], odd.largest[3]));
-          const int e = min(max(top - 13, -126), 126);     // below 2^15, with what rounding adds
+          if (lane == 0) odd.largest[t & 1][st >> 5] = top;
+        }
+        named_barrier_sync(bar_id, kStream);               // the landed units are read; the next tile's may take their place
+        if (st < 32 && ok_all) request(t + 1);
+        float down = 1.f;
+        if (!values) {
+          const int* l = odd.largest[t & 1];
+          const int e = min(max(max(max(l[0], l[1]), max(l[2], l[3])) + 8, -126), 126);
           down = power_of_two(-e);
           if (st == 0) odd.key_power[t & 3] = power_of_two(e);
         }
-        // thread st takes piece st % kQuads of rows st / kQuads, + kStream / kQuads, ..: always the same row of a unit
-        constexpr int kStep = kStream / kQuads;
-        static_assert(kStep % cache4::kUnit == 0, "a thread's rows are the same row of units");
-        const int q = st % kQuads, row0 = st / kQuads, tt = row0 % cache4::kUnit, vr = cache4::value_row(tt);
-        const int piece = values ? vr * (D / 2) + (G == 2 ? q ^ (vr & 2) : q) * 16 : tt * (D / 2) + q * 16;
-        const uint8_t* unit = raw + row0 / cache4::kUnit * kUnitBytes;
-#pragma unroll 2
-        for (int row = row0; row < kKeys; row += kStep, unit += kStep / cache4::kUnit * kUnitBytes) {
-          bool zero0 = false, zero1 = false;
-          if (!clean) zero0 = zero1 = !(have >> (row / cache4::kUnit) & 1) || key0 + row < k_lo || key0 + row >= k_hi;
-          uint32_t sz0, sz1 = 0;
-          if constexpr (G == 2) {
-            const uint2 both = *reinterpret_cast<const uint2*>(unit + cache4::scale_at(tt, 0, D));
-            sz0 = both.x;
-            sz1 = both.y;
-          } else {
-            sz0 = *reinterpret_cast<const uint32_t*>(unit + cache4::scale_at(tt, 0, D));
-          }
-          if (values) {
-            // (z + 15 s is the largest value; what would not be a bfloat16 number counts with the NaN)
-            const bool odd0 = !(fabsf(fmaf(15.f, cache4::scale_of(sz0), cache4::offset_of(sz0))) <= 3.3895e38f);
-            const bool odd1 = G == 2 && !(fabsf(fmaf(15.f, cache4::scale_of(sz1), cache4::offset_of(sz1))) <= 3.3895e38f);
-            if ((odd0 || odd1) && !zero0) {
-              if (q == 0) {
+        if (t >= 2 && ok_all && !mbar_wait_long(bar_free + 8 * (t & 1), ((t >> 1) - 1) & 1, giveup)) ok_all = false;
+        ok_all = __all_sync(0xffffffffu, ok_all);
+        const uint32_t tile = tiles + (t & 1) * kTileBytes;
 #pragma unroll
-                for (int g = 0; g < G; ++g) {
-                  if (!(g == 0 ? odd0 : odd1)) continue;
-                  const int at = atomicAdd(&odd.count, 1);
-                  if (at < kOddKeys) {
-                    odd.key[at] = (key0 + row) * 2 + g;
-                  } else {
-                    atomicMin(&odd.lo[g], key0 + row);
-                    atomicMax(&odd.hi[g], key0 + row);
-                  }
-                }
-              }
-              zero0 |= odd0;
-              zero1 |= odd1;
+        for (int i = 0; i < kMine; ++i) {
+          // scales and offsets as the operand's type
+          uint32_t lo[G], hi[G], z[G];
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            const float s = cache4::scale_of(sz[i][g]), o = cache4::offset_of(sz[i][g]);
+            if (values) {
+              constexpr float kTo = 590295810358705651712.f, kLeast = 5.421010862427522e-20f;            // 2^69, 2^-64
+              const __nv_bfloat162 a = __floats2bfloat162_rn(s * kTo, s * kTo), b = __floats2bfloat162_rn(s * (kTo / 16), s * (kTo / 16)),
+                                   c = __floats2bfloat162_rn(o * kLeast, o * kLeast);
+              lo[g] = *reinterpret_cast<const uint32_t*>(&a);
+              hi[g] = *reinterpret_cast<const uint32_t*>(&b);
+              z[g] = *reinterpret_cast<const uint32_t*>(&c);
+            } else {
+              const float sd = s * down, od = o * down;
+              const __half2 a = __floats2half2_rn(sd * 16777216.f, sd * 16777216.f), b = __floats2half2_rn(sd * 1048576.f, sd * 1048576.f),
+                            c = __floats2half2_rn(od, od);
+              lo[g] = *reinterpret_cast<const uint32_t*>(&a);
+              hi[g] = *reinterpret_cast<const uint32_t*>(&b);
+              z[g] = *reinterpret_cast<const uint32_t*>(&c);
             }
-            // a zero group: codes, scale and offset 0
-            unpack_quad<D, true>(unit + piece, tile, row, q, zero0 ? 0u : sz0, zero1 ? 0u : sz1);
-          } else {
-            auto as_fp16 = [&](uint32_t sz) {
-              const __half2 v = __floats2half2_rn(cache4::scale_of(sz) * down, cache4::offset_of(sz) * down);
-              return *reinterpret_cast<const uint32_t*>(&v);
-            };
-            unpack_quad<D, false>(unit + piece, tile, row, q, zero0 ? 0u : as_fp16(sz0), G == 1 || zero1 ? 0u : as_fp16(sz1));
           }
+          if (values) unpack_quad<D, true>(words[i], tile, row0 + i * kStep, q, lo, hi, z);
+          else unpack_quad<D, false>(words[i], tile, row0 + i * kStep, q, lo, hi, z);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        named_barrier_sync(bar_id, kStream);             // the landed units are read; the next tile's may take their place
+        __syncwarp();
         if (lane == 0) mbar_arrive(bar_full + 8 * (t & 1));
-        if (st < 32 && ok_all) request(t + 1);
       }
     } else if (warp >= kLoadWarp0) {
       // ---------------- the warps that gather the tiles ----------------
@@ -845,6 +870,8 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
         tc_fence_after();
         float inv = (rules.weights == 2 ? 1.f : (l_row > 0.f ? 1.f / l_row : 0.f)) * (kPooled ? pooled.out_scale : 1.f);
         if constexpr (kPacked) {
+          constexpr float kUp = 18446744073709551616.f;    // 2^64: the values were stored times 2^-64
+          inv *= kUp;
           const int count = odd.count;                     // (almost always 0)
           if (count > 0 && my_pos >= 0) {
             const int g = D == 64 ? 0 : half, from = window > 0 ? max(0, my_pos - window + 1) : 0;
@@ -856,7 +883,7 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
             if (sees) inv = NAN;
           }
           if (parts.part_o != nullptr) {                   // this split's part, as it is
-            const float as_is = isnan(inv) && !isnan(l_row) ? inv : 1.f;
+            const float as_is = isnan(inv) && !isnan(l_row) ? inv : kUp;
             const bool store = ok_all && my_pos >= 0;
             if (store && half == 0) *reinterpret_cast<float2*>(parts.part_ml + part_row * 2) = make_float2(m_run, l_row);
             float4* dst = reinterpret_cast<float4*>(parts.part_o + part_row * D + half * (D / 2));
