@@ -53,6 +53,22 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a) {          // an 8x8 
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
+// Loads of a stage: after the wait for it and before the next request into it, which are volatile too; free to move among the rest.
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
 constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;           // codes as c 2^-133 and as 16 c 2^-133
 constexpr uint32_t kMinus8 = 0x80088008u;                              // -8 2^-133, twice
 constexpr float kUp = 281474976710656.f;                              // 2^48
@@ -114,23 +130,23 @@ struct Warp4 {
   }
 
   // The keys' words of a unit are multiplied with the queries: st += (its scores of keys gid and gid + 8) * scale * log2 e.
-  __device__ __forceinline__ void scores(const uint8_t* k_s, float (&st)[NT][4], float back, int gid, int tig) {
+  __device__ __forceinline__ void scores(uint32_t k_s, float (&st)[NT][4], float back, int gid, int tig) {
     uint32_t w0[2 * G], w1[2 * G], p0[G], p1[G];
-    const uint8_t* at = k_s + gid * (D / 2) + tig * (8 * G);
+    const uint32_t at = k_s + gid * (D / 2) + tig * (8 * G);
     if constexpr (G == 2) {
-      const uint4 a = *reinterpret_cast<const uint4*>(at), b = *reinterpret_cast<const uint4*>(at + 8 * (D / 2));
+      const uint4 a = lds128(at), b = lds128(at + 8 * (D / 2));
       w0[0] = a.x; w0[1] = a.y; w0[2] = a.z; w0[3] = a.w;
       w1[0] = b.x; w1[1] = b.y; w1[2] = b.z; w1[3] = b.w;
-      const uint2 c = *reinterpret_cast<const uint2*>(k_s + kScales + gid * 8);
-      const uint2 d = *reinterpret_cast<const uint2*>(k_s + kScales + gid * 8 + 64);
+      const uint2 c = lds64(k_s + kScales + gid * 8);
+      const uint2 d = lds64(k_s + kScales + gid * 8 + 64);
       p0[0] = c.x; p0[1] = c.y;
       p1[0] = d.x; p1[1] = d.y;
     } else {
-      const uint2 a = *reinterpret_cast<const uint2*>(at), b = *reinterpret_cast<const uint2*>(at + 8 * (D / 2));
+      const uint2 a = lds64(at), b = lds64(at + 8 * (D / 2));
       w0[0] = a.x; w0[1] = a.y;
       w1[0] = b.x; w1[1] = b.y;
-      p0[0] = *reinterpret_cast<const uint32_t*>(k_s + kScales + gid * 4);
-      p1[0] = *reinterpret_cast<const uint32_t*>(k_s + kScales + gid * 4 + 32);
+      p0[0] = lds32(k_s + kScales + gid * 4);
+      p1[0] = lds32(k_s + kScales + gid * 4 + 32);
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -169,7 +185,7 @@ struct Warp4 {
   }
 
   // A unit's values times the weights p of keys gid and gid + 8 join the outputs; keep0, keep1: whether those keys are seen.
-  __device__ __forceinline__ void outputs(const uint8_t* v_s, const float (&p)[NT][4], bool whole, bool keep0, bool keep1, int gid,
+  __device__ __forceinline__ void outputs(uint32_t v_s, const float (&p)[NT][4], bool whole, bool keep0, bool keep1, int gid,
                                           int tig) {
     uint2 v[4];
     uint32_t q0[G], q1[G];
@@ -177,17 +193,17 @@ struct Warp4 {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = tig + 4 * i;
-        v[i] = *reinterpret_cast<const uint2*>(v_s + row * 64 + ((gid * 8) ^ (((row >> 1) & 1) << 5)));
+        v[i] = lds64(v_s + row * 64 + ((gid * 8) ^ (((row >> 1) & 1) << 5)));
       }
-      const uint2 c = *reinterpret_cast<const uint2*>(v_s + kScales + gid * 8);
-      const uint2 d = *reinterpret_cast<const uint2*>(v_s + kScales + gid * 8 + 64);
+      const uint2 c = lds64(v_s + kScales + gid * 8);
+      const uint2 d = lds64(v_s + kScales + gid * 8 + 64);
       q0[0] = c.x; q0[1] = c.y;
       q1[0] = d.x; q1[1] = d.y;
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i].x = *reinterpret_cast<const uint32_t*>(v_s + (tig + 4 * i) * 32 + gid * 4);
-      q0[0] = *reinterpret_cast<const uint32_t*>(v_s + kScales + gid * 4);
-      q1[0] = *reinterpret_cast<const uint32_t*>(v_s + kScales + gid * 4 + 32);
+      for (int i = 0; i < 4; ++i) v[i].x = lds32(v_s + (tig + 4 * i) * 32 + gid * 4);
+      q0[0] = lds32(v_s + kScales + gid * 4);
+      q1[0] = lds32(v_s + kScales + gid * 4 + 32);
     }
     if (!whole) {
 #pragma unroll
@@ -232,7 +248,7 @@ struct Warp4 {
 
   // kPart units (a part of a stage: keys, then values) from position key0 on; keys in [k_lo, k_end) are seen but for units whose bit
   // of `gone` is set.  back: scale * log2 e * 2^85
-  __device__ __forceinline__ void part(const uint8_t* at, int key0, int k_lo, int k_end, unsigned gone, float back, int lane) {
+  __device__ __forceinline__ void part(uint32_t at, int key0, int k_lo, int k_end, unsigned gone, float back, int lane) {
     const int gid = lane >> 2, tig = lane & 3;
     float p[kPart][NT][4];
 #pragma unroll
@@ -440,7 +456,7 @@ attention4_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int row_stride, 
   unsigned phase = 0;
   for (int i = 0; i < mine; ++i) {
     if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, phase, giveup))) break;
-    state.part(smem + (warp * kStages + stage) * kPartBytes, (u0 + kPart * (warp + kDecodeWarps * i)) * kUnit, k_lo, ctx,
+    state.part(ring + stage * kPartBytes, (u0 + kPart * (warp + kDecodeWarps * i)) * kUnit, k_lo, ctx,
                gone >> (kPart * stage) & ((1u << kPart) - 1), back, lane);
     __syncwarp();                                          // everyone has read the stage that the next request refills
     request(i + kStages);
