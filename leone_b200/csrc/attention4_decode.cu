@@ -11,7 +11,7 @@
 // the smallest exponent have one step), so of a word a code in bits 0-3 is c 2^-133, one in bits 4-7 is 16 c 2^-133.  Queries
 // and weights are multiplied by 2^48 before (the queries that meet bits 4-7 by 2^44), so that the sums lie in the middle of fp32's range,
 // and the sums by 2^85 after; both are exact while queries stay below 2^79 and scales below 2^40.  (128 + c by AND-OR, which needs
-// a shift for every code but a word's first and the 128 taken out again, took 425 instructions for 16 keys of 128 where this takes 311.)
+// a shift for every code but a word's first and the 128 taken out again, took 425 instructions for 16 keys of 128 where this takes 296.)
 //
 // Keys ride the MMA's M side and up to 8 query heads its N side (NT tiles of them), as in attention_tiled.cu.  The pages' layout is
 // made so that a thread's operands are words that lie side by side: 16 keys are one piece of 1,152 bytes (576 with 64 elements) for
@@ -33,8 +33,8 @@ using tc::smem_u32;
 
 constexpr int kDecodeWarps = 4;
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
-constexpr int kPart = 2;                    // units that a warp takes at once: their chains of instructions overlap
-constexpr int kStages = 3;                  // parts in flight
+constexpr int kPart = 3;                    // units that a warp takes at once: their chains of instructions overlap
+constexpr int kStages = 2;                  // parts in flight (parts of 2 with 3 in flight: 166 sequences of 2,048 keys 88.2 us, 86.7 so)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleAt = 8.f;          // the running maximum moves when a score exceeds it by this (log2): weights stay below 2^8
 
@@ -88,7 +88,8 @@ struct Warp4 {
   static constexpr int kScales = kUnit * (D / 2);
   uint32_t qb[G][NT][8];             // [pair of a word's 4][..]: queries of head gid, elements 64 g + 16 tig ..
   float qsum[G][NT][2];              // sums of the queries' group, times scale * log2 e
-  float m_run[NT][2], m_use[NT][2], l_run[NT][2], corr[G][NT][2];    // m_use: the maximum, 0 before the first key; corr: sum p (z + 8 s)
+  float m_run[NT][2], limit[NT][2], l_run[NT][2], corr[G][NT][2];   // limit: scores past the maximum that move it; corr: sum p (z + 8 s)
+  float base[NT][2];                 // minus the maximum, 0 before the first key: scores are taken relative to it
   float psum[G][NT][4];              // -8 sum P, as o (every row the same)
   float o[G][4][NT][4];              // O^T: rows = elements 64 g + 8 gid + 2 j (gid + 8: + 1)
 
@@ -124,12 +125,12 @@ struct Warp4 {
           for (int j = 0; j < 4; ++j) o[g][j][nt][i] = 0.f;
         }
       }
-      m_run[nt][0] = m_run[nt][1] = -INFINITY;
-      m_use[nt][0] = m_use[nt][1] = l_run[nt][0] = l_run[nt][1] = 0.f;
+      m_run[nt][0] = m_run[nt][1] = limit[nt][0] = limit[nt][1] = -INFINITY;
+      base[nt][0] = base[nt][1] = l_run[nt][0] = l_run[nt][1] = 0.f;
     }
   }
 
-  // The keys' words of a unit are multiplied with the queries: st += (its scores of keys gid and gid + 8) * scale * log2 e.
+  // The keys' words of a unit are multiplied with the queries: st = base + (its scores of keys gid and gid + 8) * scale * log2 e.
   __device__ __forceinline__ void scores(uint32_t k_s, float (&st)[NT][4], float back, int gid, int tig) {
     uint32_t w0[2 * G], w1[2 * G], p0[G], p1[G];
     const uint32_t at = k_s + gid * (D / 2) + tig * (8 * G);
@@ -169,24 +170,17 @@ struct Warp4 {
       const float f0 = scale_of(p0[g]) * back, f1 = scale_of(p1[g]) * back;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if (g == 0) {
-          st[nt][0] = fmaf(f0, acc[nt][0], z0 * qsum[g][nt][0]);
-          st[nt][1] = fmaf(f0, acc[nt][1], z0 * qsum[g][nt][1]);
-          st[nt][2] = fmaf(f1, acc[nt][2], z1 * qsum[g][nt][0]);
-          st[nt][3] = fmaf(f1, acc[nt][3], z1 * qsum[g][nt][1]);
-        } else {
-          st[nt][0] = fmaf(f0, acc[nt][0], fmaf(z0, qsum[g][nt][0], st[nt][0]));
-          st[nt][1] = fmaf(f0, acc[nt][1], fmaf(z0, qsum[g][nt][1], st[nt][1]));
-          st[nt][2] = fmaf(f1, acc[nt][2], fmaf(z1, qsum[g][nt][0], st[nt][2]));
-          st[nt][3] = fmaf(f1, acc[nt][3], fmaf(z1, qsum[g][nt][1], st[nt][3]));
-        }
+        st[nt][0] = fmaf(f0, acc[nt][0], fmaf(z0, qsum[g][nt][0], g == 0 ? base[nt][0] : st[nt][0]));
+        st[nt][1] = fmaf(f0, acc[nt][1], fmaf(z0, qsum[g][nt][1], g == 0 ? base[nt][1] : st[nt][1]));
+        st[nt][2] = fmaf(f1, acc[nt][2], fmaf(z1, qsum[g][nt][0], g == 0 ? base[nt][0] : st[nt][2]));
+        st[nt][3] = fmaf(f1, acc[nt][3], fmaf(z1, qsum[g][nt][1], g == 0 ? base[nt][1] : st[nt][3]));
       }
     }
   }
 
   // A unit's values times the weights p of keys gid and gid + 8 join the outputs; keep0, keep1: whether those keys are seen.
-  __device__ __forceinline__ void outputs(uint32_t v_s, const float (&p)[NT][4], bool whole, bool keep0, bool keep1, int gid,
-                                          int tig) {
+  template <bool kWhole>
+  __device__ __forceinline__ void outputs(uint32_t v_s, const float (&p)[NT][4], bool keep0, bool keep1, int gid, int tig) {
     uint2 v[4];
     uint32_t q0[G], q1[G];
     if constexpr (G == 2) {
@@ -205,7 +199,7 @@ struct Warp4 {
       q0[0] = lds32(v_s + kScales + gid * 4);
       q1[0] = lds32(v_s + kScales + gid * 4 + 32);
     }
-    if (!whole) {
+    if constexpr (!kWhole) {
 #pragma unroll
       for (int g = 0; g < G; ++g) {                          // what stands in a row that is not seen may be anything, NaN too
         if (!keep0) q0[g] = 0;
@@ -248,16 +242,16 @@ struct Warp4 {
 
   // kPart units (a part of a stage: keys, then values) from position key0 on; keys in [k_lo, k_end) are seen but for units whose bit
   // of `gone` is set.  back: scale * log2 e * 2^85
+  template <bool kWhole>
   __device__ __forceinline__ void part(uint32_t at, int key0, int k_lo, int k_end, unsigned gone, float back, int lane) {
     const int gid = lane >> 2, tig = lane & 3;
     float p[kPart][NT][4];
 #pragma unroll
     for (int u = 0; u < kPart; ++u) scores(at + 2 * u * kUnitBytes, p[u], back, gid, tig);
-    const bool whole = key0 >= k_lo && key0 + kPart * kUnit <= k_end && gone == 0;       // the same for the whole warp
     bool keep[kPart][2];
 #pragma unroll
     for (int u = 0; u < kPart; ++u) keep[u][0] = keep[u][1] = true;
-    if (!whole) {
+    if constexpr (!kWhole) {
 #pragma unroll
       for (int u = 0; u < kPart; ++u)
 #pragma unroll
@@ -278,7 +272,7 @@ struct Warp4 {
         top[nt][h] = fmaxf(p[0][nt][h], p[0][nt][2 + h]);
 #pragma unroll
         for (int u = 1; u < kPart; ++u) top[nt][h] = fmaxf(top[nt][h], fmaxf(p[u][nt][h], p[u][nt][2 + h]));
-        moves |= top[nt][h] > m_run[nt][h] + kRescaleAt;
+        moves |= top[nt][h] > limit[nt][h];
       }
     if (__any_sync(0xffffffffu, moves)) {
 #pragma unroll
@@ -289,7 +283,7 @@ struct Warp4 {
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
-          const float m_new = fmaxf(m_run[nt][h], t);
+          const float m_new = fmaxf(m_run[nt][h], t - base[nt][h]);
           if (m_run[nt][h] != -INFINITY && m_new > m_run[nt][h]) {        // (nothing is summed before the first key)
             const float alpha = ex2(m_run[nt][h] - m_new);
             l_run[nt][h] *= alpha;
@@ -305,7 +299,14 @@ struct Warp4 {
             }
           }
           m_run[nt][h] = m_new;
-          m_use[nt][h] = m_new == -INFINITY ? 0.f : m_new;
+          const float to = m_new == -INFINITY ? 0.f : -m_new;
+#pragma unroll
+          for (int u = 0; u < kPart; ++u) {
+            p[u][nt][h] += to - base[nt][h];
+            p[u][nt][2 + h] += to - base[nt][h];
+          }
+          base[nt][h] = to;
+          limit[nt][h] = m_new == -INFINITY ? -INFINITY : kRescaleAt;
         }
     }
 #pragma unroll
@@ -313,12 +314,12 @@ struct Warp4 {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[u][nt][i] = ex2(p[u][nt][i] - m_use[nt][i & 1]);
+        for (int i = 0; i < 4; ++i) p[u][nt][i] = ex2(p[u][nt][i]);
         l_run[nt][0] += p[u][nt][0] + p[u][nt][2];
         l_run[nt][1] += p[u][nt][1] + p[u][nt][3];
       }
 #pragma unroll
-    for (int u = 0; u < kPart; ++u) outputs(at + (2 * u + 1) * kUnitBytes, p[u], whole, keep[u][0], keep[u][1], gid, tig);
+    for (int u = 0; u < kPart; ++u) outputs<kWhole>(at + (2 * u + 1) * kUnitBytes, p[u], keep[u][0], keep[u][1], gid, tig);
   }
 
   // This warp's (max, sum, unnormalised output) per head into mo [warps][8 NT][D] and ml [warps][8 NT][2].
@@ -456,8 +457,11 @@ attention4_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int row_stride, 
   unsigned phase = 0;
   for (int i = 0; i < mine; ++i) {
     if (!__all_sync(0xffffffffu, mbar_wait(bars + 8 * stage, phase, giveup))) break;
-    state.part(ring + stage * kPartBytes, (u0 + kPart * (warp + kDecodeWarps * i)) * kUnit, k_lo, ctx,
-               gone >> (kPart * stage) & ((1u << kPart) - 1), back, lane);
+    const uint32_t at = ring + stage * kPartBytes;
+    const int key0 = (u0 + kPart * (warp + kDecodeWarps * i)) * kUnit;
+    const unsigned lost = gone >> (kPart * stage) & ((1u << kPart) - 1);
+    if (key0 >= k_lo && key0 + kPart * kUnit <= ctx && lost == 0) state.template part<true>(at, key0, k_lo, ctx, lost, back, lane);
+    else state.template part<false>(at, key0, k_lo, ctx, lost, back, lane);
     __syncwarp();                                          // everyone has read the stage that the next request refills
     request(i + kStages);
     if (++stage == kStages) {
@@ -542,13 +546,17 @@ attention4_decode_kernel(const __nv_bfloat16* __restrict__ qkv, int row_stride, 
   }
 }
 
-// The parts of more splits than a cluster holds, and those of prompt portions.  grid = (sequences or tokens, heads), a thread for two
-// columns; rows: where a sequence's row of the output is, or null for token i in row i.
+constexpr int kMergeWays = 4;
+constexpr int merge_ways(int splits) { return splits > 8 ? kMergeWays : 1; }
+// The parts of more splits than a cluster holds, and those of prompt portions.  grid = (sequences or tokens, heads), merge_ways(splits)
+// threads for two columns (one sequence of 40,960 keys in 37 splits: 21.7 us with four, 25.2 with one, which fetches 8 parts at a time);
+// rows: where a sequence's row of the output is, or null for token i in row i.
 __global__ void attention4_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
                                         __nv_bfloat16* __restrict__ out, int out_stride, const int* __restrict__ rows, int n_q, int d,
                                         int splits) {
   __shared__ float f_s[64];
   __shared__ float l_s;
+  __shared__ float2 o_s[kMergeWays][64];
   pdl_trigger();
   pdl_wait();
   const int head = blockIdx.y, seq = blockIdx.x, tid = threadIdx.x;
@@ -575,14 +583,25 @@ __global__ void attention4_merge_kernel(const float* __restrict__ part_o, const 
     if (tid == 0) l_s = sum;
   }
   __syncthreads();
-  const int c = tid * 2;
+  // `ways` threads share two columns: 64 splits are 16 loads a thread, all in flight at once
+  const int ways = blockDim.x / (d / 2), way = tid / (d / 2), c = (tid - way * (d / 2)) * 2;
   float o0 = 0.f, o1 = 0.f;
-#pragma unroll 8
-  for (int s = 0; s < splits; ++s) {
-    if (f_s[s] == 0.f) continue;
-    const float2 v = *reinterpret_cast<const float2*>(part_o + (base + s) * d + c);
-    o0 = fmaf(f_s[s], v.x, o0);
-    o1 = fmaf(f_s[s], v.y, o1);
+#pragma unroll 16
+  for (int s = way; s < splits; s += ways) {
+    const float f = f_s[s];
+    float2 v = make_float2(0.f, 0.f);
+    if (f != 0.f) v = *reinterpret_cast<const float2*>(part_o + (base + s) * d + c);
+    o0 = fmaf(f, v.x, o0);
+    o1 = fmaf(f, v.y, o1);
+  }
+  if (ways > 1) {
+    o_s[way][c / 2] = make_float2(o0, o1);
+    __syncthreads();
+    if (way != 0) return;
+    for (int w = 1; w < ways; ++w) {
+      o0 += o_s[w][c / 2].x;
+      o1 += o_s[w][c / 2].y;
+    }
   }
   const float inv = l_s == 0.f ? 0.f : 1.f / l_s;
   *reinterpret_cast<__nv_bfloat162*>(out + (size_t)(rows == nullptr ? seq : rows[seq]) * out_stride + (size_t)head * d + c) =
@@ -615,7 +634,7 @@ int launch_decode(const __nv_bfloat16* qkv, int row_stride, __nv_bfloat16* out, 
                               row_stride, out, out_stride, pa, q_start, ctx_len, n_q, scale, window, splits, 0, order, scratch,
                               part_ml, status);
   if (e != 0 || splits == 1) return e;
-  return launch_kernel(attention4_merge_kernel, dim3(n_seqs, n_q), dim3(D / 2), 0, stream, (const float*)scratch,
+  return launch_kernel(attention4_merge_kernel, dim3(n_seqs, n_q), dim3(D / 2 * merge_ways(splits)), 0, stream, (const float*)scratch,
                        (const float*)part_ml, out, out_stride, q_start, n_q, D, splits);
 }
 
@@ -663,6 +682,6 @@ extern "C" int leone_attention4_merge(const float* part_o, const float* part_ml,
   if (n_tokens <= 0) return 0;
   if ((d != 64 && d != 128) || n_q <= 0 || n_q > 65535 || splits < 1 || splits > 64) return kRefusedSize;
   if (out_stride % 2 != 0 || ((uintptr_t)out & 3) || ((uintptr_t)part_o | (uintptr_t)part_ml) & 15) return kRefusedAlignment;
-  return launch_kernel(cache4::attention4_merge_kernel, dim3(n_tokens, n_q), dim3(d / 2), 0, stream, part_o, part_ml,
+  return launch_kernel(cache4::attention4_merge_kernel, dim3(n_tokens, n_q), dim3(d / 2 * cache4::merge_ways(splits)), 0, stream, part_o, part_ml,
                        (__nv_bfloat16*)out, out_stride, (const int*)nullptr, n_q, d, splits);
 }

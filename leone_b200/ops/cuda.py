@@ -682,15 +682,18 @@ class CudaOps:
     force_decode4_splits = 0               # > 0: every decode attention over pages in 4 bits splits its keys this many ways
 
     @staticmethod
-    def choose_decode4_splits(n_seqs: int, n_kv: int, g: int, keys: int):
-        """``(splits, in a cluster)`` of a decode attention over pages in 4 bits: ``keys`` are the most that a sequence reads.  Two blocks an
-        SM, though an SM holds three: what a block costs before its first and after its last key is more than the third gives (one sequence,
-        8 cached heads of 128: 8,192 keys 16.5 us with 8 to 32 splits, 18.5 with 48; 40,960 keys 26.8 with 32, 28.7 with 48; 8
-        sequences of 2,048 16.5 with 4, 18.6 with 6; 24 of 3,000 with 2 heads of 64 14.4 with 8, 16.5 with 12).  A split keeps 128 keys.  Up
-        to 8 merge in a cluster; a few more than that are not worth scratch and a second kernel."""
-        s = max(1, min(64, 2 * 148 // (n_seqs * n_kv * -(-g // 16)), keys // 128))
-        if 8 < s < 12:
+    def choose_decode4_splits(n_seqs: int, n_kv: int, g: int, keys: int, d: int):
+        """``(splits, in a cluster)`` of a decode attention over pages in 4 bits: ``keys`` are the most that a sequence reads.  As many as
+        make the three blocks that an SM holds (16 sequences of 2,048 keys, 8 cached heads of 128: 14.4 us with 3, 17.5 with 2; one of
+        40,960: 19.4 with 55, 21.7 with 37, 25.2 with 64, which no longer fit at once), and two where one would leave an SM with one
+        block and its neighbour with two (32 sequences of up to 2,048: 19.7 against 24.2; 37 of one length 31.2 against 29.3).  A split
+        keeps 128 keys.  Up to 8 merge in a cluster; more, which take scratch and a second kernel, have to save 1,024 keys of 128 a
+        block (one sequence of 4,000 8.2 with 8, 9.9 with 31; of 8,192 11.9 with 8, 11.6 with 55; four 17.6 with 8, 16.4 with 13)."""
+        blocks = n_seqs * n_kv * -(-g // 16)
+        s = max(3 * 148 // blocks, 2 if blocks <= 256 else 1)
+        if s > 8 and (s < 12 or keys * d < 1 << 20):
             s = 8
+        s = max(1, min(64, s, keys // 128))
         return s, 1 < s <= 8
 
     def _attention4_decode(self, q, row_stride, o, out_stride, n_q, n_kv, d, scale, window, pool, ctx, n_seqs, max_ctx) -> None:
@@ -699,7 +702,7 @@ class CudaOps:
         calls, order = self.packed_calls, getattr(ctx, "seq_order", None)          # these sequences, the longest first
         if order is not None and order.numel() != n_seqs:
             raise KernelError(f"an order of {order.numel()} sequences for {n_seqs}")
-        splits, in_cluster = self.choose_decode4_splits(n_seqs, n_kv, n_q // n_kv, min(max_ctx, window) if window else max_ctx)
+        splits, in_cluster = self.choose_decode4_splits(n_seqs, n_kv, n_q // n_kv, min(max_ctx, window) if window else max_ctx, d)
         if self.force_decode4_splits:
             splits = self.force_decode4_splits
             in_cluster = 1 < splits <= 8
