@@ -133,36 +133,136 @@ __global__ void append_kernel(T* __restrict__ qkv, int n_tokens, int n_q, int n_
   }
 }
 
+// One row into its page by one warp, everything in 64 bits: rows for which append_vec_kernel's 32 bits leave a code in doubt.  `row` in
+// shared memory; w: the norm's weights or null; rope: the position's pairs or null.
+template <typename T, typename TW, int D>
+__device__ __noinline__ void append_exact(const T* row, const TW* w, float eps, const float2* rope, bool adjacent, bool is_k, int slot,
+                                          uint8_t* unit) {
+  constexpr int E = D / 32, G = D / 64, kGroupLanes = 32 / G, kWordLanes = 8 / E;
+  const int lane = threadIdx.x & 31;
+  double d[E], most = -INFINITY, least = INFINITY;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < E; ++i) d[i] = (double)to_float<T>(row[lane * E + i]);
+  if (w != nullptr) {
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) ss = fma(d[i], d[i], ss);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    const double factor = rsqrt(ss / D + (double)eps);
+#pragma unroll
+    for (int i = 0; i < E; ++i) d[i] *= (double)to_float<TW>(w[lane * E + i]) * factor;
+  }
+  if (rope != nullptr) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if (adjacent) {
+        if (i & 1) continue;
+        const float2 cs = rope[(lane * E + i) >> 1];
+        const double a = d[i], b = d[i + 1];
+        d[i] = a * cs.x - b * cs.y;
+        d[i + 1] = a * cs.y + b * cs.x;
+      } else {
+        const float2 cs = rope[(lane & 15) * E + i];
+        const double other = __shfl_xor_sync(0xffffffffu, d[i], 16);
+        d[i] = lane >= 16 ? other * cs.y + d[i] * cs.x : d[i] * cs.x - other * cs.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    odd |= !isfinite(d[i]);
+    least = fmin(least, d[i]);
+    most = fmax(most, d[i]);
+  }
+#pragma unroll
+  for (int o = kGroupLanes / 2; o > 0; o >>= 1) {
+    least = fmin(least, __shfl_xor_sync(0xffffffffu, least, o));
+    most = fmax(most, __shfl_xor_sync(0xffffffffu, most, o));
+    odd |= __shfl_xor_sync(0xffffffffu, (int)odd, o) != 0;
+  }
+  __nv_bfloat16 z16 = bf16_down(least);
+  const double z = __bfloat162float(z16);
+  __nv_bfloat16 s16 = bf16_up((most - z) / 15.0);
+  if (__bfloat162float(s16) < 1.17549435e-38f) s16 = __float2bfloat16_rn(0.f);
+  odd |= !isfinite(z) || !isfinite(__bfloat162float(s16));
+  if (odd) z16 = s16 = __ushort_as_bfloat16(0x7fc0);
+  const double s = __bfloat162float(s16);
+  // the word's lanes put their nibbles together (element 2 j in nibble j, 2 j + 1 in nibble j + 4), the first of them stores it
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const uint32_t code = !odd && s > 0.0 ? (uint32_t)fmin(fmax(rint((d[i] - z) / s), 0.0), 15.0) : 0u;
+    word |= code << (4 * (i >> 1) + 16 * (i & 1));
+  }
+  word <<= 4 * (E / 2) * (lane % kWordLanes);
+#pragma unroll
+  for (int o = 1; o < kWordLanes; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
+  const int w_at = lane / kWordLanes;
+  if (lane % kWordLanes == 0)
+    *reinterpret_cast<uint32_t*>(unit + (is_k ? key_word_at(slot, w_at, D) : value_word_at(slot, w_at, D))) = word;
+  if (lane % kGroupLanes == 0)
+    *reinterpret_cast<uint32_t*>(unit + scale_at(slot, lane / kGroupLanes, D)) =
+        (uint32_t)__bfloat16_as_ushort(s16) | (uint32_t)__bfloat16_as_ushort(z16) << 16;
+}
+
 // The same for heads of 64 and 128 elements that rotate whole or not at all.  grid = (tokens, blocks of `per` heads); a block brings its
-// rows into shared memory at once, then its eight warps take a head each in turn, with the token's place, rotation and norm
-// weights at hand; lane l has elements E l .. E l + E - 1.  (Rows read one ahead of their use, four heads a warp: 49 us for 2,048 tokens of 48
-// heads, most of it waiting for them.)
+// rows into shared memory at once, then its warps take two heads each in turn, with the token's place, rotation and norm weights
+// at hand: half a warp for a head, lane r with elements H r .. H r + H - 1 of the head's first half and of its second.  So a pair
+// of the rotation lies in one lane whichever way elements pair, and a group of 64 is one half of 128 or all of 64.
 //
-// Codes are still those of 64 bits, but computed in 32 where that is certain.  A key is off by at most kKeyError (|a| + |b|) (|cos| +
-// |sin|) of its pair's elements before the rotation: of 2^-24, half of the sum's nine roundings, four for the reciprocal root
-// and its argument, two products, a product and a sum.  So the group's minimum and maximum are known to within the largest such error,
-// and where both ends of that range give the same z and the same s, those are right.  A quotient (x - z) / s is off by its key's error
-// over s and three roundings; where it comes no nearer than that to a border of two codes, so is its code.  Where anything is in doubt,
-// or not finite, the warp computes the row again in 64 bits (one row of keys in two hundred).
-// 2,048 tokens of 48 heads 29 us (floor 5); the form above takes 90.
-constexpr float kKeyError = 16.f / 16777216.f;
-constexpr int kAppendWarps = 8;
+// Codes are those of 64 bits.  Keys are normed and rotated in 64 bits and then rounded to 32 (kRounded of the value off), values
+// are what they are; minima, maxima and quotients are of 32.  Where the ends of the range in which the minimum and the maximum lie give
+// one z and one s, those are right.  A quotient that comes no nearer to a border of two codes than the roundings take it is rounded right;
+// one that does is settled by the sign of x - z - (code + 1/2) s in 64 bits.  (Values in bfloat16 lie on a border more often than
+// not in a row.)  Where z or s is in doubt, or something not finite, the warp computes the row again, which a step hardly ever does: that
+// code is never in the instruction cache, and a block waits 4 us for it.  (With norm and rotation in 32 bits a row of keys in a hundred
+// was in doubt: 2,048 tokens of 48 heads of 128 took 28.2 us, of 22 of 64 10.6, where this takes 21.5 and 8.7.
+// Their queries alone take 8.6, the floor is 5.)
+constexpr float kRounded = 1.01f / 16777216.f;
+constexpr float kToInteger = 12582912.f;           // 1.5 2^23: adding it rounds to an integer, which the low bits then hold
+constexpr int kAppendWarps = 4;
 constexpr int kAppendHeads = 48;                   // of a block, at most
 
-template <typename T, typename TW, int E>
-__global__ void __launch_bounds__(32 * kAppendWarps, 4)
+// Over the 16 lanes of half a warp.
+__device__ __forceinline__ float half_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float half_min(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float half_max(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+template <typename F> __device__ __forceinline__ void turn_pair(F& x, F& y, float2 c) {
+  const F u = x * (F)c.x - y * (F)c.y;
+  y = x * (F)c.y + y * (F)c.x;
+  x = u;
+}
+
+template <typename T, typename TW, int D>
+__global__ void __launch_bounds__(32 * kAppendWarps, 5)
 append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__ q_w, const TW* __restrict__ k_w, float eps,
                   const float2* __restrict__ rope, int max_positions, const int* __restrict__ positions,
                   const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int table_width, int n_seqs,
                   uint8_t* __restrict__ k_pool, uint8_t* __restrict__ v_pool, int num_pages, int page_tokens, int adjacent, int per,
                   int* status) {
-  constexpr int D = 32 * E, G = D / 64, kGroupLanes = 32 / G, kWordLanes = 8 / E;
+  constexpr int H = D / 32, G = D / 64, kWordLanes = 8 / H;
+  constexpr unsigned kAll = 0xffffffffu;
   pdl_trigger();
   pdl_wait();
-  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x, warp = threadIdx.x >> 5, sub = threadIdx.x >> 4 & 1, r = threadIdx.x & 15;
   const int heads = n_q + 2 * n_kv;
   const int h0 = blockIdx.y * per, h1 = min(heads, h0 + per);
-  struct __align__(sizeof(T) * E) Row { T e[E]; };         // a lane's elements of a head
+  struct __align__(sizeof(T) * H) Part { T e[H]; };        // a lane's elements of half a head
   extern __shared__ __align__(16) uint8_t rows_s[];
   T* tok = qkv + (size_t)t * heads * D;
   for (int i = threadIdx.x; i < (h1 - h0) * D * (int)sizeof(T) / 16; i += 32 * kAppendWarps) {
@@ -172,196 +272,240 @@ append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
   const int pos = positions[t];
-  const bool rotate = rope != nullptr;
-  const bool in_table = !rotate || (pos >= 0 && pos < max_positions);
-  if (!in_table && lane == 0) set_status(status, kBadPosition, t, pos);
-  // the lane's pairs: elements (i, i + D / 2) share cs[i] between lanes l and l ^ 16, elements (2 i, 2 i + 1) cs[2 i] in the lane
-  float2 cs[E];
+  const bool in_table = rope == nullptr || (pos >= 0 && pos < max_positions), rotate = rope != nullptr && in_table;
+  if (!in_table && threadIdx.x == 0) set_status(status, kBadPosition, t, pos);
+  const float2* turn = rotate ? rope + (size_t)pos * (D / 2) : nullptr;
+  // the lane's pairs: element i of the first half with i of the second, or elements 2 i, 2 i + 1 of the first, then of the second
+  float2 cs[H];
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const int pair = adjacent ? (lane * E + i) >> 1 : (lane & 15) * E + i;
-    cs[i] = rotate && in_table ? rope[(size_t)pos * (D / 2) + pair] : make_float2(1.f, 0.f);
+  for (int i = 0; i < H; ++i) {
+    const int pair = !adjacent ? H * r + i : H / 2 * r + i % (H / 2) + i / (H / 2) * (D / 4);
+    cs[i] = rotate ? turn[pair] : make_float2(1.f, 0.f);
   }
-  float w[E];
+  float wa[H], wb[H];
   auto weights = [&](const TW* from) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) w[i] = from != nullptr ? to_float<TW>(from[lane * E + i]) : 1.f;
+    for (int i = 0; i < H; ++i) {
+      wa[i] = to_float<TW>(from[H * r + i]);
+      wb[i] = to_float<TW>(from[D / 2 + H * r + i]);
+    }
   };
-  auto normed = [&](const float (&x)[E], float (&y)[E]) {
-    float ss = 0.f;
+  const Part* rows = reinterpret_cast<const Part*>(rows_s) + r;                 // 32 for every head
+  auto fetch = [&](int at, float (&a)[H], float (&b)[H]) {
+    const Part x = rows[at * 32], y = rows[at * 32 + 16];
 #pragma unroll
-    for (int i = 0; i < E; ++i) ss = fmaf(x[i], x[i], ss);
-    ss = warp_sum(ss);
-    const float f = rsqrtf(ss * (1.f / D) + eps);
-#pragma unroll
-    for (int i = 0; i < E; ++i) y[i] = x[i] * w[i] * f;
+    for (int i = 0; i < H; ++i) {
+      a[i] = to_float<T>(x.e[i]);
+      b[i] = to_float<T>(y.e[i]);
+    }
   };
-  // off[i]: how far element i may be off
-  auto turned = [&](float (&y)[E], float (&off)[E]) {
+  auto norm = [&](float (&a)[H], float (&b)[H]) {
+    float sa = a[0] * a[0], sb = b[0] * b[0];
+#pragma unroll
+    for (int i = 1; i < H; ++i) {
+      sa = fmaf(a[i], a[i], sa);
+      sb = fmaf(b[i], b[i], sb);
+    }
+    const float f = rsqrtf(half_sum(sa + sb) * (1.f / D) + eps);
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      a[i] = a[i] * wa[i] * f;
+      b[i] = b[i] * wb[i] * f;
+    }
+  };
+  auto rotated = [&](auto& a, auto& b) {                   // a pair and its turn: (x, y) (cos, sin)
     if (adjacent) {
 #pragma unroll
-      for (int i = 0; i < E; i += 2) {
-        const float a = y[i], b = y[i + 1];
-        off[i] = off[i + 1] = (fabsf(a) + fabsf(b)) * ((fabsf(cs[i].x) + fabsf(cs[i].y)) * kKeyError);
-        y[i] = a * cs[i].x - b * cs[i].y;
-        y[i + 1] = a * cs[i].y + b * cs[i].x;
+      for (int i = 0; i < H / 2; ++i) {
+        turn_pair(a[2 * i], a[2 * i + 1], cs[i]);
+        turn_pair(b[2 * i], b[2 * i + 1], cs[H / 2 + i]);
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const float other = __shfl_xor_sync(0xffffffffu, y[i], 16);
-        off[i] = (fabsf(y[i]) + fabsf(other)) * ((fabsf(cs[i].x) + fabsf(cs[i].y)) * kKeyError);
-        y[i] = lane >= 16 ? other * cs[i].y + y[i] * cs[i].x : y[i] * cs[i].x - other * cs[i].y;
-      }
+      for (int i = 0; i < H; ++i) turn_pair(a[i], b[i], cs[i]);
     }
   };
-  int h = h0 + warp;
-  if (h < n_q && q_w != nullptr) weights(q_w);
+  const int n_queries = max(0, min(h1, n_q) - h0), n_keys = max(0, min(h1, n_q + n_kv) - max(h0, n_q));
+  const int n_values = h1 - h0 - n_queries - n_keys;
+  int p = warp;                                            // two heads of one kind; the kinds' follow one another
+  if (p < (n_queries + 1) / 2 && q_w != nullptr) weights(q_w);
   Place place;
   const bool placed = h1 <= n_q || find_place(place, t, pos, seq_of_token, n_seqs, block_table, table_width, num_pages, page_tokens,
                                               status, threadIdx.x == 0);
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  const Row* mine = reinterpret_cast<const Row*>(rows_s) + lane - h0 * 32;       // + 32 for every head
-  if (h < n_q) {
-    for (const int end = min(h1, n_q); h < end; h += kAppendWarps) {
-      float x[E], y[E], off[E];
-      const Row row = mine[h * 32];
+  for (; p < (n_queries + 1) / 2; p += kAppendWarps) {
+    const bool real = 2 * p + sub < n_queries;
+    const int at = real ? 2 * p + sub : 2 * p;
+    float a[H], b[H];
+    fetch(at, a, b);
+    if (q_w != nullptr) norm(a, b);
+    if (rotate) rotated(a, b);
+    Part x, y;
 #pragma unroll
-      for (int i = 0; i < E; ++i) y[i] = x[i] = to_float<T>(row.e[i]);
-      if (q_w != nullptr) normed(x, y);
-      if (rotate) turned(y, off);
-      Row out;
-#pragma unroll
-      for (int i = 0; i < E; ++i) out.e[i] = from_float<T>(y[i]);
-      if (in_table) reinterpret_cast<Row*>(tok + (size_t)h * D)[lane] = out;
+    for (int i = 0; i < H; ++i) {
+      x.e[i] = from_float<T>(a[i]);
+      y.e[i] = from_float<T>(b[i]);
+    }
+    if (real && in_table) {
+      Part* to = reinterpret_cast<Part*>(tok + (size_t)(h0 + at) * D) + r;
+      to[0] = x;
+      to[16] = y;
     }
   }
-  if (h >= h1 || !placed) return;
-  if (k_w != nullptr) weights(k_w);
+  p -= (n_queries + 1) / 2;
+  if (!placed) return;
   const long long unit = unit_at(place.page, n_kv, 0, page_tokens, place.slot / kUnit * kUnit, D);
   const int slot = place.slot % kUnit, head_bytes = page_tokens * row_bytes(D);
-  const int key_at = key_word_at(slot, lane / kWordLanes, D), value_at = value_word_at(slot, lane / kWordLanes, D);
-  for (; h < h1; h += kAppendWarps) {
-    float x[E], y[E], off[E];
-    const Row row = mine[h * 32];
+  // of the lanes that share a word of the first half and one of the second, the first stores the one and the last the other
+  const int w_at = r / kWordLanes + (r % kWordLanes == kWordLanes - 1 ? D / 16 : 0);
+  const bool stores = r % kWordLanes == 0 || r % kWordLanes == kWordLanes - 1;
+  auto store = [&](bool is_k, int first, int count) {      // heads first .. first + count - 1 of the block's
+    const bool computed = is_k && (k_w != nullptr || rotate);
+    const int word_at = is_k ? key_word_at(slot, w_at, D) : value_word_at(slot, w_at, D);
+    for (; p < (count + 1) / 2; p += kAppendWarps) {
+      const bool real = 2 * p + sub < count;
+      const int at = first + (real ? 2 * p + sub : 2 * p);
+      float a[H], b[H];
+      double da[H], db[H];                                 // of keys
+      bool doubt = false;
+      fetch(at, a, b);
+      if (computed) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      y[i] = x[i] = to_float<T>(row.e[i]);
-      off[i] = 0.f;
-    }
-    const bool is_k = h < n_q + n_kv, norms = is_k && k_w != nullptr, turns = is_k && rotate;
-    if (turns && !in_table) continue;
-    float err = 0.f;                                       // the largest of off in the group
-    if (norms) {
-      normed(x, y);
+        for (int i = 0; i < H; ++i) {
+          da[i] = a[i];
+          db[i] = b[i];
+        }
+        if (k_w != nullptr) {
+          double ss = 0.0;
 #pragma unroll
-      for (int i = 0; i < E; ++i) off[i] = fabsf(y[i]) * kKeyError;
-    }
-    if (turns) turned(y, off);
-    float lo = y[0], hi = y[0];
-    bool doubt = false;
+          for (int i = 0; i < H; ++i) ss = fma(da[i], da[i], fma(db[i], db[i], ss));
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      doubt |= !(fabsf(y[i]) < INFINITY);
-      lo = fminf(lo, y[i]);
-      hi = fmaxf(hi, y[i]);
-    }
-    if (is_k) {
+          for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(kAll, ss, o);
+          ss = ss * (1.0 / D) + (double)eps;
+          doubt |= !(ss > 1e-37 && ss < 1e37);
+          double f = rsqrtf((float)ss);                    // two steps of Newton's take it to 64 bits
+          f *= fma(-0.5 * ss * f, f, 1.5);
+          f *= fma(-0.5 * ss * f, f, 1.5);
 #pragma unroll
-      for (int i = 0; i < E; ++i) err = fmaxf(err, off[i]);
-#pragma unroll
-      for (int o = kGroupLanes / 2; o > 0; o >>= 1) err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, o));
-    }
-#pragma unroll
-    for (int o = kGroupLanes / 2; o > 0; o >>= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    float z = __bfloat162float(__float2bfloat16_rd(lo - err));
-    doubt |= z != __bfloat162float(__float2bfloat16_rd(lo + err));
-    // (hi - z) / 15 with what its ends and its own five roundings leave open
-    float s = __bfloat162float(__float2bfloat16_ru((hi - z - err) * (1.f / 15.f) * (1.f - 6e-7f)));
-    doubt |= s != __bfloat162float(__float2bfloat16_ru((hi - z + err) * (1.f / 15.f) * (1.f + 6e-7f)));
-    doubt |= (s != 0.f && !(s > 1e-37f && s < 1e37f)) || !(fabsf(z) < 3e38f);
-    const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-    uint32_t code[E];
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float gap = y[i] - z, q = gap * inv;
-      float r = rintf(q);
-      if (fabsf(fabsf(q - r) - 0.5f) <= fmaf(off[i], inv * 1.01f, fabsf(q) * 2.5e-7f) && s > 0.f) {
-        // An element that is known exactly (a value) and an exact difference: the sign of gap - (k + 1/2) s is exact too, and a tie
-        // goes to the even code.  (Values in bfloat16 lie on a border more often than not in a row.)
-        const float low = floorf(q), back = y[i] - gap, side = fmaf(-(low + 0.5f), s, gap);
-        doubt |= off[i] != 0.f || (y[i] - (gap + back)) + (back - z) != 0.f;
-        r = side > 0.f || (side == 0.f && ((int)low & 1)) ? low + 1.f : low;
-      }
-      code[i] = (uint32_t)fminf(fmaxf(r, 0.f), 15.f);
-    }
-    uint32_t sz = __float_as_uint(s) >> 16 | (__float_as_uint(z) & 0xffff0000u);
-    if (__any_sync(0xffffffffu, doubt)) {
-      // again in 64 bits, as the form above
-      double d[E], most = -INFINITY, least = INFINITY, factor = 1.0;
-      bool odd = false;
-      if (norms) {
-        double ss = 0.0;
-#pragma unroll
-        for (int i = 0; i < E; ++i) ss = fma((double)x[i], (double)x[i], ss);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        factor = rsqrt(ss / D + (double)eps);
-      }
-#pragma unroll
-      for (int i = 0; i < E; ++i) d[i] = norms ? (double)x[i] * ((double)w[i] * factor) : (double)x[i];
-      if (turns) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-          if (adjacent) {
-            if (i & 1) continue;
-            const double a = d[i], b = d[i + 1];
-            d[i] = a * cs[i].x - b * cs[i].y;
-            d[i + 1] = a * cs[i].y + b * cs[i].x;
-          } else {
-            const double other = __shfl_xor_sync(0xffffffffu, d[i], 16);
-            d[i] = lane >= 16 ? other * cs[i].y + d[i] * cs[i].x : d[i] * cs[i].x - other * cs[i].y;
+          for (int i = 0; i < H; ++i) {
+            da[i] *= (double)wa[i] * f;
+            db[i] *= (double)wb[i] * f;
           }
         }
+        if (rotate) rotated(da, db);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          a[i] = (float)da[i];
+          b[i] = (float)db[i];
+        }
+      }
+      float lo[2], hi[2];                                  // of the halves
+      lo[0] = hi[0] = a[0];
+      lo[1] = hi[1] = b[0];
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        doubt |= !(fabsf(a[i]) < INFINITY) || !(fabsf(b[i]) < INFINITY);
+        lo[0] = fminf(lo[0], a[i]);
+        hi[0] = fmaxf(hi[0], a[i]);
+        lo[1] = fminf(lo[1], b[i]);
+        hi[1] = fmaxf(hi[1], b[i]);
+      }
+      if (G == 1) {
+        lo[0] = fminf(lo[0], lo[1]);
+        hi[0] = fmaxf(hi[0], hi[1]);
+      }
+      float z[2], s[2], inv[2], limit[2];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        lo[g] = half_min(lo[g]);
+        hi[g] = half_max(hi[g]);
+        const float err = computed ? fmaxf(fabsf(lo[g]), fabsf(hi[g])) * kRounded : 0.f;
+        z[g] = __bfloat162float(__float2bfloat16_rd(__fsub_rd(lo[g], err)));
+        doubt |= z[g] != __bfloat162float(__float2bfloat16_rd(__fadd_ru(lo[g], err)));
+        // s is the smallest with 15 s >= hi - z; 15 s has 12 bits.  Of a value the rounded difference is on the side of 15 s that the
+        // difference is on, or meets it; of a key it is off by the maximum's rounding and its own (and the margin's).
+        const float range = hi[g] - z[g], margin = err + 2.f * kRounded * range;
+        s[g] = __bfloat162float(__float2bfloat16_ru(range * (1.f / 15.f) * (1.f - 6e-7f)));    // or the next
+        if (15.f * s[g] < range) s[g] = __uint_as_float(__float_as_uint(s[g]) + 0x10000u);
+        if (err != 0.f) {
+          const float below = __uint_as_float(__float_as_uint(s[g]) - 0x10000u);
+          doubt |= !(range - margin > 15.f * below && range + margin < 15.f * s[g]);
+        } else if (range == 15.f * s[g]) {
+          const float back = hi[g] - range;
+          doubt |= (hi[g] - (range + back)) + (back - z[g]) != 0.f;
+        }
+        doubt |= (s[g] != 0.f && !(s[g] > 1e-37f && s[g] < 1e37f)) || !(fabsf(z[g]) < 3e38f);
+        inv[g] = s[g] > 0.f ? __frcp_rn(s[g]) : 0.f;
+        limit[g] = 0.5f - fmaf(err, inv[g] * 1.01f, 15.5f * 2.5e-7f);
+      }
+      if (G == 1) {
+        z[1] = z[0];
+        s[1] = s[0];
+        inv[1] = inv[0];
+        limit[1] = limit[0];
+      }
+      float code[2][H];                                    // + kToInteger
+      bool near = false;
+#pragma unroll
+      for (int i = 0; i < H; ++i)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const float gap = (g ? b[i] : a[i]) - z[g], c = fmaf(gap, inv[g], kToInteger);
+          near |= fabsf(fmaf(gap, inv[g], kToInteger - c)) >= limit[g];
+          code[g][i] = c;
+        }
+      if (near) {
+#pragma unroll
+        for (int i = 0; i < H; ++i)
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const float x = g ? b[i] : a[i], q = (x - z[g]) * inv[g], low = floorf(q);
+            if (fabsf(fabsf(q - low) - 0.5f) > 1e-3f) continue;
+            const double gap = (computed ? (g ? db[i] : da[i]) : (double)x) - (double)z[g];
+            const double side = fma(-(double)(low + 0.5f), (double)s[g], gap);
+            code[g][i] = (side > 0.0 || (side == 0.0 && ((int)low & 1)) ? low + 1.f : low) + kToInteger;
+          }
+      }
+      // the word's lanes put their nibbles together (element 2 j in nibble j, 2 j + 1 in nibble j + 4)
+      uint32_t word[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        word[g] = 0;
+#pragma unroll
+        for (int i = 0; i < H; ++i) word[g] += (__float_as_uint(code[g][i]) - __float_as_uint(kToInteger)) << (4 * (i >> 1) + 16 * (i & 1));
+        word[g] <<= 4 * (H / 2) * (r % kWordLanes);
       }
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        odd |= !isfinite(d[i]);
-        least = fmin(least, d[i]);
-        most = fmax(most, d[i]);
+      for (int o = kWordLanes / 2; o > 1; o >>= 1) {
+        word[0] |= __shfl_xor_sync(kAll, word[0], o);
+        word[1] |= __shfl_xor_sync(kAll, word[1], o);
       }
-#pragma unroll
-      for (int o = kGroupLanes / 2; o > 0; o >>= 1) {
-        least = fmin(least, __shfl_xor_sync(0xffffffffu, least, o));
-        most = fmax(most, __shfl_xor_sync(0xffffffffu, most, o));
-        odd |= __shfl_xor_sync(0xffffffffu, (int)odd, o) != 0;
+      const uint32_t other = __shfl_xor_sync(kAll, r & 1 ? word[0] : word[1], 1), whole = (r & 1 ? word[1] : word[0]) | other;
+      const unsigned again = __ballot_sync(kAll, doubt);
+      uint8_t* pool = is_k ? k_pool + (size_t)(h0 + at - n_q) * head_bytes : v_pool + (size_t)(h0 + at - n_q - n_kv) * head_bytes;
+      if (again == 0) {
+        if (real && stores) *reinterpret_cast<uint32_t*>(pool + unit + word_at) = whole;
+        if (real && r < G)
+          *reinterpret_cast<uint32_t*>(pool + unit + scale_at(slot, r, D)) =
+              __float_as_uint(r ? s[1] : s[0]) >> 16 | (__float_as_uint(r ? z[1] : z[0]) & 0xffff0000u);
+        continue;
       }
-      __nv_bfloat16 z16 = bf16_down(least);
-      const double z64 = __bfloat162float(z16);
-      __nv_bfloat16 s16 = bf16_up((most - z64) / 15.0);
-      if (__bfloat162float(s16) < 1.17549435e-38f) s16 = __float2bfloat16_rn(0.f);
-      odd |= !isfinite(z64) || !isfinite(__bfloat162float(s16));
-      if (odd) z16 = s16 = __ushort_as_bfloat16(0x7fc0);
-      const double s64 = __bfloat162float(s16);
-#pragma unroll
-      for (int i = 0; i < E; ++i) code[i] = !odd && s64 > 0.0 ? (uint32_t)fmin(fmax(rint((d[i] - z64) / s64), 0.0), 15.0) : 0u;
-      sz = (uint32_t)__bfloat16_as_ushort(s16) | (uint32_t)__bfloat16_as_ushort(z16) << 16;
+      for (int u = 0; u < 2 && 2 * p + u < count; ++u) {
+        const int h = first + 2 * p + u;
+        append_exact<T, TW, D>(reinterpret_cast<const T*>(rows_s) + (size_t)h * D, is_k ? k_w : (const TW*)nullptr, eps,
+                               is_k ? turn : nullptr, adjacent != 0, is_k, slot,
+                               (is_k ? k_pool + (size_t)(h0 + h - n_q) * head_bytes
+                                     : v_pool + (size_t)(h0 + h - n_q - n_kv) * head_bytes) + unit);
+      }
     }
-    // the word's lanes put their nibbles together (element 2 j in nibble j, 2 j + 1 in nibble j + 4), the first of them stores it
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < E; i += 2) word |= (code[i] | code[i + 1] << 16) << (4 * (i >> 1));
-    word <<= 4 * (E / 2) * (lane % kWordLanes);
-#pragma unroll
-    for (int o = 1; o < kWordLanes; o <<= 1) word |= __shfl_xor_sync(0xffffffffu, word, o);
-    uint8_t* to = (is_k ? k_pool + (size_t)(h - n_q) * head_bytes : v_pool + (size_t)(h - n_q - n_kv) * head_bytes) + unit;
-    if (lane % kWordLanes == 0) *reinterpret_cast<uint32_t*>(to + (is_k ? key_at : value_at)) = word;
-    if (lane % kGroupLanes == 0) *reinterpret_cast<uint32_t*>(to + scale_at(slot, lane / kGroupLanes, D)) = sz;
-  }
+    p -= (count + 1) / 2;
+  };
+  if (in_table) {
+    if (k_w != nullptr && p < (n_keys + 1) / 2) weights(k_w);
+    store(true, n_queries, n_keys);
+  } else p -= (n_keys + 1) / 2;
+  store(false, n_queries + n_keys, n_values);
 }
 
 // What the pages hold for the step's tokens: rows [n_tokens][n_kv * d] of keys and of values.  grid = (tokens, blocks of heads); a warp takes
@@ -548,28 +692,29 @@ extern "C" int leone_append4(int dtype, void* qkv, int n_tokens, int n_q, int n_
   if (n_q <= 0 || !pool_ok(d, n_kv, page_tokens, table_width, k_pool, v_pool)) return kRefusedSize;
   if (rope != nullptr && (rotary_dim <= 0 || rotary_dim > d || (rotary_dim & 1))) return kRefusedSize;
   if (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return kRefusedAlignment;
-  // Heads that rotate whole or not at all.  A block has a head a warp for few tokens, all of a token's heads (up to 48) for many.
+  // Heads that rotate whole or not at all.  A block has two heads a warp for few tokens, all of a token's heads (up to 48) for many: 200
+  // tokens of 48 heads 6.0 us in blocks of 8 heads, 6.3 in blocks of 48; 500 tokens 10.3 and 7.8.
   if ((d == 64 || d == 128) && (rope == nullptr || rotary_dim == d) && (q_w == nullptr) == (k_w == nullptr) && ((uintptr_t)qkv & 15) == 0 &&
       n_q + 2 * n_kv <= 65535) {
-    const int heads = n_q + 2 * n_kv, most = n_tokens <= 96 ? cache4::kAppendWarps : cache4::kAppendHeads;
+    const int heads = n_q + 2 * n_kv, most = n_tokens <= 200 ? 2 * cache4::kAppendWarps : cache4::kAppendHeads;
     const int blocks_of = (heads + most - 1) / most, per = (heads + blocks_of - 1) / blocks_of;
     const dim3 grid(n_tokens, blocks_of);
     const size_t row_bytes = (size_t)per * d * (dtype == 0 ? 4 : 2);
-#define LAUNCH_VEC(T, TW, E)                                                                                                     \
-  return launch_kernel(cache4::append_vec_kernel<T, TW, E>, grid, dim3(32 * cache4::kAppendWarps), row_bytes, stream, (T*)qkv, n_q, n_kv, \
+#define LAUNCH_VEC(T, TW, D)                                                                                                     \
+  return launch_kernel(cache4::append_vec_kernel<T, TW, D>, grid, dim3(32 * cache4::kAppendWarps), row_bytes, stream, (T*)qkv, n_q, n_kv, \
                        (const TW*)q_w, (const TW*)k_w, eps, (const float2*)rope, max_positions, positions, seq_of_token,          \
                        block_table, table_width, n_seqs, (uint8_t*)k_pool, (uint8_t*)v_pool, num_pages, page_tokens, adjacent, per, \
                        status)
     if (d == 64) {
-      if (dtype == 0 && w_dtype == 0) LAUNCH_VEC(float, float, 2);
-      if (dtype == 1 && w_dtype == 0) LAUNCH_VEC(__nv_bfloat16, float, 2);
-      if (dtype == 0 && w_dtype == 1) LAUNCH_VEC(float, __nv_bfloat16, 2);
-      if (dtype == 1 && w_dtype == 1) LAUNCH_VEC(__nv_bfloat16, __nv_bfloat16, 2);
+      if (dtype == 0 && w_dtype == 0) LAUNCH_VEC(float, float, 64);
+      if (dtype == 1 && w_dtype == 0) LAUNCH_VEC(__nv_bfloat16, float, 64);
+      if (dtype == 0 && w_dtype == 1) LAUNCH_VEC(float, __nv_bfloat16, 64);
+      if (dtype == 1 && w_dtype == 1) LAUNCH_VEC(__nv_bfloat16, __nv_bfloat16, 64);
     } else {
-      if (dtype == 0 && w_dtype == 0) LAUNCH_VEC(float, float, 4);
-      if (dtype == 1 && w_dtype == 0) LAUNCH_VEC(__nv_bfloat16, float, 4);
-      if (dtype == 0 && w_dtype == 1) LAUNCH_VEC(float, __nv_bfloat16, 4);
-      if (dtype == 1 && w_dtype == 1) LAUNCH_VEC(__nv_bfloat16, __nv_bfloat16, 4);
+      if (dtype == 0 && w_dtype == 0) LAUNCH_VEC(float, float, 128);
+      if (dtype == 1 && w_dtype == 0) LAUNCH_VEC(__nv_bfloat16, float, 128);
+      if (dtype == 0 && w_dtype == 1) LAUNCH_VEC(float, __nv_bfloat16, 128);
+      if (dtype == 1 && w_dtype == 1) LAUNCH_VEC(__nv_bfloat16, __nv_bfloat16, 128);
     }
 #undef LAUNCH_VEC
   }

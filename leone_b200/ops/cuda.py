@@ -672,12 +672,14 @@ class CudaOps:
     force_prompt4_splits = 0               # > 0: the same for prompt portions
 
     def choose_prompt4_splits(self, n_seqs: int, n_kv: int, group: int, q_len: int, keys: int) -> int:
-        """How many blocks share the keys of a query tile (128 rows of tokens and heads) of prompt portions over pages in 4 bits."""
+        """How many blocks share the keys of a query tile (128 rows of tokens and heads) of prompt portions over pages in 4 bits: as many
+        as one wave of blocks holds (128 tokens behind 8,000, 8 cached heads of 128: 54 us with 4, 82 with 5, 91 with 2), while a split
+        keeps two tiles of 128 keys (64 tokens behind 2,000: 23.7 with 8, 26.3 with 5; 17 behind 4,000: 16.4 with 16, 18.8 with 10)."""
         if self.force_prompt4_splits:
             return self.force_prompt4_splits
         tokens = 128 // group
         blocks = -(-q_len // tokens) * n_kv * n_seqs
-        return max(1, min(64, 148 // blocks, -(-keys // 128) // 3))
+        return max(1, min(64, 148 // blocks, -(-keys // 128) // 2))
 
     force_decode4_splits = 0               # > 0: every decode attention over pages in 4 bits splits its keys this many ways
 

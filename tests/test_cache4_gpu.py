@@ -147,6 +147,42 @@ def test_append_of_odd_groups(ops_of, dtype, d):
     assert step.ctx.status.tolist() == [0, 0, 0, 0]
 
 
+@pytest.mark.parametrize("pairing", ["half_split", "adjacent"])
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("dtype,d,n_kv", [(BF16, 128, 3), (FP32, 128, 2), (BF16, 64, 5), (FP32, 64, 1)])
+def test_append_of_many_rows(ops_of, dtype, d, n_kv, norm, pairing):
+    """So many rows that codes next to a border and scales in doubt are among them, and rows that no norm is at ease with."""
+    ops = ops_of(dtype)
+    step = Step([(1501, 0), (900, 333)], 16, DEV, seed=d)
+    n, n_q = step.ctx.n_tokens, 1
+    x = torch.randn((n, n_q + 2 * n_kv, d), generator=_gen(n_kv), device=DEV)
+    x[3] = 0.0
+    x[4] = 1.5
+    x[5] *= 1e-18
+    x[6] *= 1e18
+    x[7, :, 1:] *= 1e-7
+    x[8] = torch.arange(d, device=DEV) / 16
+    x[9] *= 1e-30
+    x[1600] = -0.25
+    rows = x.to(dtype).flatten(1)
+    weights = (1 + 0.1 * torch.randn((2, d), generator=_gen(2), device=DEV)).to(dtype) if norm else (None, None)
+    pools = _pools(step, n_kv, d)
+    table = build_rotary_table(int(step.pos.max()) + 1, d, 10000.0).to(DEV)
+    eps = 2.0 ** -20
+    ops.qk_norm_rope_write(step.ctx, rows.clone(), n_q, n_kv, d, weights[0], weights[1], eps, table, d, step.view(*pools),
+                           pairing=pairing)
+    k, v = rows.double().unflatten(1, (n_q + 2 * n_kv, d))[:, n_q:].split(n_kv, 1)
+    if norm:
+        k = k * weights[1].double() * torch.rsqrt(k.square().mean(-1, keepdim=True) + eps)
+    k = rotate(k, step.pos, 10000.0, pairing, d)
+    for pool, want, values in ((pools[0], k, False), (pools[1], v, True)):
+        have = [t[step.page, :, step.slot] for t in packed.unpack_pages(pool, d, values)]
+        codes, s, z = quantize4(want)
+        assert torch.equal(have[1].double(), s) and torch.equal(have[2].double(), z)
+        assert torch.equal(have[0].long(), codes)
+    assert step.ctx.status.tolist() == [0, 0, 0, 0]
+
+
 def test_append_and_read_report_bad_metadata(ops_of):
     ops = ops_of(BF16)
     d, n_kv = 128, 2
