@@ -218,7 +218,7 @@ __device__ __noinline__ void append_exact(const T* row, const TW* w, float eps, 
 // one that does is settled by the sign of x - z - (code + 1/2) s in 64 bits.  (Values in bfloat16 lie on a border more often than
 // not in a row.)  Where z or s is in doubt, or something not finite, the warp computes the row again, which a step hardly ever does: that
 // code is never in the instruction cache, and a block waits 4 us for it.  (With norm and rotation in 32 bits a row of keys in a hundred
-// was in doubt: 2,048 tokens of 48 heads of 128 took 28.2 us, of 22 of 64 10.6, where this takes 21.5 and 8.7.
+// was in doubt: 2,048 tokens of 48 heads of 128 took 28.2 us, of 22 of 64 10.6, where this takes 20.7 and 8.6.
 // Their queries alone take 8.6, the floor is 5.)
 constexpr float kRounded = 1.01f / 16777216.f;
 constexpr float kToInteger = 12582912.f;           // 1.5 2^23: adding it rounds to an integer, which the low bits then hold
@@ -242,6 +242,17 @@ __device__ __forceinline__ float half_max(float v) {
   return v;
 }
 
+// The largest number of 8 bits that is not above v, and the smallest that is not below v >= 0; v finite (of another a doubt is known).
+__device__ __forceinline__ float eight_bits_down(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return __uint_as_float((b + ((int)b < 0 ? 0xffffu : 0u)) & 0xffff0000u);
+}
+__device__ __forceinline__ float eight_bits_up(float v) { return __uint_as_float((__float_as_uint(v) + 0xffffu) & 0xffff0000u); }
+__device__ __forceinline__ float reciprocal(float v) {                   // off by at most 2^-23 of itself
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 template <typename F> __device__ __forceinline__ void turn_pair(F& x, F& y, float2 c) {
   const F u = x * (F)c.x - y * (F)c.y;
   y = x * (F)c.y + y * (F)c.x;
@@ -421,12 +432,12 @@ append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__
         lo[g] = half_min(lo[g]);
         hi[g] = half_max(hi[g]);
         const float err = computed ? fmaxf(fabsf(lo[g]), fabsf(hi[g])) * kRounded : 0.f;
-        z[g] = __bfloat162float(__float2bfloat16_rd(__fsub_rd(lo[g], err)));
-        doubt |= z[g] != __bfloat162float(__float2bfloat16_rd(__fadd_ru(lo[g], err)));
+        z[g] = eight_bits_down(__fsub_rd(lo[g], err));
+        doubt |= z[g] != eight_bits_down(__fadd_ru(lo[g], err));
         // s is the smallest with 15 s >= hi - z; 15 s has 12 bits.  Of a value the rounded difference is on the side of 15 s that the
         // difference is on, or meets it; of a key it is off by the maximum's rounding and its own (and the margin's).
         const float range = hi[g] - z[g], margin = err + 2.f * kRounded * range;
-        s[g] = __bfloat162float(__float2bfloat16_ru(range * (1.f / 15.f) * (1.f - 6e-7f)));    // or the next
+        s[g] = eight_bits_up(range * (1.f / 15.f) * (1.f - 6e-7f));         // or the next
         if (15.f * s[g] < range) s[g] = __uint_as_float(__float_as_uint(s[g]) + 0x10000u);
         if (err != 0.f) {
           const float below = __uint_as_float(__float_as_uint(s[g]) - 0x10000u);
@@ -436,7 +447,7 @@ append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__
           doubt |= (hi[g] - (range + back)) + (back - z[g]) != 0.f;
         }
         doubt |= (s[g] != 0.f && !(s[g] > 1e-37f && s[g] < 1e37f)) || !(fabsf(z[g]) < 3e38f);
-        inv[g] = s[g] > 0.f ? __frcp_rn(s[g]) : 0.f;
+        inv[g] = s[g] > 0.f ? reciprocal(s[g]) : 0.f;
         limit[g] = 0.5f - fmaf(err, inv[g] * 1.01f, 15.5f * 2.5e-7f);
       }
       if (G == 1) {
