@@ -1080,7 +1080,7 @@ extern "C" int leone_attention4_prefill(const void* qkv, int row_stride, void* o
   if (page_tokens <= 0 || page_tokens % cache4::kUnit != 0 || table_width <= 0 || n_seqs > 65535) return kRefusedSize;
   if (splits < 1 || splits > 64 || (splits > 1) != (part_o != nullptr) || (part_o == nullptr) != (part_ml == nullptr)) return kRefusedSize;
   if (row_stride % 8 != 0 || out_stride % 8 != 0) return kRefusedAlignment;
-  if (((uintptr_t)qkv | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)part_o | (uintptr_t)part_ml) & 15)
+  if (((uintptr_t)qkv | (uintptr_t)out | (uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)part_o) & 15 || ((uintptr_t)part_ml & 7))
     return kRefusedAlignment;
   const pingpong::PagedArgs pa{(const __nv_bfloat16*)k_pool, (const __nv_bfloat16*)v_pool, block_table, table_width,
                                page_tokens, num_pages, n_kv};

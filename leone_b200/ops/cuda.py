@@ -519,6 +519,18 @@ class CudaOps:
             self._scratch_bufs[key] = buf
         return buf[:rows]
 
+    def _workspace(self, name: str, count: int, dtype=torch.float32) -> torch.Tensor:
+        """``count`` numbers for the call at hand.  A captured graph has its own (from the graph's pool), so that graphs may be replayed
+        beside one another; every other call one of its stream's, which only grows."""
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(count, dtype=dtype, device=self.device)
+        held = self.__dict__.setdefault("_workspaces", {})
+        key = (name, self._stream())
+        buf = held.get(key)
+        if buf is None or buf.numel() < count:
+            buf = held[key] = torch.empty(max(count, 1 << 16), dtype=dtype, device=self.device)
+        return buf
+
     def qk_norm_rope_write(self, ctx, qkv, n_q, n_kv, d, q_norm_w, k_norm_w, eps, table,
                            rotary_dim, cache, pairing="half_split"):
         """``pairing``: which elements of a head form rotation pair ``i``: ``(i, i + rotary_dim/2)``
@@ -542,6 +554,7 @@ class CudaOps:
             max_pos = shape[0]
         if cache is not None and getattr(cache, "bits", None) == 4:
             pool_args = self._pool4(cache, n_kv, d)
+            _need(ctx.positions.numel() >= n and ctx.seq_of_token.numel() >= n, "qk_norm_rope_write: a position for every token")
             self.launches += 1
             _check(self.packed_calls.leone_append4(
                 _dt(dtype), qkv, n, n_q, n_kv, d, q_norm_w, k_norm_w, w_dtype, float(eps), table, rotary_dim, max_pos, ctx.positions,
@@ -608,6 +621,7 @@ class CudaOps:
         portions each have their kernel), everything else on the kernel of any size."""
         bt, width, rows, kp, vp, pages, page_tokens = pool = self._pool4(cache, n_kv, d)
         n, row_stride = qkv.shape[0], qkv.stride(0)
+        _need(rows >= ctx.n_seqs, "attention: a row of the block table for every sequence")
         _need(n_q > 0 and n_q % n_kv == 0 and qkv.stride(1) == 1 and qkv.shape[1] >= n_q * d, "attention: query rows")
         if n == 0:
             return
@@ -651,23 +665,24 @@ class CudaOps:
         n_seqs, stream = ctx.n_seqs - lead, self._stream()
         splits = self.force_prompt4_splits or \
             self.choose_prompt4_splits(n_seqs, n_kv, n_q // n_kv, q_len, min(keys, window + q_len) if window else keys)
-        part_o = part_ml = None
+        parts = to_o = to_ml = None
         if splits > 1:
-            # outputs [token][head][split][d], then (maximum, sum) [token][head][split]; the leading decode rows' stay unused
-            count = n * n_q * splits
-            part_o = self._scratch("attention4_parts", -(-count * (d + 2) // 1024), 1024, torch.float32).data_ptr()
+            # outputs [token][head][split][d], then (maximum, sum) [token][head][split], of the tokens behind the leading rows; the kernel
+            # counts from the step's first token
+            count, skipped = (n - lead) * n_q * splits, lead * n_q * splits
+            parts = self._workspace("attention4_parts", count * (d + 2))
+            part_o = parts.data_ptr()
             part_ml = part_o + 4 * count * d
+            to_o, to_ml = part_o - 4 * skipped * d, part_ml - 8 * skipped
             self.launches += 1
         self.launches += 1
         _check(self.fast.calls.leone_attention4_prefill(
             q, row_stride, o, out_stride, kp, vp, bt.data_ptr() + 4 * lead * width, width, ctx.q_start.data_ptr() + 4 * lead,
-            ctx.ctx_len.data_ptr() + 4 * lead, n_seqs, q_len, n_q, n_kv, d, scale, window, page_tokens, pages, splits, part_o, part_ml,
+            ctx.ctx_len.data_ptr() + 4 * lead, n_seqs, q_len, n_q, n_kv, d, scale, window, page_tokens, pages, splits, to_o, to_ml,
             ctx.status, stream), "attention (4 bits, prompt)")
         if splits > 1:
-            first = lead * n_q * splits
             _check(self.packed_calls.leone_attention4_merge(
-                part_o + 4 * first * d, part_ml + 8 * first, o + 2 * lead * out_stride, out_stride, n - lead, n_q, d, splits, stream),
-                "attention (4 bits, merge)")
+                part_o, part_ml, o + 2 * lead * out_stride, out_stride, n - lead, n_q, d, splits, stream), "attention (4 bits, merge)")
 
     force_prompt4_splits = 0               # > 0: the same for prompt portions
 
@@ -710,7 +725,7 @@ class CudaOps:
             in_cluster = 1 < splits <= 8
         scratch = None
         if splits > 1 and not in_cluster:
-            scratch = self._scratch("attention4", -(-n_seqs * n_q * splits * (d + 2) // 1024), 1024, torch.float32)
+            scratch = self._workspace("attention4", n_seqs * n_q * splits * (d + 2))
             self.launches += 1
         self.launches += 1
         _check(calls.leone_attention4_decode(

@@ -67,7 +67,7 @@ class Int8Products:
             self.lib.leone_bf16_set_pdl(1 if ops._pdl else 0)
         self.calls = EntryPoints(self.lib)
         self.sm_count = torch.cuda.get_device_properties(ops.device).multi_processor_count
-        self.plans, self.buffers, self.retired = {}, {}, []
+        self.plans, self.buffers = {}, {}
 
     force = None               # (form, splits or tile width) of every product, whatever the rule says (tests set it)
 
@@ -123,14 +123,15 @@ class Int8Products:
         return 2
 
     def tokens(self, m: int, k: int, stream):
-        """Codes and scales of ``m`` tokens: one buffer for each width and stream, which only grows; an outgrown one stays for captured graphs
-        that use it."""
-        key = (k, stream)
-        held = self.buffers.get(key)
-        if held is None or held[0].shape[0] < m:
-            if held is not None:
-                self.retired.append(held)
-            rows = max(m, 64 if held is None else 2 * held[0].shape[0])
-            held = self.buffers[key] = (torch.empty((rows, k), dtype=torch.int8, device=self.ops.device),
-                                        torch.empty(rows, dtype=torch.float32, device=self.ops.device))
-        return held
+        """Codes and scales of ``m`` tokens for the call at hand.  A captured graph has its own (from the graph's pool), so that graphs may
+        be replayed beside one another; every other call those of its width and stream, which only grow."""
+        captured = torch.cuda.is_current_stream_capturing()
+        held = None if captured else self.buffers.get((k, stream))
+        if held is not None and held[0].shape[0] >= m:
+            return held
+        rows = m if captured else -(-m // 64) * 64
+        fresh = (torch.empty((rows, k), dtype=torch.int8, device=self.ops.device),
+                 torch.empty(rows, dtype=torch.float32, device=self.ops.device))
+        if not captured:
+            self.buffers[k, stream] = fresh
+        return fresh

@@ -48,6 +48,7 @@ import math
 
 import torch
 
+from ..cache import packed
 from ..registry import MIXERS
 from .base import DeferredNorm, Mixer, PagedKV, WeightSpec
 
@@ -174,7 +175,8 @@ class Attention(Mixer):
 
     def scratch_bytes(self, max_tokens):
         return max_tokens * (self.in_cols + self.n_q * self.dv) * self.rt.dtype.itemsize + \
-            self.rt.token_scratch_bytes(max_tokens, self.hidden) + self.rt.token_scratch_bytes(max_tokens, self.n_q * self.dv)
+            self.rt.token_scratch_bytes(max_tokens, self.hidden) + self.rt.token_scratch_bytes(max_tokens, self.n_q * self.dv) + \
+            (packed.ATTENTION_WORKSPACE if self.rt.cache_bits == 4 else 0)
 
     def load_transient_bytes(self):
         return self.in_cols * self.hidden * self.rt.dtype.itemsize       # q, k, v beside their stacked copy

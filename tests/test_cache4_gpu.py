@@ -359,6 +359,63 @@ def test_attention_prompt(ops_of, n_q, n_kv, d, lens, page, window, splits):
     assert ((out - want).abs() <= _bounds(BF16, step, d, n_q, want, top_s, top_v, True) + extra[..., None]).all()
 
 
+def test_attention_prompt_behind_an_odd_number_of_rows(ops_of):
+    """Three leading rows, seven heads, three splits: an odd number of parts stands before the portion's."""
+    ops = ops_of(BF16)
+    n_q, n_kv, d = 7, 1, 64
+    ops.force_prompt4_splits = 3
+    try:
+        step, qkv, pools, out, want, top_s, top_v = _attention_case(ops, BF16, n_q, n_kv, d, [(1, 30), (1, 7), (1, 100), (40, 700)], 16, 0)
+    finally:
+        ops.force_prompt4_splits = 0
+    half = 2.0 ** -8
+    extra = top_v * (2 * half * top_s + half)
+    assert ((out - want).abs() <= _bounds(BF16, step, d, n_q, want, top_s, top_v, True) + extra[..., None]).all()
+
+
+@pytest.mark.parametrize("lens,splits", [([(1, 9000)], 33), ([(40, 5000)], 18)])
+def test_attention_of_two_graphs_at_once(ops_of, lens, splits):
+    """Two captured calls that split their keys, replayed beside one another on two streams, and two eager ones: neither writes into the
+    other's parts."""
+    ops = ops_of(BF16)
+    n_q, n_kv, d = 8, 2, 128
+    ops.force_decode4_splits = ops.force_prompt4_splits = splits
+    try:
+        cases = []
+        for seed in (1, 2):
+            step, qkv, pools, out, *_ = _attention_case(ops, BF16, n_q, n_kv, d, lens, 16, 0, seed=seed)
+            view, got = step.view(*pools), torch.zeros((qkv.shape[0], n_q * d), dtype=BF16, device=DEV)
+            cases.append((step, qkv, view, got, out.flatten(1).to(BF16)))
+
+        def call(step, qkv, view, got, _):
+            ops.attention(step.ctx, qkv, got, n_q, n_kv, d, d ** -0.5, None, view)
+
+        streams, graphs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+        for case in cases:
+            graph = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph, stream=streams[0]):
+                call(*case)
+            graphs.append(graph)
+        for eager in (False, True):
+            for _ in range(20):
+                for case in cases:
+                    case[3].zero_()
+                torch.cuda.synchronize()
+                for stream, graph, case in zip(streams, graphs, cases):
+                    with torch.cuda.stream(stream):
+                        if eager:
+                            call(*case)
+                        else:
+                            graph.replay()
+                torch.cuda.synchronize()
+                for case in cases:
+                    assert torch.equal(case[3], case[4])
+        del graphs
+    finally:
+        ops.force_decode4_splits = ops.force_prompt4_splits = 0
+
+
 @pytest.mark.parametrize("window", [0, 40])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("many", [False, True])
@@ -446,3 +503,7 @@ def test_attention_refusals(ops_of):
     bad = step.view(*pools)
     bad.block_table = step.table.long()
     refused("block table", cache=bad)
+    bad.block_table = step.table[:0]
+    refused("row of the block table", cache=bad)
+    with pytest.raises(KernelError, match="position for every token"):
+        ops.qk_norm_rope_write(step.ctx, qkv.repeat(2, 1), n_q, n_kv, d, None, None, 1e-6, None, 0, good)

@@ -222,3 +222,37 @@ def test_refusals(ops_of):
     with pytest.raises(KernelError, match="differ"):
         ops.prepare_gate_up_int8(codes, scales, codes[:32], scales[:32])
     ops.linear(x[:0], w, out[:0])                              # no tokens: nothing to do
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 4096, 8192), (100, 2048, 8192), (300, 2048, 4096)])
+def test_two_graphs_at_once(ops_of, m, n, k):
+    """Two captured products of one width, replayed beside one another on two streams, and two eager ones: each has its own tokens."""
+    ops = ops_of(BF16)
+    cases = []
+    for seed in (1, 2):
+        x, codes, scales = _inputs(m, n, k, BF16, seed)
+        w, want = ops.prepare_matrix_int8(codes, scales), torch.empty((m, n), dtype=BF16, device=DEV)
+        ops.linear(x, w, want)
+        cases.append((x, w, torch.empty_like(want), want))
+    streams, graphs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for x, w, got, _ in cases:
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=streams[0]):
+            ops.linear(x, w, got)
+        graphs.append(graph)
+    for eager in (False, True):
+        for _ in range(20):
+            for case in cases:
+                case[2].zero_()
+            torch.cuda.synchronize()
+            for stream, graph, (x, w, got, _) in zip(streams, graphs, cases):
+                with torch.cuda.stream(stream):
+                    if eager:
+                        ops.linear(x, w, got)
+                    else:
+                        graph.replay()
+            torch.cuda.synchronize()
+            for _, _, got, want in cases:
+                assert torch.equal(got, want)
+    del graphs
