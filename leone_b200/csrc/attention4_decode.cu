@@ -15,11 +15,18 @@
 //
 // Keys ride the MMA's M side and up to 8 query heads its N side (NT tiles of them), as in attention_tiled.cu.  The pages' layout is
 // made so that a thread's operands are words that lie side by side: 16 keys are one piece of 1,152 bytes (576 with 64 elements) for
-// keys and one for values, each fetched by one untiled copy of the TMA into a ring of kStages units that every warp has of its own,
-// and read from there with 16- and 8-byte loads without bank conflicts.
+// keys and one for values, each fetched by one untiled copy of the TMA into a ring of kStages parts of kPart units that every warp
+// has of its own, and read from there with 16- and 8-byte loads without bank conflicts.
 //
 // A block is 4 warps for one (sequence, cached head, up to 16 of its query heads, split of the keys); its warps take units in turn.
 // Splits of up to 8 merge inside a thread-block cluster through distributed shared memory, more through scratch and a kernel.
+//
+// 32 query heads on 8 of 128, one call behind another: 166 sequences of 2,048 keys 87 us (4.5 TB/s of the copy's 6.5), 64 of them 45 us (512
+// blocks where 444 run at once), 64 of up to 2,048 30 us, one of 40,960 19.4 us (2.4 TB/s).  What bounds it is the instructions: with every page
+// in the L2 166 sequences take 92 us where they take 96 from memory; 12 warps an SM keep half of the issue slots busy (fixed latencies first,
+// then the ALUs that mask codes).  Of 296 instructions for 16 keys the scores take 74, the outputs 105, maximum, weights and the ring 80.
+// Slower or no faster: four blocks an SM with parts of two (64 sequences 41 us, of up to 2,048 34, one of 40,960 23), parts of one, keys
+// dealt to warps as one line of all sequences, blocks that sort the sequences by length themselves.
 #include "cache4.cuh"
 #include "tc_common.cuh"
 

@@ -10,8 +10,8 @@
 // the low half, z in the high half), so that a unit of keys or values is one piece of 16 * row_bytes(d) bytes (a multiple of
 // 16): 1,152 for 128 elements, where bfloat16 has 4,096.  How the words of codes lie in a unit follows the tensor cores' operands:
 //   * word w of a row holds elements 8 w .. 8 w + 7, element 2 j in nibble j and element 2 j + 1 in nibble j + 4: (word >> 4 j) &
-//     0x000f000f is the pair 2 j, 2 j + 1 in the two halves of a register, and with 0x4300 in front of each code the pair is 128 +
-//     code in bfloat16 (whose step is 1 from 128 to 256).
+//     0x000f000f is the pair 2 j, 2 j + 1 in the two halves of a register.  As bit patterns codes are numbers already (c 2^-133 in
+//     bfloat16, c 2^-24 in fp16, 16 times that in bits 4-7), so that one AND makes an operand of a tensor core.
 //   * keys: a thread of an mma.sync operand needs, of the key of its row, a quarter of every group: with groups of 64 word (g, i)
 //     of a row stands at (i / 2) * 2 G + 2 g + i % 2, so that a thread's words are side by side (16 bytes with 128 elements).
 //   * values: a thread needs the same 8 elements of every group of four tokens: word (g, i) stands at i * G + g.  Of the tokens

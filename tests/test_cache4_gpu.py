@@ -242,7 +242,7 @@ def _bounds(dtype, step, d, n_q, want, top_s, top_v, tensor_cores):
     """How far an output may be off, per (token, head).
 
     Scores: d products summed in fp32, relative to sum |q k| at most (d + 4) 2^-23 (a tensor core's additions truncate).  On tensor cores
-    codes are 128 + code, 9 times the largest code, and the offset is taken out again: 10 times that.  A score's error moves each
+    a form may have codes as 128 + code, 9 times the largest code, and take the offset out again: 10 times that.  A score's error moves each
     weight by that much relative to itself, twice (the sum too).  Weights and sums: (keys + 8) 2^-23.  On tensor cores a weight times its
     scale is rounded to bfloat16: a half step of the weighted codes around their middle, 8 s <= 0.54 (max - min) of 2^-8 each; again
     codes of 128 + code in the sums.  Then one rounding to the type."""
