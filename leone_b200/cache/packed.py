@@ -12,9 +12,12 @@ import torch
 
 UNIT = 16          # tokens whose rows lie together; pages are multiples of it
 MAX_DIM = 512
-# What the parts of split attention over such pages take at most: 148 tiles of 128 rows of prompt portions, or three blocks an SM of up to 16
-# rows of decode, 130 numbers each.
-ATTENTION_WORKSPACE = 148 * 130 * 4 * (128 + 3 * 16)
+
+def attention_workspace(d: int) -> int:
+    """Bytes that the parts of split attention over such pages take at most: 148 tiles of 128 rows of prompt portions, three blocks an SM of up
+    to 16 rows of decode, or 2,048 blocks of 8 rows of the kernel of any size."""
+    return 4 * ((148 * 128 + 3 * 148 * 16) * 130 + 2048 * 8 * (d + 2))
+
 
 
 def groups(d: int) -> int:

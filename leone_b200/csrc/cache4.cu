@@ -555,47 +555,67 @@ read_kernel(T* __restrict__ k_out, T* __restrict__ v_out, int n_kv, int d, const
 }
 
 // Causal grouped-query attention over pages in 4 bits, any sizes, any cut: the formulas of attention_generic.cu.  One block per
-// (token, cached head, up to 8 of its query heads) walks the keys in tiles of 32: a tile's keys, then its values, are brought into
-// shared memory in fp32; warp w has the scores of heads w and w + 4, a lane a key; thread c sums the outputs' columns c, c + 128, ..
+// (token, cached head, up to kHeads of its query heads, split of the keys) walks its keys in tiles of 32: a tile's keys, then its values,
+// are brought into shared memory in fp32; warp w has the scores of heads w and w + 4, a lane a key; thread c sums the outputs' columns
+// c, c + 128, ..  A key's or value's number is read once for all heads (2,048 tokens behind 6,144, 32 heads on 8 of
+// 128: 34 ms, 58 where it was read for each).  Where there are too few blocks for the SMs,
+// `splits` of them share a token's keys and leave their (maximum, sum, unnormalised outputs) in scratch, [token][query head][split], for
+// attention_any_merge_kernel (one sequence of 8,192 keys, 8 heads on 2
+// of 128, 32 bits: 31 us with 64, 1,380 without).
 constexpr int kAnyThreads = 128;
 constexpr int kAnyKeys = 32;
-constexpr int kAnyHeads = 8;
 __host__ __device__ constexpr int any_row(int d) { return d + 1; }      // floats between the tile's rows: lanes on different banks
 
-template <typename T>
+template <typename T, int kHeads>
 __global__ void __launch_bounds__(kAnyThreads)
 attention_any_kernel(const T* __restrict__ qkv, int row_stride, T* __restrict__ out, int out_stride,
                      const uint8_t* __restrict__ k_pool, const uint8_t* __restrict__ v_pool, const int* __restrict__ block_table,
                      int table_width, const int* __restrict__ seq_of_token, const int* __restrict__ positions, int n_q, int n_kv,
-                     int d, float scale, int window, int page_tokens, int num_pages, int n_seqs, int* status) {
+                     int d, float scale, int window, int page_tokens, int num_pages, int n_seqs, int splits, float* __restrict__ part_o,
+                     float* __restrict__ part_ml, int* status) {
   extern __shared__ float smem_f[];
   float* tile = smem_f;                                    // [32][any_row(d)]
-  float* q_s = tile + kAnyKeys * any_row(d);               // [8][d]
-  float* p_s = q_s + kAnyHeads * d;                        // [8][32]
-  float* alpha_s = p_s + kAnyHeads * kAnyKeys;             // [8]
-  float* l_s = alpha_s + kAnyHeads;                        // [8]
+  float* q_s = tile + kAnyKeys * any_row(d);               // [kHeads][d]
+  float* p_s = q_s + kHeads * d;                           // [32][kHeads]
+  float* alpha_s = p_s + kHeads * kAnyKeys;                // [kHeads]
+  float* l_s = alpha_s + kHeads;                           // [kHeads]
   __shared__ long long unit_s[kAnyKeys];
+  constexpr int kWarpHeads = (kHeads + 3) / 4;             // of a warp
   pdl_trigger();
   pdl_wait();
-  const int t = blockIdx.x, g = n_q / n_kv, parts = (g + kAnyHeads - 1) / kAnyHeads;
+  const int t = blockIdx.x, g = n_q / n_kv, parts = (g + kHeads - 1) / kHeads;
   const int kvh = blockIdx.y / parts, part = blockIdx.y - kvh * parts;
-  const int head0 = kvh * g + part * kAnyHeads, heads = min(kAnyHeads, g - part * kAnyHeads);
+  const int head0 = kvh * g + part * kHeads, heads = min(kHeads, g - part * kHeads);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int pos = positions[t], s = seq_of_token[t];
   T* dst = out + (size_t)t * out_stride + (size_t)head0 * d;
+  auto part_at = [&](int h) { return ((size_t)t * n_q + head0 + h) * splits + blockIdx.z; };
   if (s < 0 || s >= n_seqs || pos < 0) {
     if (tid == 0) set_status(status, s < 0 || s >= n_seqs ? kBadSequence : kBadPosition, t, s < 0 || s >= n_seqs ? s : pos);
+    if (splits > 1) {
+      if (tid < heads) *reinterpret_cast<float2*>(part_ml + 2 * part_at(tid)) = make_float2(-INFINITY, 0.f);
+      return;
+    }
     for (int c = tid; c < heads * d; c += kAnyThreads) dst[c] = from_float<T>(0.f);
     return;
   }
   const T* q = qkv + (size_t)t * row_stride + (size_t)head0 * d;
-  for (int c = tid; c < heads * d; c += kAnyThreads) q_s[c] = to_float<T>(q[c]);
+  for (int c = tid; c < kHeads * d; c += kAnyThreads) q_s[c] = c < heads * d ? to_float<T>(q[c]) : 0.f;
+  for (int c = tid; c < kHeads * (kAnyKeys + 1); c += kAnyThreads) p_s[c] = 0.f;        // (and alpha_s: heads that are not there)
   const int G = groups(d), size = d / G, words = d / 8;
-  const int lo = window > 0 ? max(0, pos - window + 1) : 0;
-  float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-  float acc[kAnyHeads][kMaxDim / kAnyThreads];
+  const int first = window > 0 ? max(0, pos - window + 1) : 0;
+  const int share = ((pos - first) / kAnyKeys + splits) / splits;               // tiles of a split, rounded up
+  const long long lo = first + (long long)blockIdx.z * share * kAnyKeys;
+  const int end = (int)min((long long)pos + 1, lo + (long long)share * kAnyKeys);
+  float m_run[kWarpHeads], l_run[kWarpHeads];
 #pragma unroll
-  for (int h = 0; h < kAnyHeads; ++h)
+  for (int u = 0; u < kWarpHeads; ++u) {
+    m_run[u] = -INFINITY;
+    l_run[u] = 0.f;
+  }
+  float acc[kHeads][kMaxDim / kAnyThreads];
+#pragma unroll
+  for (int h = 0; h < kHeads; ++h)
 #pragma unroll
     for (int i = 0; i < kMaxDim / kAnyThreads; ++i) acc[h][i] = 0.f;
   auto fetch = [&](const uint8_t* pool, bool keys, int j0) {
@@ -615,12 +635,12 @@ attention_any_kernel(const T* __restrict__ qkv, int row_stride, T* __restrict__ 
       for (int e = 0; e < 8; ++e) to[e] = fmaf(scale_of(sz), (float)code_of(word, e), offset_of(sz));
     }
   };
-  for (int j0 = lo; j0 <= pos; j0 += kAnyKeys) {
+  for (int j0 = (int)min(lo, (long long)end); j0 < end; j0 += kAnyKeys) {
     __syncthreads();                                       // the tile before is done with
     if (tid < kAnyKeys) {
       const int j = j0 + tid;
       long long unit = -1;
-      if (j <= pos) {
+      if (j < end) {
         const int blk = j / page_tokens;
         const int page = blk < table_width ? block_table[(size_t)s * table_width + blk] : -1;
         if (page < 0 || page >= num_pages) set_status(status, kBadPage, t, page, j);
@@ -631,22 +651,34 @@ attention_any_kernel(const T* __restrict__ qkv, int row_stride, T* __restrict__ 
     __syncthreads();
     fetch(k_pool, true, j0);
     __syncthreads();
+    float dot[kWarpHeads];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < kWarpHeads; ++u) dot[u] = 0.f;
+    if (warp < heads) {
+      const float* k = tile + lane * any_row(d);
+#pragma unroll 2
+      for (int c = 0; c < d; c += 4) {
+        const float k0 = k[c], k1 = k[c + 1], k2 = k[c + 2], k3 = k[c + 3];
+#pragma unroll
+        for (int u = 0; u < kWarpHeads; ++u) {
+          const float4 v = *reinterpret_cast<const float4*>(q_s + (warp + 4 * u) * d + c);
+          dot[u] = fmaf(v.w, k3, fmaf(v.z, k2, fmaf(v.y, k1, fmaf(v.x, k0, dot[u]))));
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kWarpHeads; ++u) {
       const int h = warp + 4 * u;
       if (h >= heads) break;
-      const float* k = tile + lane * any_row(d);
-      float dot = 0.f;
-      for (int c = 0; c < d; ++c) dot = fmaf(q_s[h * d + c], k[c], dot);
       const bool here = unit_s[lane] >= 0;
-      const float score = here ? dot * scale : -INFINITY;
+      const float score = here ? dot[u] * scale : -INFINITY;
       // (fmaxf leaves out a NaN; the weight of its key is NaN all the same, and with it the sum)
       const float m_new = fmaxf(m_run[u], warp_max(score));
       const float p = here ? (m_new == -INFINITY ? (isnan(score) ? score : 0.f) : expf(score - m_new)) : 0.f;
       const float alpha = m_run[u] == -INFINITY ? (l_run[u] == 0.f ? 0.f : 1.f) : expf(m_run[u] - m_new);
       l_run[u] = l_run[u] * alpha + warp_sum(p);
       m_run[u] = m_new;
-      p_s[h * kAnyKeys + lane] = p;
+      p_s[lane * kHeads + h] = p;
       if (lane == 0) alpha_s[h] = alpha;
     }
     __syncthreads();
@@ -657,28 +689,72 @@ attention_any_kernel(const T* __restrict__ qkv, int row_stride, T* __restrict__ 
       const int c = tid + i * kAnyThreads;
       if (c >= d) break;
 #pragma unroll
-      for (int h = 0; h < kAnyHeads; ++h) {
-        if (h >= heads) break;
-        float a = acc[h][i] * alpha_s[h];
-        for (int r = 0; r < kAnyKeys; ++r) a = fmaf(p_s[h * kAnyKeys + r], tile[r * any_row(d) + c], a);
-        acc[h][i] = a;
+      for (int h = 0; h < kHeads; ++h) acc[h][i] *= alpha_s[h];
+#pragma unroll 4
+      for (int r = 0; r < kAnyKeys; ++r) {
+        const float v = tile[r * any_row(d) + c];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) acc[h][i] = fmaf(p_s[r * kHeads + h], v, acc[h][i]);
       }
     }
   }
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
-    if (warp + 4 * u < heads && lane == 0) l_s[warp + 4 * u] = l_run[u];
+  for (int u = 0; u < kWarpHeads; ++u)
+    if (warp + 4 * u < heads && lane == 0) {
+      l_s[warp + 4 * u] = l_run[u];
+      if (splits > 1) *reinterpret_cast<float2*>(part_ml + 2 * part_at(warp + 4 * u)) = make_float2(m_run[u], l_run[u]);
+    }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kMaxDim / kAnyThreads; ++i) {
     const int c = tid + i * kAnyThreads;
     if (c >= d) break;
 #pragma unroll
-    for (int h = 0; h < kAnyHeads; ++h) {
+    for (int h = 0; h < kHeads; ++h) {
       if (h >= heads) break;
+      if (splits > 1) part_o[part_at(h) * d + c] = acc[h][i];
       // no key at all: 0; a sum that is NaN stays one
-      dst[(size_t)h * d + c] = from_float<T>(l_s[h] == 0.f ? 0.f : acc[h][i] / l_s[h]);
+      else dst[(size_t)h * d + c] = from_float<T>(l_s[h] == 0.f ? 0.f : acc[h][i] / l_s[h]);
     }
+  }
+}
+
+// grid = (tokens, heads): a head's parts, up to 64 of them, into its output.
+template <typename T>
+__global__ void __launch_bounds__(kAnyThreads)
+attention_any_merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, T* __restrict__ out, int out_stride,
+                           int n_q, int d, int splits) {
+  __shared__ float f_s[64];
+  __shared__ float l_s;
+  pdl_trigger();
+  pdl_wait();
+  const size_t base = ((size_t)blockIdx.x * n_q + blockIdx.y) * splits;
+  const int tid = threadIdx.x;
+  if (tid < 32) {
+    float2 v[2];
+    float f[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      v[i] = tid + 32 * i < splits ? *reinterpret_cast<const float2*>(part_ml + 2 * (base + tid + 32 * i)) : make_float2(-INFINITY, 0.f);
+    const float top = warp_max(fmaxf(v[0].x, v[1].x));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // a part without a key has no sums (perhaps its outputs were not written); one whose scores are all NaN has sums that are
+      f[i] = v[i].x == -INFINITY ? (v[i].y == 0.f ? 0.f : 1.f) : expf(v[i].x - top);
+      f_s[tid + 32 * i] = f[i];
+    }
+    const float sum = warp_sum(fmaf(f[0], v[0].y, f[1] * v[1].y));
+    if (tid == 0) l_s = sum;
+  }
+  __syncthreads();
+  for (int c = tid; c < d; c += kAnyThreads) {
+    float o = 0.f;
+#pragma unroll 16
+    for (int s = 0; s < splits; ++s) {
+      const float f = f_s[s];
+      o = fmaf(f, f != 0.f ? part_o[(base + s) * d + c] : 0.f, o);
+    }
+    out[(size_t)blockIdx.x * out_stride + (size_t)blockIdx.y * d + c] = from_float<T>(l_s == 0.f ? 0.f : o / l_s);
   }
 }
 
@@ -764,33 +840,52 @@ extern "C" int leone_read4(int dtype, void* k_out, void* v_out, int n_tokens, in
   return kRefusedDtype;
 }
 
-// Arguments as leone_attention_generic, the pools in 4 bits.
+template <typename T, int kHeads>
+static int launch_any(const void* qkv, int row_stride, void* out, int out_stride, const void* k_pool, const void* v_pool,
+                      const int* block_table, int table_width, const int* seq_of_token, const int* positions, int n_tokens, int n_q,
+                      int n_kv, int d, float scale, int window, int page_tokens, int num_pages, int n_seqs, int splits, float* scratch,
+                      int* status, cudaStream_t stream) {
+  using namespace cache4;
+  static bool configured = false;
+  if (!configured) {
+    cudaError_t e = cudaFuncSetAttribute(attention_any_kernel<T, kHeads>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+    if (e != cudaSuccess) return (int)e;
+    configured = true;
+  }
+  const long long rows = (long long)n_kv * ((n_q / n_kv + kHeads - 1) / kHeads);
+  if (rows > 65535) return kRefusedSize;
+  const int smem = (kAnyKeys * any_row(d) + kHeads * (d + kAnyKeys + 2)) * 4;
+  float* part_ml = splits > 1 ? scratch + (size_t)n_tokens * n_q * splits * d : nullptr;
+  const int e = launch_kernel(attention_any_kernel<T, kHeads>, dim3(n_tokens, (unsigned)rows, splits), dim3(kAnyThreads), smem, stream,
+                              (const T*)qkv, row_stride, (T*)out, out_stride, (const uint8_t*)k_pool, (const uint8_t*)v_pool,
+                              block_table, table_width, seq_of_token, positions, n_q, n_kv, d, scale, window, page_tokens, num_pages,
+                              n_seqs, splits, scratch, part_ml, status);
+  if (e != 0 || splits == 1) return e;
+  return launch_kernel(attention_any_merge_kernel<T>, dim3(n_tokens, n_q), dim3(kAnyThreads), 0, stream, (const float*)scratch,
+                       (const float*)part_ml, (T*)out, out_stride, n_q, d, splits);
+}
+
+// Arguments as leone_attention_generic, the pools in 4 bits.  `splits`: blocks that share a token's keys, up to 64; more than one take
+// n_tokens n_q splits (d + 2) floats of scratch.
 extern "C" int leone_attention4_any(int dtype, const void* qkv, int row_stride, void* out, int out_stride, const void* k_pool,
                                     const void* v_pool, const int* block_table, int table_width, const int* seq_of_token,
                                     const int* positions, int n_tokens, int n_q, int n_kv, int d, float scale, int window,
-                                    int page_tokens, int num_pages, int n_seqs, int* status, cudaStream_t stream) {
+                                    int page_tokens, int num_pages, int n_seqs, int splits, float* scratch, int* status,
+                                    cudaStream_t stream) {
   if (n_tokens <= 0) return 0;
   if (n_q <= 0 || !pool_ok(d, n_kv, page_tokens, table_width, k_pool, v_pool) || n_q % n_kv != 0) return kRefusedSize;
-  if (((uintptr_t)k_pool | (uintptr_t)v_pool) & 15) return kRefusedAlignment;
-  const long long rows = (long long)n_kv * ((n_q / n_kv + cache4::kAnyHeads - 1) / cache4::kAnyHeads);
-  if (rows > 65535) return kRefusedSize;
-  const int smem = (cache4::kAnyKeys * cache4::any_row(d) + cache4::kAnyHeads * (d + cache4::kAnyKeys + 2)) * 4;
-#define LAUNCH(T)                                                                                                              \
-  do {                                                                                                                         \
-    static bool configured = false;                                                                                            \
-    if (!configured) {                                                                                                         \
-      cudaError_t e = cudaFuncSetAttribute(cache4::attention_any_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,        \
-                                           100 * 1024);                                                                        \
-      if (e != cudaSuccess) return (int)e;                                                                                     \
-      configured = true;                                                                                                       \
-    }                                                                                                                          \
-    return launch_kernel(cache4::attention_any_kernel<T>, dim3(n_tokens, (unsigned)rows), dim3(cache4::kAnyThreads), smem, stream, \
-                         (const T*)qkv, row_stride, (T*)out, out_stride, (const uint8_t*)k_pool, (const uint8_t*)v_pool,        \
-                         block_table, table_width, seq_of_token, positions, n_q, n_kv, d, scale, window, page_tokens,           \
-                         num_pages, n_seqs, status);                                                                           \
-  } while (0)
-  if (dtype == 0) LAUNCH(float);
-  if (dtype == 1) LAUNCH(__nv_bfloat16);
+  if (splits < 1 || splits > 64 || (splits > 1) != (scratch != nullptr) || n_q > 65535) return kRefusedSize;
+  if (((uintptr_t)k_pool | (uintptr_t)v_pool | (uintptr_t)scratch) & 15) return kRefusedAlignment;
+  const int g = n_q / n_kv;
+#define LAUNCH(T, H)                                                                                                             \
+  return launch_any<T, H>(qkv, row_stride, out, out_stride, k_pool, v_pool, block_table, table_width, seq_of_token, positions,   \
+                          n_tokens, n_q, n_kv, d, scale, window, page_tokens, num_pages, n_seqs, splits, scratch, status, stream)
+  if (dtype == 0 && g <= 2) LAUNCH(float, 2);
+  if (dtype == 0 && g <= 4) LAUNCH(float, 4);
+  if (dtype == 0) LAUNCH(float, 8);
+  if (dtype == 1 && g <= 2) LAUNCH(__nv_bfloat16, 2);
+  if (dtype == 1 && g <= 4) LAUNCH(__nv_bfloat16, 4);
+  if (dtype == 1) LAUNCH(__nv_bfloat16, 8);
 #undef LAUNCH
   return kRefusedDtype;
 }

@@ -637,12 +637,16 @@ class CudaOps:
                 self._attention4_prompt(q, row_stride, o, out_stride, n, n_q, n_kv, d, scale, window, pool, ctx, lead, q_len, keys)
                 at = n
         if at < n:
+            splits, scratch = self.choose_any4_splits(n - at, n_kv, n_q // n_kv, min(int(ctx.max_ctx_len), window or 1 << 31)), None
+            if splits > 1:
+                scratch = self._workspace("attention4", (n - at) * n_q * splits * (d + 2))
+                self.launches += 1
             self.launches += 1
             item = qkv.element_size()
             _check(self.packed_calls.leone_attention4_any(
                 _dt(qkv.dtype), q + at * row_stride * item, row_stride, o + at * out_stride * item, out_stride, kp, vp, bt, width,
                 ctx.seq_of_token.data_ptr() + 4 * at, ctx.positions.data_ptr() + 4 * at, n - at, n_q, n_kv, d, scale, window, page_tokens,
-                pages, rows, ctx.status, self._stream()), "attention (4 bits)")
+                pages, rows, splits, scratch, ctx.status, self._stream()), "attention (4 bits)")
 
     def _parts4(self, ctx):
         """``(sequences of one token in front, the longest of them, the longest portion behind them, the most keys of one)``; looked up
@@ -695,6 +699,16 @@ class CudaOps:
         tokens = 128 // group
         blocks = -(-q_len // tokens) * n_kv * n_seqs
         return max(1, min(64, 148 // blocks, -(-keys // 128) // 2))
+
+    force_any4_splits = 0                  # > 0: the same for what the kernel of any size takes
+
+    def choose_any4_splits(self, n_tokens: int, n_kv: int, g: int, keys: int) -> int:
+        """How many blocks share a token's keys in the kernel of any size over pages in 4 bits: up to 2,048 blocks of 64 keys or more (32 bits,
+        heads of 128: one sequence of 8,192 keys, 2 cached heads 31 us with 64, 93 with 16, 1,380 with one; 8 of 2,048, 8 cached heads 51
+        with 32, 77 with 9, 350 with one; 64 of them 376 with 4, 631 with one)."""
+        if self.force_any4_splits:
+            return self.force_any4_splits
+        return max(1, min(64, 2048 // (n_tokens * n_kv * -(-g // 8)), keys // 64))
 
     force_decode4_splits = 0               # > 0: every decode attention over pages in 4 bits splits its keys this many ways
 

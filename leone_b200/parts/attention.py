@@ -176,7 +176,7 @@ class Attention(Mixer):
     def scratch_bytes(self, max_tokens):
         return max_tokens * (self.in_cols + self.n_q * self.dv) * self.rt.dtype.itemsize + \
             self.rt.token_scratch_bytes(max_tokens, self.hidden) + self.rt.token_scratch_bytes(max_tokens, self.n_q * self.dv) + \
-            (packed.ATTENTION_WORKSPACE if self.rt.cache_bits == 4 else 0)
+            (packed.attention_workspace(self.d) if self.rt.cache_bits == 4 else 0)
 
     def load_transient_bytes(self):
         return self.in_cols * self.hidden * self.rt.dtype.itemsize       # q, k, v beside their stacked copy

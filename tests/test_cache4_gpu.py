@@ -273,6 +273,43 @@ def test_attention_any_size(ops_of, dtype, n_q, n_kv, d, lens, page, window):
     assert ((out - want).abs() <= _bounds(dtype, step, d, n_q, want, top_s, top_v, False)).all()
 
 
+@pytest.mark.parametrize("splits", [1, 2, 5, 64])
+@pytest.mark.parametrize("dtype,n_q,n_kv,d,lens,page,window", ANY + [(FP32, 8, 2, 128, [(1, 3000), (1, 0), (2, 31)], 16, 0),
+                                                                     (BF16, 11, 1, 96, [(1, 700), (3, 90)], 32, 50)])
+def test_attention_any_size_split(ops_of, dtype, n_q, n_kv, d, lens, page, window, splits):
+    ops = ops_of(dtype)
+    ops.force_any4_splits = splits
+    try:
+        step, qkv, pools, out, want, top_s, top_v = _attention_case(ops, dtype, n_q, n_kv, d, lens, page, window, seed=d, stride=3)
+    finally:
+        ops.force_any4_splits = 0
+    # the parts' weights are three roundings more
+    bound = _bounds(dtype, step, d, n_q, want, top_s, top_v, False) + (top_v * 3 * 2.0 ** -23)[..., None]
+    assert ((out - want).abs() <= bound).all()
+
+
+def test_attention_any_size_split_reports_bad_metadata(ops_of):
+    ops = ops_of(FP32)
+    n_q, n_kv, d = 4, 2, 64
+    for spoil, status in (("page", [2, 0, -1, 32]), ("sequence", [5, 0, 9, 0]), ("position", [3, 0, -1, 0])):
+        step, qkv, pools, *_ = _attention_case(ops, FP32, n_q, n_kv, d, [(1, 200), (1, 90)], 16, 0)
+        if spoil == "page":
+            step.table[0, 2] = -1
+        if spoil == "sequence":
+            step.ctx.seq_of_token[0] = 9
+        if spoil == "position":
+            step.ctx.positions[0] = -1
+        out = torch.full((2, n_q * d), 5.0, device=DEV)
+        ops.force_any4_splits = 3
+        try:
+            ops.attention(step.ctx, qkv, out, n_q, n_kv, d, 0.1, None, step.view(*pools))
+        finally:
+            ops.force_any4_splits = 0
+        assert step.ctx.status.tolist() == status
+        if spoil != "page":
+            assert not out[0].any() and out[1].any()
+
+
 DECODE = [
     # n_q, n_kv, d, lens, page, window
     (16, 8, 128, [(1, 511)], 16, 0),
