@@ -227,8 +227,8 @@ class Attention(Mixer):
         attn = rt.buffer("attn_out", n, self.n_q * self.d, rt.dtype)
         # A decode step whose new key goes to this layer's own cache: the attention kernel may norm
         # and rotate q and the new k and write the cache itself.  (A layer that reads another
-        # layer's cache takes every key from there, the newest too, so it is not fused.)
-        fusable = cache.writes and (self.pos is None or (table is not None and rotary_dim == self.d))
+        # layer's cache takes every key from there, the newest too, so it is not fused, nor is one whose pages are in 4 bits.)
+        fusable = cache.writes and getattr(cache, "bits", None) is None and (self.pos is None or (table is not None and rotary_dim == self.d))
         if fusable and hasattr(rt.ops, "can_fuse_decode") and \
                 rt.ops.can_fuse_decode(ctx, qkv, self.n_q, self.n_kv, self.d):
             rt.ops.attention(ctx, qkv, attn, self.n_q, self.n_kv, self.d, self.scale, self.window, cache,

@@ -155,6 +155,38 @@ def test_captured_decode_steps_in_bfloat16_stay_near_eager_ones(folder):
     assert float((logits[0] - logits[1]).norm() / logits[0].norm()) < 0.03
 
 
+@pytest.mark.parametrize("bits", BITS)
+def test_steps_of_a_head_size_that_tuned_kernels_take(tmp_path, bits):
+    """Prompts, a mixed step, decode steps and captured ones of heads of 64 in bfloat16, whose decode steps prepare q and k in the attention
+    kernel where the cache is in the run dtype: against the engine on the 64-bit stand-ins.
+
+    The two differ by bfloat16's roundings, bounded as above, and by the codes that these move.  A rounding moves an element by half a
+    step of 2^-8, and its group's offset and scale by a step, against codes whose step is 1/15 of the group's width (1/254 of the
+    row's with 8 bits, whose scale is not rounded): 2^-9 to 2^-8 of up to 15 steps three times, 0.09 to 0.12 of a step for the largest
+    elements and half of that on average, so about one element in twelve to twenty falls on the next code.  One step in one of twelve
+    elements is in the mean square what rounding to codes makes itself (a step squared over 12): the distance of the options to the run
+    without them, once more."""
+    from leone_b200 import generate
+    from leone_b200.engine.engine import Engine
+    from tests.test_fewer_bits_engine import FewerBitsOps
+    folder = make_folder(tmp_path, "D")
+    prompt = [(11 * i) % 250 for i in range(90)]
+    trace = [[("a", prompt[:60], list(range(60)))], [("b", [prompt[3]], [0]), ("a", prompt[60:70], list(range(10)))]] + \
+        [[("a", [prompt[70 + i]], [0]), ("b", [prompt[i]], [0])] for i in range(4)]
+    got = _engine(folder, "bfloat16", **bits)
+    plain = Engine.from_folder(folder, dtype="float32", device="cpu", ops=FewerBitsOps(), page_tokens=16, num_pages=40, max_requests=4,
+                               max_batch_tokens=128, **bits)
+    without = _engine(folder, "float32")
+    for i, entries in enumerate(trace):
+        want = plain.step(entries).double()
+        away = float((without.step(entries).double().cpu() - want).norm() / want.norm())
+        have = (got.decode_logits([r for r, _, _ in entries], [t[0] for _, t, _ in entries]) if i > 3 else got.step(entries)).double().cpu()
+        assert float((have - want).norm() / want.norm()) < 24 * 2.0 ** -8 + away
+    prompts = [[(7 * i + n) % 250 for i in range(n)] for n in (5, 40, 17)]
+    outs = [generate(_engine(folder, "bfloat16", **bits), prompts, 10, eos_token_id=-1, **kw) for kw in (dict(), dict(decode_quantum=4))]
+    assert outs[0] == outs[1] and [len(t) for t in outs[0]] == [10, 10, 10]
+
+
 def test_a_captured_product_survives_larger_ones():
     """A graph keeps the buffers of codes it was captured with, also when a larger product has outgrown them."""
     ops = _ops(BF16)
