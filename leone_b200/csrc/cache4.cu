@@ -259,8 +259,14 @@ template <typename F> __device__ __forceinline__ void turn_pair(F& x, F& y, floa
   x = u;
 }
 
-template <typename T, typename TW, int D>
-__global__ void __launch_bounds__(32 * kAppendWarps, 5)
+//
+// kFew: the form for up to two blocks an SM.  Its code is one copy for keys and values, and a block first goes through it over what happens
+// to be in shared memory, with results that go nowhere, while the kernel before this one still works: a launch of a step finds the code
+// in no cache, and waited longer for it than it ran.  An 8B layer's products with append and decode attention over 2,048 keys: one token 89.8
+// us, 87.5 with one copy, 85.1 so; 8 tokens 95.6, 92.1, 89.9; 64 tokens (384 blocks) no less.  In a loop of its own, where the code stays, the
+// append of one token takes 3.5 us so and 3.0 in the other form.
+template <typename T, typename TW, int D, bool kFew>
+__global__ void __launch_bounds__(32 * kAppendWarps, kFew ? 4 : 5)
 append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__ q_w, const TW* __restrict__ k_w, float eps,
                   const float2* __restrict__ rope, int max_positions, const int* __restrict__ positions,
                   const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int table_width, int n_seqs,
@@ -269,254 +275,269 @@ append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__
   constexpr int H = D / 32, G = D / 64, kWordLanes = 8 / H;
   constexpr unsigned kAll = 0xffffffffu;
   pdl_trigger();
-  pdl_wait();
   const int t = blockIdx.x, warp = threadIdx.x >> 5, sub = threadIdx.x >> 4 & 1, r = threadIdx.x & 15;
   const int heads = n_q + 2 * n_kv;
   const int h0 = blockIdx.y * per, h1 = min(heads, h0 + per);
   struct __align__(sizeof(T) * H) Part { T e[H]; };        // a lane's elements of half a head
   extern __shared__ __align__(16) uint8_t rows_s[];
   T* tok = qkv + (size_t)t * heads * D;
-  for (int i = threadIdx.x; i < (h1 - h0) * D * (int)sizeof(T) / 16; i += 32 * kAppendWarps) {
-    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(rows_s) + 16 * i;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(reinterpret_cast<const uint4*>(tok + (size_t)h0 * D) + i)
-                 : "memory");
-  }
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  const int pos = positions[t];
-  const bool in_table = rope == nullptr || (pos >= 0 && pos < max_positions), rotate = rope != nullptr && in_table;
-  if (!in_table && threadIdx.x == 0) set_status(status, kBadPosition, t, pos);
-  const float2* turn = rotate ? rope + (size_t)pos * (D / 2) : nullptr;
-  // the lane's pairs: element i of the first half with i of the second, or elements 2 i, 2 i + 1 of the first, then of the second
-  float2 cs[H];
-#pragma unroll
-  for (int i = 0; i < H; ++i) {
-    const int pair = !adjacent ? H * r + i : H / 2 * r + i % (H / 2) + i / (H / 2) * (D / 4);
-    cs[i] = rotate ? turn[pair] : make_float2(1.f, 0.f);
-  }
-  float wa[H], wb[H];
-  auto weights = [&](const TW* from) {
-#pragma unroll
-    for (int i = 0; i < H; ++i) {
-      wa[i] = to_float<TW>(from[H * r + i]);
-      wb[i] = to_float<TW>(from[D / 2 + H * r + i]);
-    }
-  };
-  const Part* rows = reinterpret_cast<const Part*>(rows_s) + r;                 // 32 for every head
-  auto fetch = [&](int at, float (&a)[H], float (&b)[H]) {
-    const Part x = rows[at * 32], y = rows[at * 32 + 16];
-#pragma unroll
-    for (int i = 0; i < H; ++i) {
-      a[i] = to_float<T>(x.e[i]);
-      b[i] = to_float<T>(y.e[i]);
-    }
-  };
-  auto norm = [&](float (&a)[H], float (&b)[H]) {
-    float sa = a[0] * a[0], sb = b[0] * b[0];
-#pragma unroll
-    for (int i = 1; i < H; ++i) {
-      sa = fmaf(a[i], a[i], sa);
-      sb = fmaf(b[i], b[i], sb);
-    }
-    const float f = rsqrtf(half_sum(sa + sb) * (1.f / D) + eps);
-#pragma unroll
-    for (int i = 0; i < H; ++i) {
-      a[i] = a[i] * wa[i] * f;
-      b[i] = b[i] * wb[i] * f;
-    }
-  };
-  auto rotated = [&](auto& a, auto& b) {                   // a pair and its turn: (x, y) (cos, sin)
-    if (adjacent) {
-#pragma unroll
-      for (int i = 0; i < H / 2; ++i) {
-        turn_pair(a[2 * i], a[2 * i + 1], cs[i]);
-        turn_pair(b[2 * i], b[2 * i + 1], cs[H / 2 + i]);
+#pragma unroll 1
+  for (int pass = kFew ? 0 : 1; pass < 2; ++pass) {
+    const bool dry = kFew && pass == 0;
+    if (!dry) {
+      pdl_wait();
+      for (int i = threadIdx.x; i < (h1 - h0) * D * (int)sizeof(T) / 16; i += 32 * kAppendWarps) {
+        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(rows_s) + 16 * i;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(reinterpret_cast<const uint4*>(tok + (size_t)h0 * D) + i)
+                     : "memory");
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < H; ++i) turn_pair(a[i], b[i], cs[i]);
+      asm volatile("cp.async.commit_group;" ::: "memory");
     }
-  };
-  const int n_queries = max(0, min(h1, n_q) - h0), n_keys = max(0, min(h1, n_q + n_kv) - max(h0, n_q));
-  const int n_values = h1 - h0 - n_queries - n_keys;
-  int p = warp;                                            // two heads of one kind; the kinds' follow one another
-  if (p < (n_queries + 1) / 2 && q_w != nullptr) weights(q_w);
-  Place place;
-  const bool placed = h1 <= n_q || find_place(place, t, pos, seq_of_token, n_seqs, block_table, table_width, num_pages, page_tokens,
-                                              status, threadIdx.x == 0);
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
-  for (; p < (n_queries + 1) / 2; p += kAppendWarps) {
-    const bool real = 2 * p + sub < n_queries;
-    const int at = real ? 2 * p + sub : 2 * p;
-    float a[H], b[H];
-    fetch(at, a, b);
-    if (q_w != nullptr) norm(a, b);
-    if (rotate) rotated(a, b);
-    Part x, y;
+    const int pos = dry ? 0 : positions[t];
+    const bool in_table = rope == nullptr || dry || (pos >= 0 && pos < max_positions), rotate = rope != nullptr && in_table;
+    if (!in_table && threadIdx.x == 0) set_status(status, kBadPosition, t, pos);
+    const float2* turn = rotate ? rope + (size_t)pos * (D / 2) : nullptr;
+    // the lane's pairs: element i of the first half with i of the second, or elements 2 i, 2 i + 1 of the first, then of the second
+    float2 cs[H];
 #pragma unroll
     for (int i = 0; i < H; ++i) {
-      x.e[i] = from_float<T>(a[i]);
-      y.e[i] = from_float<T>(b[i]);
+      const int pair = !adjacent ? H * r + i : H / 2 * r + i % (H / 2) + i / (H / 2) * (D / 4);
+      cs[i] = rotate && !dry ? turn[pair] : make_float2(1.f, 0.f);
     }
-    if (real && in_table) {
-      Part* to = reinterpret_cast<Part*>(tok + (size_t)(h0 + at) * D) + r;
-      to[0] = x;
-      to[16] = y;
-    }
-  }
-  p -= (n_queries + 1) / 2;
-  if (!placed) return;
-  const long long unit = unit_at(place.page, n_kv, 0, page_tokens, place.slot / kUnit * kUnit, D);
-  const int slot = place.slot % kUnit, head_bytes = page_tokens * row_bytes(D);
-  // of the lanes that share a word of the first half and one of the second, the first stores the one and the last the other
-  const int w_at = r / kWordLanes + (r % kWordLanes == kWordLanes - 1 ? D / 16 : 0);
-  const bool stores = r % kWordLanes == 0 || r % kWordLanes == kWordLanes - 1;
-  auto store = [&](bool is_k, int first, int count) {      // heads first .. first + count - 1 of the block's
-    const bool computed = is_k && (k_w != nullptr || rotate);
-    const int word_at = is_k ? key_word_at(slot, w_at, D) : value_word_at(slot, w_at, D);
-    for (; p < (count + 1) / 2; p += kAppendWarps) {
-      const bool real = 2 * p + sub < count;
-      const int at = first + (real ? 2 * p + sub : 2 * p);
-      float a[H], b[H];
-      double da[H], db[H];                                 // of keys
-      bool doubt = false;
-      fetch(at, a, b);
-      if (computed) {
-#pragma unroll
-        for (int i = 0; i < H; ++i) {
-          da[i] = a[i];
-          db[i] = b[i];
-        }
-        if (k_w != nullptr) {
-          double ss = 0.0;
-#pragma unroll
-          for (int i = 0; i < H; ++i) ss = fma(da[i], da[i], fma(db[i], db[i], ss));
-#pragma unroll
-          for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(kAll, ss, o);
-          ss = ss * (1.0 / D) + (double)eps;
-          doubt |= !(ss > 1e-37 && ss < 1e37);
-          double f = rsqrtf((float)ss);                    // two steps of Newton's take it to 64 bits
-          f *= fma(-0.5 * ss * f, f, 1.5);
-          f *= fma(-0.5 * ss * f, f, 1.5);
-#pragma unroll
-          for (int i = 0; i < H; ++i) {
-            da[i] *= (double)wa[i] * f;
-            db[i] *= (double)wb[i] * f;
-          }
-        }
-        if (rotate) rotated(da, db);
-#pragma unroll
-        for (int i = 0; i < H; ++i) {
-          a[i] = (float)da[i];
-          b[i] = (float)db[i];
-        }
-      }
-      float lo[2], hi[2];                                  // of the halves
-      lo[0] = hi[0] = a[0];
-      lo[1] = hi[1] = b[0];
+    float wa[H], wb[H];
+    auto weights = [&](const TW* from) {
 #pragma unroll
       for (int i = 0; i < H; ++i) {
-        doubt |= !(fabsf(a[i]) < INFINITY) || !(fabsf(b[i]) < INFINITY);
-        lo[0] = fminf(lo[0], a[i]);
-        hi[0] = fmaxf(hi[0], a[i]);
-        lo[1] = fminf(lo[1], b[i]);
-        hi[1] = fmaxf(hi[1], b[i]);
+        wa[i] = dry ? 1.f : to_float<TW>(from[H * r + i]);
+        wb[i] = dry ? 1.f : to_float<TW>(from[D / 2 + H * r + i]);
       }
-      if (G == 1) {
-        lo[0] = fminf(lo[0], lo[1]);
-        hi[0] = fmaxf(hi[0], hi[1]);
-      }
-      float z[2], s[2], inv[2], limit[2];
+    };
+    const Part* rows = reinterpret_cast<const Part*>(rows_s) + r;                 // 32 for every head
+    auto fetch = [&](int at, float (&a)[H], float (&b)[H]) {
+      const Part x = rows[at * 32], y = rows[at * 32 + 16];
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        lo[g] = half_min(lo[g]);
-        hi[g] = half_max(hi[g]);
-        const float err = computed ? fmaxf(fabsf(lo[g]), fabsf(hi[g])) * kRounded : 0.f;
-        z[g] = eight_bits_down(__fsub_rd(lo[g], err));
-        doubt |= z[g] != eight_bits_down(__fadd_ru(lo[g], err));
-        // s is the smallest with 15 s >= hi - z; 15 s has 12 bits.  Of a value the rounded difference is on the side of 15 s that the
-        // difference is on, or meets it; of a key it is off by the maximum's rounding and its own (and the margin's).
-        const float range = hi[g] - z[g], margin = err + 2.f * kRounded * range;
-        s[g] = eight_bits_up(range * (1.f / 15.f) * (1.f - 6e-7f));         // or the next
-        if (15.f * s[g] < range) s[g] = __uint_as_float(__float_as_uint(s[g]) + 0x10000u);
-        if (err != 0.f) {
-          const float below = __uint_as_float(__float_as_uint(s[g]) - 0x10000u);
-          doubt |= !(range - margin > 15.f * below && range + margin < 15.f * s[g]);
-        } else if (range == 15.f * s[g]) {
-          const float back = hi[g] - range;
-          doubt |= (hi[g] - (range + back)) + (back - z[g]) != 0.f;
+      for (int i = 0; i < H; ++i) {
+        a[i] = to_float<T>(x.e[i]);
+        b[i] = to_float<T>(y.e[i]);
+      }
+    };
+    auto norm = [&](float (&a)[H], float (&b)[H]) {
+      float sa = a[0] * a[0], sb = b[0] * b[0];
+#pragma unroll
+      for (int i = 1; i < H; ++i) {
+        sa = fmaf(a[i], a[i], sa);
+        sb = fmaf(b[i], b[i], sb);
+      }
+      const float f = rsqrtf(half_sum(sa + sb) * (1.f / D) + eps);
+#pragma unroll
+      for (int i = 0; i < H; ++i) {
+        a[i] = a[i] * wa[i] * f;
+        b[i] = b[i] * wb[i] * f;
+      }
+    };
+    auto rotated = [&](auto& a, auto& b) {                   // a pair and its turn: (x, y) (cos, sin)
+      if (adjacent) {
+#pragma unroll
+        for (int i = 0; i < H / 2; ++i) {
+          turn_pair(a[2 * i], a[2 * i + 1], cs[i]);
+          turn_pair(b[2 * i], b[2 * i + 1], cs[H / 2 + i]);
         }
-        doubt |= (s[g] != 0.f && !(s[g] > 1e-37f && s[g] < 1e37f)) || !(fabsf(z[g]) < 3e38f);
-        inv[g] = s[g] > 0.f ? reciprocal(s[g]) : 0.f;
-        limit[g] = 0.5f - fmaf(err, inv[g] * 1.01f, 15.5f * 2.5e-7f);
-      }
-      if (G == 1) {
-        z[1] = z[0];
-        s[1] = s[0];
-        inv[1] = inv[0];
-        limit[1] = limit[0];
-      }
-      float code[2][H];                                    // + kToInteger
-      bool near = false;
+      } else {
 #pragma unroll
-      for (int i = 0; i < H; ++i)
+        for (int i = 0; i < H; ++i) turn_pair(a[i], b[i], cs[i]);
+      }
+    };
+    const int n_queries = max(0, min(h1, n_q) - h0), n_keys = max(0, min(h1, n_q + n_kv) - max(h0, n_q));
+    const int n_values = h1 - h0 - n_queries - n_keys;
+    int p = warp;                                            // two heads of one kind; the kinds' follow one another
+    if (p < (n_queries + 1) / 2 && q_w != nullptr) weights(q_w);
+    Place place{0, 0};
+    const bool placed = h1 <= n_q || dry ||
+                        find_place(place, t, pos, seq_of_token, n_seqs, block_table, table_width, num_pages, page_tokens,
+                                                status, threadIdx.x == 0);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    for (; p < (n_queries + 1) / 2; p += kAppendWarps) {
+      const bool real = 2 * p + sub < n_queries;
+      const int at = real ? 2 * p + sub : 2 * p;
+      float a[H], b[H];
+      fetch(at, a, b);
+      if (q_w != nullptr) norm(a, b);
+      if (rotate) rotated(a, b);
+      Part x, y;
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float gap = (g ? b[i] : a[i]) - z[g], c = fmaf(gap, inv[g], kToInteger);
-          near |= fabsf(fmaf(gap, inv[g], kToInteger - c)) >= limit[g];
-          code[g][i] = c;
+      for (int i = 0; i < H; ++i) {
+        x.e[i] = from_float<T>(a[i]);
+        y.e[i] = from_float<T>(b[i]);
+      }
+      if (real && in_table && !dry) {
+        Part* to = reinterpret_cast<Part*>(tok + (size_t)(h0 + at) * D) + r;
+        to[0] = x;
+        to[16] = y;
+      }
+    }
+    p -= (n_queries + 1) / 2;
+    if (!placed) return;                                     // (in the pass that counts)
+    const long long unit = unit_at(place.page, n_kv, 0, page_tokens, place.slot / kUnit * kUnit, D);
+    const int slot = place.slot % kUnit, head_bytes = page_tokens * row_bytes(D);
+    // of the lanes that share a word of the first half and one of the second, the first stores the one and the last the other
+    const int w_at = r / kWordLanes + (r % kWordLanes == kWordLanes - 1 ? D / 16 : 0);
+    const bool stores = r % kWordLanes == 0 || r % kWordLanes == kWordLanes - 1;
+    auto store = [&](bool is_k, int first, int count) {      // heads first .. first + count - 1 of the block's
+      const bool computed = is_k && (k_w != nullptr || rotate);
+      const int word_at = is_k ? key_word_at(slot, w_at, D) : value_word_at(slot, w_at, D);
+      for (; p < (count + 1) / 2; p += kAppendWarps) {
+        const bool real = 2 * p + sub < count;
+        const int at = first + (real ? 2 * p + sub : 2 * p);
+        float a[H], b[H];
+        double da[H], db[H];                                 // of keys
+        bool doubt = false;
+        fetch(at, a, b);
+        if (computed) {
+#pragma unroll
+          for (int i = 0; i < H; ++i) {
+            da[i] = a[i];
+            db[i] = b[i];
+          }
+          if (k_w != nullptr) {
+            double ss = 0.0;
+#pragma unroll
+            for (int i = 0; i < H; ++i) ss = fma(da[i], da[i], fma(db[i], db[i], ss));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(kAll, ss, o);
+            ss = ss * (1.0 / D) + (double)eps;
+            doubt |= !(ss > 1e-37 && ss < 1e37);
+            double f = rsqrtf((float)ss);                    // two steps of Newton's take it to 64 bits
+            f *= fma(-0.5 * ss * f, f, 1.5);
+            f *= fma(-0.5 * ss * f, f, 1.5);
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+              da[i] *= (double)wa[i] * f;
+              db[i] *= (double)wb[i] * f;
+            }
+          }
+          if (rotate) rotated(da, db);
+#pragma unroll
+          for (int i = 0; i < H; ++i) {
+            a[i] = (float)da[i];
+            b[i] = (float)db[i];
+          }
         }
-      if (near) {
+        float lo[2], hi[2];                                  // of the halves
+        lo[0] = hi[0] = a[0];
+        lo[1] = hi[1] = b[0];
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+          doubt |= !(fabsf(a[i]) < INFINITY) || !(fabsf(b[i]) < INFINITY);
+          lo[0] = fminf(lo[0], a[i]);
+          hi[0] = fmaxf(hi[0], a[i]);
+          lo[1] = fminf(lo[1], b[i]);
+          hi[1] = fmaxf(hi[1], b[i]);
+        }
+        if (G == 1) {
+          lo[0] = fminf(lo[0], lo[1]);
+          hi[0] = fmaxf(hi[0], hi[1]);
+        }
+        float z[2], s[2], inv[2], limit[2];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          lo[g] = half_min(lo[g]);
+          hi[g] = half_max(hi[g]);
+          const float err = computed ? fmaxf(fabsf(lo[g]), fabsf(hi[g])) * kRounded : 0.f;
+          z[g] = eight_bits_down(__fsub_rd(lo[g], err));
+          doubt |= z[g] != eight_bits_down(__fadd_ru(lo[g], err));
+          // s is the smallest with 15 s >= hi - z; 15 s has 12 bits.  Of a value the rounded difference is on the side of 15 s that the
+          // difference is on, or meets it; of a key it is off by the maximum's rounding and its own (and the margin's).
+          const float range = hi[g] - z[g], margin = err + 2.f * kRounded * range;
+          s[g] = eight_bits_up(range * (1.f / 15.f) * (1.f - 6e-7f));         // or the next
+          if (15.f * s[g] < range) s[g] = __uint_as_float(__float_as_uint(s[g]) + 0x10000u);
+          if (err != 0.f) {
+            const float below = __uint_as_float(__float_as_uint(s[g]) - 0x10000u);
+            doubt |= !(range - margin > 15.f * below && range + margin < 15.f * s[g]);
+          } else if (range == 15.f * s[g]) {
+            const float back = hi[g] - range;
+            doubt |= (hi[g] - (range + back)) + (back - z[g]) != 0.f;
+          }
+          doubt |= (s[g] != 0.f && !(s[g] > 1e-37f && s[g] < 1e37f)) || !(fabsf(z[g]) < 3e38f);
+          inv[g] = s[g] > 0.f ? reciprocal(s[g]) : 0.f;
+          limit[g] = 0.5f - fmaf(err, inv[g] * 1.01f, 15.5f * 2.5e-7f);
+        }
+        if (G == 1) {
+          z[1] = z[0];
+          s[1] = s[0];
+          inv[1] = inv[0];
+          limit[1] = limit[0];
+        }
+        float code[2][H];                                    // + kToInteger
+        bool near = false;
 #pragma unroll
         for (int i = 0; i < H; ++i)
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
-            const float x = g ? b[i] : a[i], q = (x - z[g]) * inv[g], low = floorf(q);
-            if (fabsf(fabsf(q - low) - 0.5f) > 1e-3f) continue;
-            const double gap = (computed ? (g ? db[i] : da[i]) : (double)x) - (double)z[g];
-            const double side = fma(-(double)(low + 0.5f), (double)s[g], gap);
-            code[g][i] = (side > 0.0 || (side == 0.0 && ((int)low & 1)) ? low + 1.f : low) + kToInteger;
+            const float gap = (g ? b[i] : a[i]) - z[g], c = fmaf(gap, inv[g], kToInteger);
+            near |= fabsf(fmaf(gap, inv[g], kToInteger - c)) >= limit[g];
+            code[g][i] = c;
           }
-      }
-      // the word's lanes put their nibbles together (element 2 j in nibble j, 2 j + 1 in nibble j + 4)
-      uint32_t word[2];
+        if (near) {
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        word[g] = 0;
+          for (int i = 0; i < H; ++i)
 #pragma unroll
-        for (int i = 0; i < H; ++i) word[g] += (__float_as_uint(code[g][i]) - __float_as_uint(kToInteger)) << (4 * (i >> 1) + 16 * (i & 1));
-        word[g] <<= 4 * (H / 2) * (r % kWordLanes);
-      }
+            for (int g = 0; g < 2; ++g) {
+              const float x = g ? b[i] : a[i], q = (x - z[g]) * inv[g], low = floorf(q);
+              if (fabsf(fabsf(q - low) - 0.5f) > 1e-3f) continue;
+              const double gap = (computed ? (g ? db[i] : da[i]) : (double)x) - (double)z[g];
+              const double side = fma(-(double)(low + 0.5f), (double)s[g], gap);
+              code[g][i] = (side > 0.0 || (side == 0.0 && ((int)low & 1)) ? low + 1.f : low) + kToInteger;
+            }
+        }
+        // the word's lanes put their nibbles together (element 2 j in nibble j, 2 j + 1 in nibble j + 4)
+        uint32_t word[2];
 #pragma unroll
-      for (int o = kWordLanes / 2; o > 1; o >>= 1) {
-        word[0] |= __shfl_xor_sync(kAll, word[0], o);
-        word[1] |= __shfl_xor_sync(kAll, word[1], o);
+        for (int g = 0; g < 2; ++g) {
+          word[g] = 0;
+#pragma unroll
+          for (int i = 0; i < H; ++i)
+            word[g] += (__float_as_uint(code[g][i]) - __float_as_uint(kToInteger)) << (4 * (i >> 1) + 16 * (i & 1));
+          word[g] <<= 4 * (H / 2) * (r % kWordLanes);
+        }
+#pragma unroll
+        for (int o = kWordLanes / 2; o > 1; o >>= 1) {
+          word[0] |= __shfl_xor_sync(kAll, word[0], o);
+          word[1] |= __shfl_xor_sync(kAll, word[1], o);
+        }
+        const uint32_t other = __shfl_xor_sync(kAll, r & 1 ? word[0] : word[1], 1), whole = (r & 1 ? word[1] : word[0]) | other;
+        const unsigned again = __ballot_sync(kAll, doubt);
+        uint8_t* pool = is_k ? k_pool + (size_t)(h0 + at - n_q) * head_bytes : v_pool + (size_t)(h0 + at - n_q - n_kv) * head_bytes;
+        if (again == 0 || dry) {
+          if (real && stores && !dry) *reinterpret_cast<uint32_t*>(pool + unit + word_at) = whole;
+          if (real && r < G && !dry)
+            *reinterpret_cast<uint32_t*>(pool + unit + scale_at(slot, r, D)) =
+                __float_as_uint(r ? s[1] : s[0]) >> 16 | (__float_as_uint(r ? z[1] : z[0]) & 0xffff0000u);
+          continue;
+        }
+        for (int u = 0; u < 2 && 2 * p + u < count; ++u) {
+          const int h = first + 2 * p + u;
+          append_exact<T, TW, D>(reinterpret_cast<const T*>(rows_s) + (size_t)h * D, is_k ? k_w : (const TW*)nullptr, eps,
+                                 is_k ? turn : nullptr, adjacent != 0, is_k, slot,
+                                 (is_k ? k_pool + (size_t)(h0 + h - n_q) * head_bytes
+                                       : v_pool + (size_t)(h0 + h - n_q - n_kv) * head_bytes) + unit);
+        }
       }
-      const uint32_t other = __shfl_xor_sync(kAll, r & 1 ? word[0] : word[1], 1), whole = (r & 1 ? word[1] : word[0]) | other;
-      const unsigned again = __ballot_sync(kAll, doubt);
-      uint8_t* pool = is_k ? k_pool + (size_t)(h0 + at - n_q) * head_bytes : v_pool + (size_t)(h0 + at - n_q - n_kv) * head_bytes;
-      if (again == 0) {
-        if (real && stores) *reinterpret_cast<uint32_t*>(pool + unit + word_at) = whole;
-        if (real && r < G)
-          *reinterpret_cast<uint32_t*>(pool + unit + scale_at(slot, r, D)) =
-              __float_as_uint(r ? s[1] : s[0]) >> 16 | (__float_as_uint(r ? z[1] : z[0]) & 0xffff0000u);
-        continue;
+      p -= (count + 1) / 2;
+    };
+    if (in_table && k_w != nullptr && p < (n_keys + 1) / 2) weights(k_w);
+    if constexpr (kFew) {
+#pragma unroll 1
+      for (int kind = 0; kind < 2; ++kind) {
+        if (kind == 0 && !in_table) p -= (n_keys + 1) / 2;
+        else store(kind == 0, kind == 0 ? n_queries : n_queries + n_keys, kind == 0 ? n_keys : n_values);
       }
-      for (int u = 0; u < 2 && 2 * p + u < count; ++u) {
-        const int h = first + 2 * p + u;
-        append_exact<T, TW, D>(reinterpret_cast<const T*>(rows_s) + (size_t)h * D, is_k ? k_w : (const TW*)nullptr, eps,
-                               is_k ? turn : nullptr, adjacent != 0, is_k, slot,
-                               (is_k ? k_pool + (size_t)(h0 + h - n_q) * head_bytes
-                                     : v_pool + (size_t)(h0 + h - n_q - n_kv) * head_bytes) + unit);
-      }
+    } else {
+      if (in_table) store(true, n_queries, n_keys);
+      else p -= (n_keys + 1) / 2;
+      store(false, n_queries + n_keys, n_values);
     }
-    p -= (count + 1) / 2;
-  };
-  if (in_table) {
-    if (k_w != nullptr && p < (n_keys + 1) / 2) weights(k_w);
-    store(true, n_queries, n_keys);
-  } else p -= (n_keys + 1) / 2;
-  store(false, n_queries + n_keys, n_values);
+  }
 }
 
 // What the pages hold for the step's tokens: rows [n_tokens][n_kv * d] of keys and of values.  grid = (tokens, blocks of heads); a warp takes
@@ -786,12 +807,13 @@ extern "C" int leone_append4(int dtype, void* qkv, int n_tokens, int n_q, int n_
     const int heads = n_q + 2 * n_kv, most = n_tokens <= 200 ? 2 * cache4::kAppendWarps : cache4::kAppendHeads;
     const int blocks_of = (heads + most - 1) / most, per = (heads + blocks_of - 1) / blocks_of;
     const dim3 grid(n_tokens, blocks_of);
+    const bool few = (long long)n_tokens * blocks_of <= 2 * 148;
     const size_t row_bytes = (size_t)per * d * (dtype == 0 ? 4 : 2);
-#define LAUNCH_VEC(T, TW, D)                                                                                                     \
-  return launch_kernel(cache4::append_vec_kernel<T, TW, D>, grid, dim3(32 * cache4::kAppendWarps), row_bytes, stream, (T*)qkv, n_q, n_kv, \
-                       (const TW*)q_w, (const TW*)k_w, eps, (const float2*)rope, max_positions, positions, seq_of_token,          \
-                       block_table, table_width, n_seqs, (uint8_t*)k_pool, (uint8_t*)v_pool, num_pages, page_tokens, adjacent, per, \
-                       status)
+#define LAUNCH_VEC(T, TW, D)                                                                                                        \
+  return launch_kernel(few ? cache4::append_vec_kernel<T, TW, D, true> : cache4::append_vec_kernel<T, TW, D, false>, grid,           \
+                       dim3(32 * cache4::kAppendWarps), row_bytes, stream, (T*)qkv, n_q, n_kv, (const TW*)q_w, (const TW*)k_w, eps, \
+                       (const float2*)rope, max_positions, positions, seq_of_token, block_table, table_width, n_seqs,               \
+                       (uint8_t*)k_pool, (uint8_t*)v_pool, num_pages, page_tokens, adjacent, per, status)
     if (d == 64) {
       if (dtype == 0 && w_dtype == 0) LAUNCH_VEC(float, float, 64);
       if (dtype == 1 && w_dtype == 0) LAUNCH_VEC(__nv_bfloat16, float, 64);
