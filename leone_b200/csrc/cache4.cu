@@ -387,6 +387,7 @@ append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__
       const bool computed = is_k && (k_w != nullptr || rotate);
       const int word_at = is_k ? key_word_at(slot, w_at, D) : value_word_at(slot, w_at, D);
       for (; p < (count + 1) / 2; p += kAppendWarps) {
+        if (is_k && !in_table) continue;                     // (their position is reported; values need none)
         const bool real = 2 * p + sub < count;
         const int at = first + (real ? 2 * p + sub : 2 * p);
         float a[H], b[H];
@@ -529,12 +530,10 @@ append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__
     if constexpr (kFew) {
 #pragma unroll 1
       for (int kind = 0; kind < 2; ++kind) {
-        if (kind == 0 && !in_table) p -= (n_keys + 1) / 2;
-        else store(kind == 0, kind == 0 ? n_queries : n_queries + n_keys, kind == 0 ? n_keys : n_values);
+        store(kind == 0, kind == 0 ? n_queries : n_queries + n_keys, kind == 0 ? n_keys : n_values);
       }
     } else {
-      if (in_table) store(true, n_queries, n_keys);
-      else p -= (n_keys + 1) / 2;
+      store(true, n_queries, n_keys);
       store(false, n_queries + n_keys, n_values);
     }
   }

@@ -1,0 +1,75 @@
+"""Pages in 4 bits: what the kernels do at the edges of what they take, against plain 64-bit forms."""
+import pytest
+import torch
+
+from leone_b200.cache import packed
+from leone_b200.parts.rotary import build_rotary_table
+from tests.fewer_bits import Step, quantize4
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+BF16, FP32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def ops_of():
+    from leone_b200.ops.cuda import CudaOps
+    made = {}
+
+    def get(dtype):
+        if dtype not in made:
+            made[dtype] = CudaOps(DEV, dtype)
+            made[dtype].bind_status(torch.zeros(4, dtype=torch.int32, device=DEV))
+        return made[dtype]
+    return get
+
+
+def _gen(seed):
+    return torch.Generator(DEV).manual_seed(seed)
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("dtype,d,n_q,n_kv,new", [
+    (BF16, 128, 16, 8, 5),         # few tokens: blocks of 8 heads
+    (FP32, 64, 2, 3, 7),           # an odd number of cached heads, a block of all kinds
+    (BF16, 128, 32, 8, 700),       # many tokens: a block of all of a token's heads
+    (FP32, 128, 1, 1, 900),
+    (BF16, 64, 40, 20, 600),       # two blocks a token, the second of keys and values
+    (BF16, 96, 4, 2, 9),           # the form of any size
+])
+def test_append_behind_the_rotation_table(ops_of, dtype, d, n_q, n_kv, new, norm):
+    """Tokens whose position the rotation table does not reach, on pages that they have: the status says so, their queries and keys
+    stay as they were, their values are written, and nothing beside them."""
+    ops = ops_of(dtype)
+    past, reach = 30, 30 + new // 2                          # half of the tokens lie behind the table
+    step = Step([(new, past)], 16, DEV, seed=d)
+    rows = torch.randn((new, (n_q + 2 * n_kv) * d), generator=_gen(d + new), device=DEV).to(dtype)
+    weights = (1 + 0.1 * torch.randn((2, d), generator=_gen(2), device=DEV)) if norm else (None, None)
+    guard = 3                                                # pages in front of the pools and behind them
+    whole = [torch.full((step.pages + 2 * guard, n_kv, 16, packed.row_bytes(d)), 0xA5, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    pools = [w[guard:guard + step.pages] for w in whole]
+    table = build_rotary_table(reach, d, 10000.0).to(DEV)
+    got, full = rows.clone(), rows.clone()
+    ops.qk_norm_rope_write(step.ctx, got, n_q, n_kv, d, *weights, 1e-6, table, d, step.view(*pools))
+    assert step.ctx.status[0] == 3 and int(step.ctx.status[1]) >= new // 2
+    step.ctx.status.zero_()
+    want = [torch.full_like(w, 0xA5) for w in whole]
+    longer = build_rotary_table(past + new, d, 10000.0).to(DEV)
+    ops.qk_norm_rope_write(step.ctx, full, n_q, n_kv, d, *weights, 1e-6, longer, d, step.view(*(w[guard:guard + step.pages] for w in want)))
+    assert step.ctx.status[0] == 0
+    inside = step.pos < reach
+    assert torch.equal(got[inside], full[inside]) and torch.equal(got[~inside], rows[~inside])
+    for have, w, values in zip(whole, want, (False, True)):
+        assert (have[:guard] == 0xA5).all() and (have[-guard:] == 0xA5).all()
+        fill = packed.unpack_pages(torch.full_like(pools[0], 0xA5), d, values)
+        for a, b, untouched in zip(*(packed.unpack_pages(t[guard:guard + step.pages], d, values) for t in (have, w)), fill):
+            a, b, untouched = a.float(), b.float(), untouched.float()
+            if not values:
+                b[step.page[~inside], :, step.slot[~inside]] = untouched[step.page[~inside], :, step.slot[~inside]]
+            assert torch.equal(a, b)
+    # and they are the right ones
+    v = rows.double().unflatten(1, (n_q + 2 * n_kv, d))[:, n_q + n_kv:]
+    codes, s, z = (t[step.page, :, step.slot] for t in packed.unpack_pages(pools[1], d, True))
+    for a, b in zip((codes.long(), s.double(), z.double()), quantize4(v)):
+        assert torch.equal(a, b)
