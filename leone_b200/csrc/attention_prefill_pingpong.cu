@@ -214,14 +214,17 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 // are stored times 2^-64 (for s 2^133; scales up to 2^57 fit), which the outputs are multiplied with at the end.
 //
 // A value that is NaN must not reach rows that do not see its key (the product has 0 x NaN for them): such a group is stored as zeros
-// and kept in a list of keys and groups, and at the end the rows that see one of them become NaN in that group's columns.  What does not
-// fit into the list widens a range of keys, which counts as a whole.
+// and kept in a list of keys and groups, and at the end the rows that see one of them become NaN in that group's columns.  Of what does not
+// fit into the list the first and the last key are kept: a row that sees either is sure, one whose window lies between them looks its own
+// keys' scales up in the pages.  The first query tile may end while the gathering warps are at tiles that only the second reads; what they add
+// then lies behind all its rows, and a place of the list that is counted but not yet written holds kNoKey, behind every row.
 constexpr int kTileUnits = kKeys / cache4::kUnit;
 constexpr int kOddKeys = 32;
+constexpr int kNoKey = 0x7fffffff;
 struct OddValues {
   int count;
   int key[kOddKeys];              // key * 2 + group
-  int lo[2], hi[2];               // the range of further keys, per group
+  int lo[2], hi[2];               // the first and the last of further keys, per group
   unsigned units[2];              // of the tile that lands, keys and values: the units that have a page
   int largest[2][4];              // of the four warps that gather keys: the largest exponent of their rows of tile t % 2
   float key_power[4];             // 2^e of tile t % 4: its keys are stored times 2^-e
@@ -240,6 +243,27 @@ template <int D, bool kPacked> constexpr int smem_bytes() {
   // two Q tiles, two K and two V tiles, row sources [2 kinds][2 buffers][128], barriers; 1024 for alignment
   return 2 * kRows * D * 2 + 4 * kKeys * D * 2 + 2 * 2 * kKeys * 8 + 18 * 8 + 1024 +
          (kPacked ? 2 * kKeys * cache4::row_bytes(D) : 0);
+}
+
+// Whether a group of a value is no bfloat16 number times 2^-64: its scale and offset are NaN, z + 15 s, the largest, is none, or s is
+// past 2^57.
+__device__ __forceinline__ bool odd_value(uint32_t sz) {
+  const float s = cache4::scale_of(sz);
+  return !(fabsf(fmaf(15.f, s, cache4::offset_of(sz))) <= 3.3895e38f && s <= 144115188075855872.f);
+}
+// Whether group g of one of the values from .. to is odd_value; `table`: the sequence's row of the block table.
+template <int D>
+__device__ __noinline__ bool any_odd_value(const PagedArgs& pa, const int* table, int kvh, int g, int from, int to) {
+  const uint8_t* pool = reinterpret_cast<const uint8_t*>(pa.v_pool);
+  for (int key = from; key <= to; ++key) {
+    const int blk = key / pa.page_tokens;
+    const int page = blk < pa.table_width ? table[blk] : -1;
+    if (page < 0 || page >= pa.num_pages) continue;
+    const int slot = key - blk * pa.page_tokens, at = slot % cache4::kUnit;
+    const uint8_t* unit = pool + cache4::unit_at(page, pa.n_kv, kvh, pa.page_tokens, slot - at, D);
+    if (odd_value(*reinterpret_cast<const uint32_t*>(unit + cache4::scale_at(at, g, D)))) return true;
+  }
+  return false;
 }
 
 // 2^e for e in -126 .. 127.
@@ -328,6 +352,7 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
     }
     if constexpr (kPacked) {
       odd.count = 0;
+      for (int i = 0; i < kOddKeys; ++i) odd.key[i] = kNoKey;
       odd.lo[0] = odd.lo[1] = 0x7fffffff;
       odd.hi[0] = odd.hi[1] = -1;
     }
@@ -502,13 +527,11 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
           }
         }
         if (values) {
-          // (z + 15 s is the largest value; what would not be a bfloat16 number, or a scale too large, counts with the NaN)
 #pragma unroll
           for (int i = 0; i < kMine; ++i)
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-              const float s = cache4::scale_of(sz[i][g]);
-              if (fabsf(fmaf(15.f, s, cache4::offset_of(sz[i][g]))) <= 3.3895e38f && s <= 144115188075855872.f) continue;      // 2^57
+              if (!odd_value(sz[i][g])) continue;
               sz[i][g] = 0;
               if (q != 0) continue;
               const int key = key0 + row0 + i * kStep, at = atomicAdd(&odd.count, 1);
@@ -875,11 +898,14 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
           const int count = odd.count;                     // (almost always 0)
           if (count > 0 && my_pos >= 0) {
             const int g = D == 64 ? 0 : half, from = window > 0 ? max(0, my_pos - window + 1) : 0;
-            bool sees = from <= odd.hi[g] && my_pos >= odd.lo[g];
-            for (int i = 0; i < min(count, kOddKeys); ++i) {
-              const int key = odd.key[i] >> 1;
-              sees |= (odd.key[i] & 1) == g && key <= my_pos && key >= from;
+            const int first_odd = odd.lo[g], last_odd = odd.hi[g];
+            bool sees = (from <= first_odd && first_odd <= my_pos) || (from <= last_odd && last_odd <= my_pos);
+            for (int i = 0; i < kOddKeys; ++i) {
+              const int listed = odd.key[i], key = listed >> 1;
+              sees |= listed != kNoKey && (listed & 1) == g && key <= my_pos && key >= from;
             }
+            if (!sees && first_odd < from && last_odd > my_pos)
+              sees = any_odd_value<D>(pa, pa.block_table + (size_t)seq * pa.table_width, kvh, g, max(from, k_lo), min(my_pos, k_hi - 1));
             if (sees) inv = NAN;
           }
           if (parts.part_o != nullptr) {                   // this split's part, as it is

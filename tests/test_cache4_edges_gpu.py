@@ -73,3 +73,58 @@ def test_append_behind_the_rotation_table(ops_of, dtype, d, n_q, n_kv, new, norm
     codes, s, z = (t[step.page, :, step.slot] for t in packed.unpack_pages(pools[1], d, True))
     for a, b in zip((codes.long(), s.double(), z.double()), quantize4(v)):
         assert torch.equal(a, b)
+
+
+def _nan_pattern(ops, n_q, n_kv, d, lens, window, bad, runs=1, splits=0):
+    """Prompt attention over pages whose last cached head has NaN in the last group of the values `bad` [(sequence, key)]: the outputs'
+    NaN, and which of them there have to be, ``[tokens, n_q, d]``."""
+    step = Step(lens, 16, DEV, window=window)
+    pools = []
+    for values in (False, True):
+        codes, s, z = quantize4(torch.randn((step.pages, n_kv, 16, d), generator=_gen(7 + values), device=DEV).double())
+        for seq, key in bad if values else ():
+            page = int(step.table[seq, key // 16])
+            if page >= 0:
+                s[page, -1, key % 16, -1] = z[page, -1, key % 16, -1] = float("nan")
+        pools.append(packed.pack_pages(codes, s, z, values))
+    n = step.ctx.n_tokens
+    qkv = torch.randn((n, (n_q + 2 * n_kv) * d), generator=_gen(9), device=DEV).to(BF16)
+    got = []
+    ops.force_prompt4_splits = splits
+    try:
+        for _ in range(runs):
+            out = torch.zeros((n, n_q * d), dtype=BF16, device=DEV)
+            ops.attention(step.ctx, qkv, out, n_q, n_kv, d, d ** -0.5, window or None, step.view(*pools))
+            got.append(out.view(n, n_q, d).isnan())
+    finally:
+        ops.force_prompt4_splits = 0
+    assert step.ctx.status.tolist() == [0, 0, 0, 0]
+    sees = torch.zeros(n, dtype=torch.bool, device=DEV)
+    for seq, key in bad:
+        sees |= (step.seq == seq) & (step.pos >= key) & ((step.pos < key + window) if window else True)
+    want = torch.zeros((n, n_q, d), dtype=torch.bool, device=DEV)
+    want[:, n_q - n_q // n_kv:, max(0, d - 64):] = sees[:, None, None]
+    return got, want
+
+
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("d", [64, 128])
+def test_nan_values_on_both_sides_of_a_window(ops_of, d, splits):
+    """Far more values with NaN than a block lists, in two places: rows whose window lies between the places see none of them."""
+    bad = [(0, 60 + i) for i in range(100)] + [(0, 700 + i) for i in range(100)]
+    got, want = _nan_pattern(ops_of(BF16), 4, 2, d, [(840, 50), (40, 300)], 45, bad, splits=splits)
+    assert torch.equal(got[0], want)
+    assert want.any() and not want[200:600].any()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_nan_values_that_only_the_second_query_tile_sees(ops_of, d):
+    """Blocks of two query tiles of 32 tokens, the second of which reads a tile of keys that the first does not: NaN in that tile, many
+    of them or one, is not the first's."""
+    lens = [(640, 20)] * 3 + [(500, 52)]                      # 68 query tiles of 32 tokens, for each of 8 cached heads
+    for behind in ([129, 130, 180, 250], range(128, 256)):
+        bad = [(seq, key + 128 * tile) for seq in range(4) for tile in (0, 2) for key in behind]
+        got, want = _nan_pattern(ops_of(BF16), 32, 8, d, lens, 0, bad, runs=5)
+        assert want.any() and not want.all()
+        for g in got:
+            assert torch.equal(g, want)
