@@ -44,6 +44,7 @@
 // S_0 at column 0, S_1 at 128 (P_j over columns 0-31 and 64-95 of S_j), O_0 at 256, O_1 at 384
 // (all 512 columns: one block per SM).
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "cache4.cuh"
 #include "tc_common.cuh"
 
@@ -200,18 +201,25 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 
 // Pages in 4 bits (cache4.cuh; kernel form 3, ordinary softmax).  A tile's keys, and its values, are eight units that the TMA copies
 // into shared memory as they lie in their pages, one tile ahead; the gathering warps turn them into the 16-bit operand tiles: a word of
-// codes is the 16-byte piece of its row, and a pair of its codes becomes z + s c by an AND and an FMA, which rounds once.  For as a bit
-// pattern a code in bits 0-3 is the subnormal number c 2^-24 of fp16, or c 2^-133 of bfloat16, and one in bits 4-7 is 16 times that (for
-// bfloat16 the eighth bit is the exponent's lowest, and the numbers up to there have one step); s is multiplied by the other power
-// of two before.  A tile is taken into registers whole, so that the next one can be asked for before it is converted (2,048 tokens behind
-// 6,144 on 32 and 8 heads of 128: 348 us, 381 where it was asked for after that).
+// codes is the 16-byte piece of its row, and a pair of its codes becomes z + s c by an FMA, which rounds once.  Values: as a bit pattern
+// of bfloat16 a code in bits 0-3 is the subnormal number c 2^-133 and one in bits 4-7 is 16 times that (the eighth bit is the exponent's
+// lowest, and the numbers up to there have one step), so that one AND makes a factor; s is multiplied by the other power of two before.
+// Keys: with the exponent of 1,024 beside it a code in bits 0-3 is the number 1,024 + c of fp16, with that of 64 one in bits 4-7 is 64 + c,
+// by the same one logic instruction, and a subtraction leaves c.  A tile is taken into registers whole, so that the next one can be asked
+// for before it is converted (2,048 tokens behind 6,144 on 32 and 8 heads of 128: 348 us, 381 where it was asked for after that).  The warps
+// that turn keys are what the time depends on: with the tile's largest value sought by every thread in all its rows, where the
+// four threads of a row now take one each, it was 353 us, 320 as it is.
 //
 // Values become bfloat16, and so do the weights, as in the other forms.  Keys become fp16, and queries are fp16 too, which is exact:
 // z + s c has 12 significant bits and more, and rounded to the 8 of bfloat16 its error in the scores was most of the output's (8,192
 // keys with a spread of scores of 3: 0.0075 of the output's norm, 0.0026 with the 11 of fp16).  For fp16's range a query's row is
 // multiplied by a power of two that brings its largest element to 2^7 .. 2^8, and a tile of keys by one that brings its largest value
-// to 2^-8 .. 2^-7 (s 2^24 is then a number of fp16 too); the row's and the tile's power are taken out with the scale of the scores.  Values
-// are stored times 2^-64 (for s 2^133; scales up to 2^57 fit), which the outputs are multiplied with at the end.
+// to 2^14 .. 2^15; the row's and the tile's power are taken out with the scale of the scores.  A key keeps its 11 bits while it is no
+// more than 2^28 smaller than the largest of its tile, so that one which is larger than its neighbours, seen by a row or not, takes nothing from
+// them.  (Codes as subnormal numbers of fp16 would spare the subtraction, but s 2^24 has to be a number too then: with the largest value at
+// 2^-7 a key 2^10 times the rest moved the output of rows that do not see it by 1.1 %.)
+//
+// Values are stored times 2^-64 (for s 2^133; scales up to 2^57 fit), which the outputs are multiplied with at the end.
 //
 // A value that is NaN must not reach rows that do not see its key (the product has 0 x NaN for them): such a group is stored as zeros
 // and kept in a list of keys and groups, and at the end the rows that see one of them become NaN in that group's columns.  Of what does not
@@ -226,7 +234,7 @@ struct OddValues {
   int key[kOddKeys];              // key * 2 + group
   int lo[2], hi[2];               // the first and the last of further keys, per group
   unsigned units[2];              // of the tile that lands, keys and values: the units that have a page
-  int largest[2][4];              // of the four warps that gather keys: the largest exponent of their rows of tile t % 2
+  uint32_t largest[2][4];         // of the four warps that gather keys: the largest value of their rows of tile t % 2
   float key_power[4];             // 2^e of tile t % 4: its keys are stored times 2^-e
   float query_power[2][kRows];    // the same of a row of queries
 };
@@ -271,18 +279,23 @@ __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e 
 // The exponent of |v|, -126 at least (128: an infinity or NaN).
 __device__ __forceinline__ int exponent_of(float v) { return max((int)(__float_as_uint(v) >> 23 & 255u) - 127, -126); }
 
+template <typename T> __device__ __forceinline__ uint32_t twice(T pair) { return *reinterpret_cast<const uint32_t*>(&pair); }
+
 // Four words of codes of a row (place q of its 16-byte pieces) become their chunks of the operand tile at `tile`.  lo, hi, z: by
 // group, twice in a register: the scale that a code in bits 0-3 is multiplied with, that for bits 4-7, and the offset.
 template <int D, bool kValues>
 __device__ __forceinline__ void unpack_quad(const uint4& words, uint32_t tile, int row, int q, const uint32_t (&lo)[D / 64],
                                             const uint32_t (&hi)[D / 64], const uint32_t (&z)[D / 64]) {
   const uint32_t w[4] = {words.x, words.y, words.z, words.w};
-  auto value = [](uint32_t c, uint32_t s, uint32_t z) {
+  auto value = [](uint32_t c, uint32_t one, uint32_t s, uint32_t z) {
     uint32_t v;
+    if constexpr (!kValues) asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(c) : "r"(c | one), "r"(one));
     if constexpr (kValues) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(c), "r"(s), "r"(z));
     else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(v) : "r"(c), "r"(s), "r"(z));
     return v;
   };
+  auto low = [&](uint32_t x, int g) { return value(x & 0x000f000fu, 0x64006400u, lo[g], z[g]); };
+  auto high = [&](uint32_t x, int g) { return value(x & 0x00f000f0u, 0x54005400u, hi[g], z[g]); };
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     // which word of the row stands in place 4 q + i (cache4.cuh)
@@ -290,8 +303,7 @@ __device__ __forceinline__ void unpack_quad(const uint4& words, uint32_t tile, i
     const int chunk = D == 64 ? 4 * q + i : 8 * g + 2 * q + (kValues ? i >> 1 : i & 1);
     const uint32_t x = w[i], y = x >> 8;
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + swizzled(row, chunk)),
-                 "r"(value(x & 0x000f000fu, lo[g], z[g])), "r"(value(x & 0x00f000f0u, hi[g], z[g])),
-                 "r"(value(y & 0x000f000fu, lo[g], z[g])), "r"(value(y & 0x00f000f0u, hi[g], z[g]))
+                 "r"(low(x, g)), "r"(high(x, g)), "r"(low(y, g)), "r"(high(y, g))
                  : "memory");
   }
 }
@@ -543,56 +555,56 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
               }
             }
         } else {
-          // the tile's largest |z|, |z + 15 s|; a NaN does not count
-          int top = -126;
+          // the tile's largest |z|, |z + 15 s|: of its kMine = kQuads rows a thread takes row q; a NaN does not count
+          static_assert(kMine == kQuads, "the threads of a row share its thread's rows");
+          float most = 0.f;
 #pragma unroll
-          for (int i = 0; i < kMine; ++i)
+          for (int g = 0; g < G; ++g) {
+            uint32_t mine = sz[0][g];
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-              const float z = cache4::offset_of(sz[i][g]), most = fmaxf(fabsf(z), fabsf(fmaf(15.f, cache4::scale_of(sz[i][g]), z)));
-              if (most < INFINITY) top = max(top, exponent_of(most));
-            }
-          top = __reduce_max_sync(0xffffffffu, top);
-          if (lane == 0) odd.largest[t & 1][st >> 5] = top;
+            for (int i = 1; i < kMine; ++i) mine = q == i ? sz[i][g] : mine;
+            const float z = cache4::offset_of(mine), end = fmaxf(fabsf(z), fabsf(fmaf(15.f, cache4::scale_of(mine), z)));
+            most = fmaxf(most, end < INFINITY ? end : 0.f);
+          }
+          const uint32_t largest = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+          if (lane == 0) odd.largest[t & 1][st >> 5] = largest;
         }
         named_barrier_sync(bar_id, kStream);               // the landed units are read; the next tile's may take their place
         if (st < 32 && ok_all) request(t + 1);
         float down = 1.f;
         if (!values) {
-          const int* l = odd.largest[t & 1];
-          const int e = min(max(max(max(l[0], l[1]), max(l[2], l[3])) + 8, -126), 126);
+          const uint32_t* l = odd.largest[t & 1];
+          // (no less than -60: the product with a row's power, 2^-60 at least too, stays a number)
+          const int e = max(exponent_of(__uint_as_float(max(max(l[0], l[1]), max(l[2], l[3])))) - 14, -60);
           down = power_of_two(-e);
           if (st == 0) odd.key_power[t & 3] = power_of_two(e);
         }
         if (t >= 2 && ok_all && !mbar_wait_long(bar_free + 8 * (t & 1), ((t >> 1) - 1) & 1, giveup)) ok_all = false;
         ok_all = __all_sync(0xffffffffu, ok_all);
         const uint32_t tile = tiles + (t & 1) * kTileBytes;
+        auto convert = [&](auto is_values) {
+          constexpr bool kValues = decltype(is_values)::value;
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          // scales and offsets as the operand's type
-          uint32_t lo[G], hi[G], z[G];
+          for (int i = 0; i < kMine; ++i) {
+            uint32_t lo[G], hi[G], z[G];                   // as the operand's type
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            const float s = cache4::scale_of(sz[i][g]), o = cache4::offset_of(sz[i][g]);
-            if (values) {
-              constexpr float kTo = 590295810358705651712.f, kLeast = 5.421010862427522e-20f;            // 2^69, 2^-64
-              const __nv_bfloat162 a = __floats2bfloat162_rn(s * kTo, s * kTo), b = __floats2bfloat162_rn(s * (kTo / 16), s * (kTo / 16)),
-                                   c = __floats2bfloat162_rn(o * kLeast, o * kLeast);
-              lo[g] = *reinterpret_cast<const uint32_t*>(&a);
-              hi[g] = *reinterpret_cast<const uint32_t*>(&b);
-              z[g] = *reinterpret_cast<const uint32_t*>(&c);
-            } else {
-              const float sd = s * down, od = o * down;
-              const __half2 a = __floats2half2_rn(sd * 16777216.f, sd * 16777216.f), b = __floats2half2_rn(sd * 1048576.f, sd * 1048576.f),
-                            c = __floats2half2_rn(od, od);
-              lo[g] = *reinterpret_cast<const uint32_t*>(&a);
-              hi[g] = *reinterpret_cast<const uint32_t*>(&b);
-              z[g] = *reinterpret_cast<const uint32_t*>(&c);
+            for (int g = 0; g < G; ++g) {
+              const float s = cache4::scale_of(sz[i][g]), o = cache4::offset_of(sz[i][g]);
+              if constexpr (kValues) {
+                constexpr float kTo = 590295810358705651712.f, kLeast = 5.421010862427522e-20f;            // 2^69, 2^-64
+                lo[g] = twice(__floats2bfloat162_rn(s * kTo, s * kTo));
+                hi[g] = twice(__floats2bfloat162_rn(s * (kTo / 16), s * (kTo / 16)));
+                z[g] = twice(__floats2bfloat162_rn(o * kLeast, o * kLeast));
+              } else {
+                lo[g] = hi[g] = twice(__floats2half2_rn(s * down, s * down));
+                z[g] = twice(__floats2half2_rn(o * down, o * down));
+              }
             }
+            unpack_quad<D, kValues>(words[i], tile, row0 + i * kStep, q, lo, hi, z);
           }
-          if (values) unpack_quad<D, true>(words[i], tile, row0 + i * kStep, q, lo, hi, z);
-          else unpack_quad<D, false>(words[i], tile, row0 + i * kStep, q, lo, hi, z);
-        }
+        };
+        if (values) convert(std::true_type{});
+        else convert(std::false_type{});
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_full + 8 * (t & 1));
@@ -720,7 +732,7 @@ attention_prefill_pingpong_kernel(const __nv_bfloat16* __restrict__ qkv, int row
               top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
 #pragma unroll
             for (int o = 1; o < kChunks; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const int e = top > 0.f && top < INFINITY ? min(max(exponent_of(top) - 7, -126), 126) : 0;
+            const int e = top > 0.f && top < INFINITY ? min(max(exponent_of(top) - 7, -60), 120) : 0;
             const float by = power_of_two(-e);
             if (ch == 0) odd.query_power[j][r] = power_of_two(e);
             uint32_t out4[4];

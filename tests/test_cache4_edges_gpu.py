@@ -4,7 +4,7 @@ import torch
 
 from leone_b200.cache import packed
 from leone_b200.parts.rotary import build_rotary_table
-from tests.fewer_bits import Step, quantize4
+from tests.fewer_bits import Step, attention64, quantize4, values4
 
 pytestmark = pytest.mark.gpu
 
@@ -110,11 +110,11 @@ def _nan_pattern(ops, n_q, n_kv, d, lens, window, bad, runs=1, splits=0):
 @pytest.mark.parametrize("splits", [1, 2])
 @pytest.mark.parametrize("d", [64, 128])
 def test_nan_values_on_both_sides_of_a_window(ops_of, d, splits):
-    """Far more values with NaN than a block lists, in two places: rows whose window lies between the places see none of them."""
-    bad = [(0, 60 + i) for i in range(100)] + [(0, 700 + i) for i in range(100)]
-    got, want = _nan_pattern(ops_of(BF16), 4, 2, d, [(840, 50), (40, 300)], 45, bad, splits=splits)
+    """A block of 128 tokens whose first 40 and last 40 keys have NaN, more than it lists: rows whose window lies between see none."""
+    bad = [(0, 64 + 128 * block + i) for block in range(2) for i in (*range(40), *range(88, 128))]
+    got, want = _nan_pattern(ops_of(BF16), 2, 2, d, [(256, 64)], 16, bad, splits=splits)
     assert torch.equal(got[0], want)
-    assert want.any() and not want[200:600].any()
+    assert want[:40, 1].any(-1).all() and not want[56:88].any()
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -128,3 +128,56 @@ def test_nan_values_that_only_the_second_query_tile_sees(ops_of, d):
         assert want.any() and not want.all()
         for g in got:
             assert torch.equal(g, want)
+
+
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kind", ["key", "channel"])
+@pytest.mark.parametrize("power", [10, 16, 20])
+def test_prompt_of_keys_of_unlike_size(ops_of, power, kind, d, splits):
+    """One key, or one channel of every key, 2^10 and more times the rest: rows that do not see the key lose nothing by it, and the small
+    channels count as they did.
+
+    An output's roundings: its own to bfloat16 and its values' (an element each, off by 2^-7 / 12^(1/2) of the number's power of two,
+    0.0016 of the numbers of a row by their squares), and the weights': the same again for many keys, at most 2^-8 of every element
+    alike where one key has all the weight.  Keys are fp16: 2^-11 at most of a score's products, which are random, about 0.0003 for
+    scores of a size of one.  So 0.0028 of a call's outputs and 2^-8 + 2^(1/2) 0.0016, a fourth more for the chance of 64 elements, of a row's."""
+    ops = ops_of(BF16)
+    n_q, n_kv, lens, large = 4, 2, [(200, 100), (60, 300)], [(0, 255), (1, 305)]
+    step = Step(lens, 16, DEV, seed=power)
+    x = [torch.randn((step.pages, n_kv, 16, d), generator=_gen(power + i), device=DEV).double() for i in range(2)]
+    n = step.ctx.n_tokens
+    qkv = torch.randn((n, (n_q + 2 * n_kv) * d), generator=_gen(5), device=DEV)
+    if kind == "key":
+        for seq, key in large:
+            x[0][int(step.table[seq, key // 16]), :, key % 16] *= 2.0 ** power
+    else:
+        x[0][..., 5] = x[0][..., 5].abs() * 2.0 ** power
+        qkv[:, 5:n_q * d:d] *= 2.0 ** -power
+    qkv = qkv.to(BF16)
+    pools, plain = [], []
+    for t, values in zip(x, (False, True)):
+        coded = quantize4(t)
+        pools.append(packed.pack_pages(*coded, values))
+        plain.append(values4(*coded))
+    out = torch.zeros((n, n_q * d), dtype=BF16, device=DEV)
+    ops.force_prompt4_splits = splits
+    try:
+        ops.attention(step.ctx, qkv, out, n_q, n_kv, d, d ** -0.5, None, step.view(*pools))
+    finally:
+        ops.force_prompt4_splits = 0
+    q = qkv[:, :n_q * d].double().unflatten(1, (n_q, d))
+    want, *_ = attention64(q, *plain, lens, step.table, 16, d ** -0.5, 0)
+    off = (out.double().view_as(want) - want).square()
+    counts = torch.ones((n, n_q), dtype=torch.bool, device=DEV)
+    if kind == "key":
+        # rows whose score with the large key is not far from the others' turn on its last bits
+        for seq, key in large:
+            k = plain[0][int(step.table[seq, key // 16]), :, key % 16].repeat_interleave(n_q // n_kv, 0)
+            score = (q * k).sum(-1) * d ** -0.5
+            counts &= ~((step.seq == seq) & (step.pos >= key))[:, None] | (score.abs() > 40)
+        assert counts[:155].all() and counts.float().mean() > 0.9
+    off, size = off[counts], want.square()[counts]
+    assert (off.sum() / size.sum()).sqrt() < 1.25 * 3 ** 0.5 * 0.0016
+    assert (off.sum(-1) / size.sum(-1)).sqrt().max() < 2.0 ** -8 + 1.25 * 2 ** 0.5 * 0.0016
+    assert step.ctx.status.tolist() == [0, 0, 0, 0]
