@@ -216,10 +216,10 @@ __device__ __noinline__ void append_exact(const T* row, const TW* w, float eps, 
 // are what they are; minima, maxima and quotients are of 32.  Where the ends of the range in which the minimum and the maximum lie give
 // one z and one s, those are right.  A quotient that comes no nearer to a border of two codes than the roundings take it is rounded right;
 // one that does is settled by the sign of x - z - (code + 1/2) s in 64 bits.  (Values in bfloat16 lie on a border more often than
-// not in a row.)  Where z or s is in doubt, or something not finite, the warp computes the row again, which a step hardly ever does: that
-// code is never in the instruction cache, and a block waits 4 us for it.  (With norm and rotation in 32 bits a row of keys in a hundred
-// was in doubt: 2,048 tokens of 48 heads of 128 took 28.2 us, of 22 of 64 10.6, where this takes 20.7 and 8.6.
-// Their queries alone take 8.6, the floor is 5.)
+// not in a row.)  Where z or s is in doubt, where a key's rounding is a quarter of a step and more, or something is not finite, the
+// warp computes the row again, which a step hardly ever does: that code is never in the instruction cache, and a block waits 4 us for it.
+// (With norm and rotation in 32 bits a row of keys in a hundred was in doubt: 2,048 tokens of 48 heads of 128 took 28.2 us, of 22 of 64
+// 10.6, where this takes 20.6 and 8.6.  Their queries alone take 8.6, the bytes 6.8.)
 constexpr float kRounded = 1.01f / 16777216.f;
 constexpr float kToInteger = 12582912.f;           // 1.5 2^23: adding it rounds to an integer, which the low bits then hold
 constexpr int kAppendWarps = 4;
@@ -462,6 +462,7 @@ append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__
           doubt |= (s[g] != 0.f && !(s[g] > 1e-37f && s[g] < 1e37f)) || !(fabsf(z[g]) < 3e38f);
           inv[g] = s[g] > 0.f ? reciprocal(s[g]) : 0.f;
           limit[g] = 0.5f - fmaf(err, inv[g] * 1.01f, 15.5f * 2.5e-7f);
+          doubt |= limit[g] < 0.25f;                         // (one border has to be the only one in reach)
         }
         if (G == 1) {
           z[1] = z[0];
@@ -485,7 +486,7 @@ append_vec_kernel(T* __restrict__ qkv, int n_q, int n_kv, const TW* __restrict__
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               const float x = g ? b[i] : a[i], q = (x - z[g]) * inv[g], low = floorf(q);
-              if (fabsf(fabsf(q - low) - 0.5f) > 1e-3f) continue;
+              if (fabsf(fabsf(q - low) - 0.5f) > 0.5f - limit[g] + 1e-5f) continue;      // (what made it near, and the product's rounding)
               const double gap = (computed ? (g ? db[i] : da[i]) : (double)x) - (double)z[g];
               const double side = fma(-(double)(low + 0.5f), (double)s[g], gap);
               code[g][i] = (side > 0.0 || (side == 0.0 && ((int)low & 1)) ? low + 1.f : low) + kToInteger;

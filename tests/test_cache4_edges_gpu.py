@@ -181,3 +181,29 @@ def test_prompt_of_keys_of_unlike_size(ops_of, power, kind, d, splits):
     assert (off.sum() / size.sum()).sqrt() < 1.25 * 3 ** 0.5 * 0.0016
     assert (off.sum(-1) / size.sum(-1)).sqrt().max() < 2.0 ** -8 + 1.25 * 2 ** 0.5 * 0.0016
     assert step.ctx.status.tolist() == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("spread", [1e-6, 2e-5, 1e-4, 1e-3])
+@pytest.mark.parametrize("dtype,d,n_kv,tokens", [(FP32, 64, 2, 3000), (FP32, 128, 2, 3000), (FP32, 64, 8, 20), (BF16, 128, 4, 1500)])
+def test_append_of_keys_that_are_nearly_equal(ops_of, dtype, d, n_kv, tokens, spread):
+    """Groups of normed keys whose spread is small against their size: their rounding to 32 bits is a good part of a step, and codes are
+    those of 64 bits all the same."""
+    ops = ops_of(dtype)
+    step = Step([(tokens, 3)], 16, DEV)
+    x = 1 + torch.rand((tokens, 1 + 2 * n_kv, d), generator=_gen(tokens), device=DEV) * spread
+    # the least of a normed head lies just above 1.5, a number of bfloat16
+    weights = torch.full((2, d), 1.5 * (1 + 0.7 * spread), device=DEV)
+    if dtype == BF16:                                        # equal elements, and weights that are not
+        x = torch.randn((tokens, 1 + 2 * n_kv, 1), generator=_gen(1), device=DEV).expand_as(x).abs() + 0.1
+        weights = 1.5 * (1 + 0.2 * spread + 2.0 ** -20 + torch.rand((2, d), generator=_gen(2), device=DEV) * spread)
+    rows = x.to(dtype).flatten(1)
+    pools = [torch.zeros((step.pages, n_kv, 16, packed.row_bytes(d)), dtype=torch.uint8, device=DEV) for _ in range(2)]
+    eps = 2.0 ** -30
+    ops.qk_norm_rope_write(step.ctx, rows.clone(), 1, n_kv, d, weights[0], weights[1], eps, None, 0, step.view(*pools))
+    k = rows.double().unflatten(1, (1 + 2 * n_kv, d))[:, 1:1 + n_kv]
+    k = k * weights[1].double() * torch.rsqrt(k.square().mean(-1, keepdim=True) + eps)
+    have = [t[step.page, :, step.slot] for t in packed.unpack_pages(pools[0], d, False)]
+    codes, s, z = quantize4(k)
+    assert torch.equal(have[1].double(), s) and torch.equal(have[2].double(), z)
+    assert torch.equal(have[0].long(), codes)
+    assert (s.amax() < 2 * spread) and len(codes.unique()) >= 8 and step.ctx.status.tolist() == [0, 0, 0, 0]
