@@ -22,7 +22,7 @@ from ..cache import packed
 from ..csrc.build import ensure_built
 from .entry_points import EntryPoints
 from .fast import leading_ones
-from .int8 import MAX_K, Int8Matrix, Int8Products
+from .int8 import MAX_K, Int8Matrix, Int8Products, PerThread
 
 _STATUS_TEXT = {
     1: "a token id outside the vocabulary reached the embedding kernel",
@@ -161,6 +161,7 @@ class CudaOps:
         self.launches = 0
         self.use_latent_tc = None          # True, False: latent attention of prompt portions on tcgen05 or not, whatever the rule says
         self._sample_scratch = None
+        self._workspaces = PerThread()
         self.status = None
         # LEONE_NO_PDL=1 launches every kernel fully serialised after its predecessor
         self.set_pdl(os.environ.get("LEONE_NO_PDL", "0") != "1")
@@ -521,10 +522,11 @@ class CudaOps:
 
     def _workspace(self, name: str, count: int, dtype=torch.float32) -> torch.Tensor:
         """``count`` numbers for the call at hand.  A captured graph has its own (from the graph's pool), so that graphs may be replayed
-        beside one another; every other call one of its stream's, which only grows."""
+        beside one another; every other call one of its thread's and stream's, which only grows.  (A call makes several launches, and
+        another thread's on the same stream may come between them.)"""
         if torch.cuda.is_current_stream_capturing():
             return torch.empty(count, dtype=dtype, device=self.device)
-        held = self.__dict__.setdefault("_workspaces", {})
+        held = self._workspaces.held
         key = (name, self._stream())
         buf = held.get(key)
         if buf is None or buf.numel() < count:

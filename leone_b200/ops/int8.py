@@ -8,6 +8,7 @@ or with 8-bit activations on dp4a (crates/leone-cuda/cuda/ie_cuda.cu:1718-1931).
 from __future__ import annotations
 
 import ctypes
+import threading
 from ctypes import addressof, c_float
 from typing import Optional
 
@@ -39,6 +40,13 @@ def quantize_matrix(w: torch.Tensor):
     return codes, scales
 
 
+class PerThread(threading.local):
+    """``held``: a dictionary of the calling thread's own."""
+
+    def __init__(self):
+        self.held = {}
+
+
 class Int8Matrix:
     """A matrix ``[out, in]`` in 8-bit integers with a scale for each row, and the fp32 bias ``[out]`` (or None) of its products."""
 
@@ -67,7 +75,7 @@ class Int8Products:
             self.lib.leone_bf16_set_pdl(1 if ops._pdl else 0)
         self.calls = EntryPoints(self.lib)
         self.sm_count = torch.cuda.get_device_properties(ops.device).multi_processor_count
-        self.plans, self.buffers = {}, {}
+        self.plans, self.buffers = {}, PerThread()
 
     force = None               # (form, splits or tile width) of every product, whatever the rule says (tests set it)
 
@@ -124,14 +132,16 @@ class Int8Products:
 
     def tokens(self, m: int, k: int, stream):
         """Codes and scales of ``m`` tokens for the call at hand.  A captured graph has its own (from the graph's pool), so that graphs may
-        be replayed beside one another; every other call those of its width and stream, which only grow."""
+        be replayed beside one another; every other call those of its width, thread and stream, which only grow.  (Between a call's
+        two launches there may be one of another thread's on the same stream.)"""
         captured = torch.cuda.is_current_stream_capturing()
-        held = None if captured else self.buffers.get((k, stream))
+        buffers = self.buffers.held
+        held = None if captured else buffers.get((k, stream))
         if held is not None and held[0].shape[0] >= m:
             return held
         rows = m if captured else -(-m // 64) * 64
         fresh = (torch.empty((rows, k), dtype=torch.int8, device=self.ops.device),
                  torch.empty(rows, dtype=torch.float32, device=self.ops.device))
         if not captured:
-            self.buffers[k, stream] = fresh
+            buffers[k, stream] = fresh
         return fresh
