@@ -476,10 +476,11 @@ class CudaOps:
             self.launches += 1
             return
         _need(getattr(w_gate_up, "gate_up_layout", None) == "stacked", "gate/up layout")
-        scratch = self._scratch("gate_up", m, 2 * inter, x.dtype)
         if int8:
+            scratch = self._workspace("gate_up", m * 2 * inter, x.dtype)[:m * 2 * inter].view(m, 2 * inter)
             self.linear(x, w_gate_up, scratch)
         else:
+            scratch = self._scratch("gate_up", m, 2 * inter, x.dtype)
             self._gemm_simt(x, w_gate_up.weight, scratch, 0, None, w_gate_up.bias)
         self.launches += 1
         if gate_shape is None:
@@ -527,7 +528,7 @@ class CudaOps:
         if torch.cuda.is_current_stream_capturing():
             return torch.empty(count, dtype=dtype, device=self.device)
         held = self._workspaces.held
-        key = (name, self._stream())
+        key = (name, self._stream(), dtype)
         buf = held.get(key)
         if buf is None or buf.numel() < count:
             buf = held[key] = torch.empty(max(count, 1 << 16), dtype=dtype, device=self.device)

@@ -123,3 +123,42 @@ def test_split_attention_of_two_threads_on_one_stream(lens, splits):
     for outs, right in zip(_in_threads(3, work), want):
         torch.cuda.synchronize()
         assert torch.equal(outs, right.expand_as(outs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_gates_without_the_epilogue_on_two_streams_at_once(captured):
+    """Where gate and up lie side by side before the gate (32-bit runs), they lie in the stream's own workspace, or the graph's."""
+    from leone_b200.ops.int8 import quantize_matrix
+    ops = CudaOps(DEV, torch.float32)
+    ops.bind_status(torch.zeros(4, dtype=torch.int32, device=DEV))
+    gen = torch.Generator(DEV).manual_seed(3)
+    m, k, inter = 700, 256, 1000
+    gate, up = (quantize_matrix(torch.randn((inter, k), generator=gen, device=DEV)) for _ in range(2))
+    w = ops.prepare_gate_up_int8(*gate, *up)
+    xs = [torch.randn((m, k), generator=gen, device=DEV) for _ in range(2)]
+    want = [torch.empty((m, inter), device=DEV) for _ in range(2)]
+    for x, y in zip(xs, want):
+        ops.linear_swiglu(x, w, y)
+    streams, outs, graphs = [torch.cuda.Stream() for _ in range(2)], [torch.zeros_like(y) for y in want], []
+    torch.cuda.synchronize()
+    if captured:
+        for x, y in zip(xs, outs):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=streams[0]):
+                ops.linear_swiglu(x, w, y)
+    for _ in range(20):
+        for y in outs:
+            y.zero_()
+        torch.cuda.synchronize()
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                if captured:
+                    graphs[i].replay()
+                else:
+                    for _ in range(4):
+                        ops.linear_swiglu(xs[i], w, outs[i])
+        torch.cuda.synchronize()
+        for y, z in zip(outs, want):
+            assert torch.equal(y, z)
+    del graphs
