@@ -13,11 +13,13 @@ import torch
 UNIT = 16          # tokens whose rows lie together; pages are multiples of it
 MAX_DIM = 512
 
-def attention_workspace(d: int) -> int:
-    """Bytes that the parts of split attention over such pages take at most: 148 tiles of 128 rows of prompt portions, three blocks an SM of up
-    to 16 rows of decode, or 2,048 blocks of 8 rows of the kernel of any size."""
-    return 4 * ((148 * 128 + 3 * 148 * 16) * 130 + 2048 * 8 * (d + 2))
 
+def attention_workspace(d: int) -> int:
+    """Bytes that the parts of split attention over such pages take at most: of a step 148 tiles of 128 rows of prompt portions, three blocks
+    an SM of up to 16 rows of decode, or 2,048 blocks of 8 rows of the kernel of any size; and the latter two twice more, for the
+    captured decode steps and for the stream on which they are captured."""
+    decode = 3 * 148 * 16 * 130 + 2048 * 8 * (d + 2)
+    return 4 * (148 * 128 * 130 + 3 * decode)
 
 
 def groups(d: int) -> int:

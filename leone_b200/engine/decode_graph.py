@@ -72,7 +72,6 @@ class DecodeGraph:
             self.meta[self._tables_at:].fill_(-1)
         self._events = [torch.cuda.Event(), torch.cuda.Event()]
         self.launches_per_step = 0
-        self.stream = torch.cuda.Stream(device=dev)
 
     def bucket_for(self, longest: int) -> int:
         """The context bucket of a step whose longest sequence holds ``longest`` tokens after it:
@@ -195,9 +194,9 @@ class DecodeGraph:
         capture one step for contexts of up to ``bucket`` tokens and select it.  The caller fills
         the buffers again afterwards: the eager step has advanced them."""
         self.ctx.max_ctx_len = bucket
-        cur = torch.cuda.current_stream(self.engine.device)
-        self.stream.wait_stream(cur)
-        with torch.cuda.stream(self.stream):
+        cur, stream = torch.cuda.current_stream(self.engine.device), self.engine.capture_stream()
+        stream.wait_stream(cur)
+        with torch.cuda.stream(stream):
             # The eager step really runs.  What it writes into pages and into the step's own
             # buffers is written again by the first replayed step, but fixed-size state would
             # be advanced by a token for good: keep it and put it back.
@@ -205,22 +204,23 @@ class DecodeGraph:
             self._one_step()
             for pos, state in kept.items():
                 self.engine._run_state[pos].copy_(state)
-            self.stream.synchronize()
+            stream.synchronize()
             before = self.engine.ops.launches
-            self.graph = self.graphs[bucket] = torch.cuda.CUDAGraph()
-            self.bucket = bucket
+            graph, pool = torch.cuda.CUDAGraph(), self.engine.capture_pool()
             # an object that the collector finalises in the middle of a capture (an older
             # graph, a freed pool) would invalidate the capture: keep the collector out
             was_enabled = gc.isenabled()
             gc.disable()
             try:
-                with torch.cuda.graph(self.graph, stream=self.stream, capture_error_mode="thread_local"):
+                with torch.cuda.graph(graph, pool=pool, stream=stream, capture_error_mode="thread_local"):
                     self._one_step()
             finally:
                 if was_enabled:
                     gc.enable()
+            self.graph, self.bucket = graph, bucket
+            self.graphs[bucket] = graph
             self.launches_per_step = self.engine.ops.launches - before
-        cur.wait_stream(self.stream)
+        cur.wait_stream(stream)
         self.counter.zero_()
 
     def advance_from_host(self, rids: Sequence[Hashable], table_lens) -> None:

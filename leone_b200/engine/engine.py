@@ -78,7 +78,7 @@ class Engine:
         if ops is None:
             ops = default_ops(self.device, self.dtype)
         self.ops = ops
-        self.rt = Runtime(self.device, self.dtype, ops, max_batch_tokens, cache_bits, weight_bits)
+        self.rt = Runtime(self.device, self.dtype, ops, max_batch_tokens, cache_bits, weight_bits, max_requests)
         self.max_batch_tokens = max_batch_tokens
         self.model = Model(spec, self.rt)
         specs = self.model.weight_specs()
@@ -209,6 +209,7 @@ class Engine:
         # size holds is small, because the logits buffer is shared
         self.max_decode_graphs = max(64, max_requests)
         self._decode_logits = None
+        self._capture_stream = None
         # a decode step launched before the step before it was read (see decode_steps)
         self._ahead = None
         self.lookahead = os.environ.get("LEONE_NO_LOOKAHEAD", "0") != "1"
@@ -481,6 +482,17 @@ class Engine:
             self._decode_logits = torch.empty((self.max_requests, self.spec.vocab_size), dtype=torch.float32,
                                               device=self.device)
         return self._decode_logits
+
+    def capture_stream(self) -> torch.cuda.Stream:
+        """The stream on which decode steps are captured, and run once before."""
+        if self._capture_stream is None:
+            self._capture_stream = torch.cuda.Stream(device=self.device)
+        return self._capture_stream
+
+    def capture_pool(self):
+        """The memory pool of the decode steps captured so far (None before the first).  An engine's steps run one behind another, so the
+        workspaces of its captured ones may lie in the same memory."""
+        return next((g.pool() for d in self._decode_graphs.values() for g in d.graphs.values()), None)
 
     def _decode_graph(self, rids, last_tokens, lengths, params, state, steps: int = 1):
         """The captured decode step for this batch size and for the context bucket that holds

@@ -206,7 +206,7 @@ class Runtime:
     """What every part gets at construction: device, run dtype, kernels and scratch buffers."""
 
     def __init__(self, device, dtype: torch.dtype, ops, max_tokens: int, cache_bits: Optional[int] = None,
-                 weight_bits: Optional[int] = None):
+                 weight_bits: Optional[int] = None, max_requests: Optional[int] = None):
         if cache_bits not in (None, 4) or weight_bits not in (None, 8):
             raise ValueError(f"caches are held in the run dtype or in 4 bits, matrices in the run dtype or in 8 bits, "
                              f"not in {cache_bits} and {weight_bits}")
@@ -218,6 +218,7 @@ class Runtime:
         self.max_tokens = max_tokens
         self.cache_bits = cache_bits       # 4: mixers that can ask for their pages in 4 bits
         self.weight_bits = weight_bits     # 8: parts that can keep their matrices in 8-bit integers
+        self.max_requests = max_requests   # tokens of a decode step at most (None: as many as of any step)
         self._buffers: Dict[str, torch.Tensor] = {}
         self._views: Dict[tuple, torch.Tensor] = {}
 
@@ -264,8 +265,10 @@ class Runtime:
         return rows * cols + 4 * rows if self.weight_bits == 8 else rows * cols * self.dtype.itemsize
 
     def token_scratch_bytes(self, max_tokens: int, width: int) -> int:
-        """Bytes of what the ops keep of a step's tokens for products with such matrices (codes and scales)."""
-        return max_tokens * (width + 4) if self.weight_bits == 8 else 0
+        """Bytes of what the ops keep of a step's tokens for products with such matrices (codes and scales): a step's, and twice a decode
+        step's, for the captured ones and for the stream on which they are captured."""
+        decode = max_tokens if self.max_requests is None else min(max_tokens, self.max_requests)
+        return (max_tokens + 2 * decode) * (width + 4) if self.weight_bits == 8 else 0
 
     def flat_buffer(self, name: str, numel: int, dtype: torch.dtype, reserve: int = 0) -> torch.Tensor:
         """A scratch vector of at least ``numel`` elements under ``name`` (``reserve``: what to
