@@ -1,0 +1,52 @@
+"""Products of 8-bit integers: a tile's width moves no bit of a result."""
+import pytest
+import torch
+
+from leone_b200.ops.int8 import NARROW, PAIRS, Int8Products
+from tests.test_int8_gpu import BF16, DEV, _check, _gen, _inputs, _want, ops_of  # noqa: F401 (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("form", [NARROW, PAIRS])
+@pytest.mark.parametrize("m,n,k", [(1, 400, 272), (129, 9760, 1024), (257, 96, 4096), (300, 1056, 1040), (130, 1600, 144)])
+def test_every_width(ops_of, form, m, n, k):  # noqa: F811
+    """All widths that the rule chooses from, with a bias, onto a residual and through the gates: the sums are exact and the epilogue is one, so
+    that results are equal bit for bit, and those of one width are right."""
+    ops = ops_of(BF16)
+    x, codes, scales = _inputs(m, n, k, BF16, m)
+    bias = torch.randn(n, generator=_gen(3), device=DEV)
+    plain, biased = ops.prepare_matrix_int8(codes, scales), ops.prepare_matrix_int8(codes, scales, bias)
+    half = n // 2
+    gates = [ops.prepare_gate_up_int8(codes[:half], scales[:half], codes[half:], scales[half:], *b) for b in ((), (bias[:half], bias[half:]))] \
+        if half % 16 == 0 else []
+    residual = torch.randn((m, n), generator=_gen(8), device=DEV)
+
+    def results(width):
+        outs = [torch.full((m, n), 9.0, dtype=dtype, device=DEV) for dtype in (BF16, torch.float32, BF16, torch.float32)] + [residual.clone()]
+        ops.int8.force = (form, width)
+        try:
+            for w, out in zip((plain, plain, biased, biased), outs):
+                ops.linear(x, w, out)
+            ops.linear(x, biased, outs[4], residual=outs[4])
+            for w in gates:
+                for shape in (None, (1.0, 7.0, 1.0, 0.0)):
+                    outs.append(torch.full((m, half), 9.0, dtype=BF16, device=DEV))
+                    ops.linear_swiglu(x, w, outs[-1], gate_shape=shape)
+        finally:
+            ops.int8.force = None
+        return outs
+
+    first = results(64)
+    want = _want(x, codes, scales)
+    _check(first[0], want, want * 0, BF16)
+    _check(first[1], want, want * 0, torch.float32)
+    _check(first[3], want + bias.double(), bias.double(), torch.float32)
+    for width in range(32, 257, 32):
+        for a, b in zip(first, results(width)):
+            assert torch.equal(a, b), width
+
+
+def test_the_rule_takes_160_weight_rows(ops_of):  # noqa: F811
+    products: Int8Products = ops_of(BF16).int8
+    assert products.choose(129, 9760, 1024) == (PAIRS, 160)
