@@ -545,10 +545,12 @@ class CudaOps:
         if cols != (n_q + 2 * n_kv) * d or not qkv.is_contiguous():
             raise KernelError("qkv layout")
         w_dtype = 0
-        if q_norm_w is not None:
-            if k_norm_w is None or q_norm_w.dtype != k_norm_w.dtype or q_norm_w.numel() != d or k_norm_w.numel() != d:
+        if q_norm_w is not None or k_norm_w is not None:     # (keys alone may have a norm)
+            if k_norm_w is None or k_norm_w.numel() != d or not k_norm_w.is_contiguous():
                 raise KernelError("q/k norm weights")
-            w_dtype = _dt(q_norm_w.dtype)
+            if q_norm_w is not None and (q_norm_w.dtype != k_norm_w.dtype or q_norm_w.numel() != d or not q_norm_w.is_contiguous()):
+                raise KernelError("q/k norm weights")
+            w_dtype = _dt(k_norm_w.dtype)
         max_pos = 0
         if table is not None:
             shape = table.shape
