@@ -97,10 +97,10 @@ quantize_rows16_kernel(const T* __restrict__ x, int ldx, int8_t* __restrict__ co
 
 using namespace leone;
 
-// x [m, k] with ldx elements between rows; codes [m, k] without gaps, scales [m].
+// x [m, k] with ldx elements between rows (0: one row for all; rows may overlap); codes [m, k] without gaps, scales [m].
 extern "C" int leone_quantize_rows(int dtype, const void* x, int m, int k, int ldx, void* codes, float* scales, cudaStream_t stream) {
   if (m <= 0) return 0;
-  if (k <= 0 || ldx < k) return kRefusedSize;
+  if (k <= 0 || ldx < 0) return kRefusedSize;
   const int item = dtype == 0 ? 4 : 2;
   if (k % 16 == 0 && k <= 16384 && ((long long)ldx * item) % 16 == 0 && (((uintptr_t)x | (uintptr_t)codes) & 15) == 0) {
     const dim3 threads((k / 16 + 31) / 32 * 32);

@@ -116,13 +116,16 @@ class Int8Products:
         if plan is None:
             plan = self.plans[m, n, k] = self.choose(m, n, k)
         form, width = self.force or plan
+        step = x.stride(0) if m > 1 else k                   # elements between rows, 32 bits in the kernels
+        if step >= 1 << 31:
+            raise OverflowError(f"linear (8 bits): rows {step} elements apart")
         stream = ops._stream()
         codes, scales = self.tokens(m, k, stream)
         gs = None
         if gate_shape is not None:
             shape = (c_float * 4)(*[float(v) for v in gate_shape])
             gs = addressof(shape)
-        code = self.calls.leone_linear_i8(1 if x.dtype == torch.bfloat16 else 0, x, x.stride(0), codes, scales, w.weight, w.scales, out,
+        code = self.calls.leone_linear_i8(1 if x.dtype == torch.bfloat16 else 0, x, step, codes, scales, w.weight, w.scales, out,
                                           residual, m, n, k, out.stride(0), epilogue, form, width, ops.status, self.sm_count, gs, w.bias,
                                           stream)
         if code != 0:

@@ -50,3 +50,16 @@ def test_every_width(ops_of, form, m, n, k):  # noqa: F811
 def test_the_rule_takes_160_weight_rows(ops_of):  # noqa: F811
     products: Int8Products = ops_of(BF16).int8
     assert products.choose(129, 9760, 1024) == (PAIRS, 160)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 96, 256), (5, 96, 256), (140, 400, 272)])
+def test_rows_that_are_one(ops_of, m, n, k):  # noqa: F811
+    """A row that is broadcast over the tokens, and rows that overlap, as products in the run dtype take them."""
+    ops = ops_of(BF16)
+    x, codes, scales = _inputs(m, n, k, BF16, m)
+    w = ops.prepare_matrix_int8(codes, scales)
+    for rows in (x[:1].expand(m, k), x.flatten().as_strided((m, k), (16 if m > 1 else 0, 1)) if m * k >= 16 * m + k else x[:1]):
+        out = torch.empty((rows.shape[0], n), dtype=BF16, device=DEV)
+        ops.linear(rows, w, out)
+        want = _want(rows, codes, scales)
+        _check(out, want, want * 0, BF16)
