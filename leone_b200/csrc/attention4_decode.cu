@@ -22,9 +22,11 @@
 // Splits of up to 8 merge inside a thread-block cluster through distributed shared memory, more through scratch and a kernel.
 //
 // 32 query heads on 8 of 128, one call behind another: 166 sequences of 2,048 keys 87 us (4.5 TB/s of the copy's 6.5), 64 of them 45 us (512
-// blocks where 444 run at once), 64 of up to 2,048 30 us, one of 40,960 19.4 us (2.4 TB/s).  What bounds it is the instructions: with every page
-// in the L2 166 sequences take 92 us where they take 96 from memory; 12 warps an SM keep half of the issue slots busy (fixed latencies first,
-// then the ALUs that mask codes).  Of 296 instructions for 16 keys the scores take 74, the outputs 105, maximum, weights and the ring 80.
+// blocks where 444 run at once), 64 of up to 2,048 30 us, one of 40,960 19.4 us (2.4 TB/s).  Memory does not bound it: with every page in the
+// L2 166 sequences take 92 us where they take 96 from memory.  Nor does a pipe: at 168 registers a thread 12 warps an SM, 2.5 a scheduler, find
+// an instruction to issue in 48 % of the cycles (fixed latencies first, then memory, then the ALUs that mask codes, 46 % busy), so the
+// chains of a part's instructions are what the time goes by, and their number.  Of 296 instructions for 16 keys the scores take 74, the
+// outputs 105, maximum, weights and the ring 80.
 // Slower or no faster: four blocks an SM with parts of two (64 sequences 41 us, of up to 2,048 34, one of 40,960 23), parts of one, keys
 // dealt to warps as one line of all sequences, blocks that sort the sequences by length themselves.
 #include "cache4.cuh"
@@ -650,12 +652,8 @@ int launch_decode(const __nv_bfloat16* qkv, int row_stride, __nv_bfloat16* out, 
 
 using namespace leone;
 
-// Floats of scratch for splits that do not merge in clusters.
-extern "C" long long leone_attention4_decode_scratch(int n_seqs, int n_q, int d, int splits) {
-  return (long long)n_seqs * n_q * splits * (d + 2);
-}
 // One query token a sequence (row q_start[s] of qkv).  `splits`: blocks that share a sequence's keys, up to 8 with in_cluster, up to 64
-// with scratch; `order`: the sequences in the order in which their blocks start, or null.
+// with scratch of n_seqs n_q splits (d + 2) floats; `order`: the sequences in the order in which their blocks start, or null.
 extern "C" int leone_attention4_decode(const void* qkv, int row_stride, void* out, int out_stride, const void* k_pool,
                                        const void* v_pool, const int* block_table, int table_width, const int* q_start,
                                        const int* ctx_len, int n_seqs, int n_q, int n_kv, int d, float scale, int window,

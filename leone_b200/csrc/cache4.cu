@@ -259,7 +259,6 @@ template <typename F> __device__ __forceinline__ void turn_pair(F& x, F& y, floa
   x = u;
 }
 
-//
 // kFew: the form for up to two blocks an SM.  Its code is one copy for keys and values, and a block first goes through it over what happens
 // to be in shared memory, with results that go nowhere, while the kernel before this one still works: a launch of a step finds the code
 // in no cache, and waited longer for it than it ran.  An 8B layer's products with append and decode attention over 2,048 keys: one token 89.8
