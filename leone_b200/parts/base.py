@@ -265,10 +265,13 @@ class Runtime:
         return rows * cols + 4 * rows if self.weight_bits == 8 else rows * cols * self.dtype.itemsize
 
     def token_scratch_bytes(self, max_tokens: int, width: int) -> int:
-        """Bytes of what the ops keep of a step's tokens for products with such matrices (codes and scales): a step's, and twice a decode
-        step's, for the captured ones and for the stream on which they are captured."""
-        decode = max_tokens if self.max_requests is None else min(max_tokens, self.max_requests)
-        return (max_tokens + 2 * decode) * (width + 4) if self.weight_bits == 8 else 0
+        """Bytes of what the ops keep of a step's tokens for products with such matrices (codes and scales)."""
+        return (max_tokens + self.captured_tokens(max_tokens)) * (width + 4) if self.weight_bits == 8 else 0
+
+    def captured_tokens(self, max_tokens: int) -> int:
+        """Tokens for which the ops' workspaces are there beside a step's: twice a decode step's, for the captured ones and for the stream on
+        which they are captured."""
+        return 2 * (max_tokens if self.max_requests is None else min(max_tokens, self.max_requests))
 
     def flat_buffer(self, name: str, numel: int, dtype: torch.dtype, reserve: int = 0) -> torch.Tensor:
         """A scratch vector of at least ``numel`` elements under ``name`` (``reserve``: what to

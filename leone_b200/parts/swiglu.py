@@ -79,9 +79,11 @@ class SwiGLU(FeedForward):
         return [(2 * self.inter, self.hidden), (self.hidden, self.inter)]
 
     def scratch_bytes(self, max_tokens):
-        # the activation; a path without the fused epilogue also holds gate and up side by side
-        return max_tokens * 3 * self.inter * self.rt.dtype.itemsize + self.rt.token_scratch_bytes(max_tokens, self.hidden) + \
-            self.rt.token_scratch_bytes(max_tokens, self.inter)
+        # the activation; a path without the fused epilogue also holds gate and up side by side (with matrices in 8 bits a workspace)
+        rt = self.rt
+        beside = 2 * rt.captured_tokens(max_tokens) * self.inter if rt.weight_bits == 8 else 0
+        return (max_tokens * 3 * self.inter + beside) * rt.dtype.itemsize + rt.token_scratch_bytes(max_tokens, self.hidden) + \
+            rt.token_scratch_bytes(max_tokens, self.inter)
 
     def load_transient_bytes(self):
         return 2 * self.inter * self.hidden * self.rt.dtype.itemsize       # gate and up beside their interleaved copy
