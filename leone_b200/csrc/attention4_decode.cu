@@ -9,8 +9,9 @@
 //
 // A code becomes a bfloat16 by one AND: as a bit pattern the integers 0 .. 255 are the numbers n 2^-133 (the subnormal ones and those of
 // the smallest exponent have one step), so of a word a code in bits 0-3 is c 2^-133, one in bits 4-7 is 16 c 2^-133.  Queries
-// and weights are multiplied by 2^48 before (the queries that meet bits 4-7 by 2^44), so that the sums lie in the middle of fp32's range,
-// and the sums by 2^85 after; both are exact while queries stay below 2^79 and scales below 2^40.  (128 + c by AND-OR, which needs
+// are multiplied by 2^48 before (those that meet bits 4-7 by 2^44) and weights by 2^62, so that the sums lie in the middle of fp32's range,
+// and the sums by 2^85 and 2^71 after; all are exact while queries stay below 2^79, scales of keys below 2^40 and scales of values between 2^-62
+// and 2^57.  (128 + c by AND-OR, which needs
 // a shift for every code but a word's first and the 128 taken out again, took 425 instructions for 16 keys of 128 where this takes 296.)
 //
 // Keys ride the MMA's M side and up to 8 query heads its N side (NT tiles of them), as in attention_tiled.cu.  The pages' layout is
@@ -82,6 +83,8 @@ constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;           // codes a
 constexpr uint32_t kMinus8 = 0x80088008u;                              // -8 2^-133, twice
 constexpr float kUp = 281474976710656.f;                              // 2^48
 constexpr float kBack = 38685626227668133590597632.f;                 // 2^85
+constexpr float kWeightUp = 4611686018427387904.f;                    // 2^62 (times weights of up to 2^8 and a scale of 2^57: a bfloat16)
+constexpr float kWeightBack = 2361183241434822606848.f;               // 2^71
 // Two bfloat16 times 2^48 and, where the word's codes of bits 4-7 meet them, times 2^44.
 __device__ __forceinline__ uint32_t raised(uint32_t q, float by) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(q << 16) * by, __uint_as_float(q & 0xffff0000u) * by);
@@ -219,7 +222,7 @@ struct Warp4 {
     for (int g = 0; g < G; ++g) {
       const float s0 = scale_of(q0[g]), s1 = scale_of(q1[g]);
       const float z0 = fmaf(8.f, s0, offset_of(q0[g])), z1 = fmaf(8.f, s1, offset_of(q1[g]));
-      const float r0 = s0 * kUp, r1 = s1 * kUp;
+      const float r0 = s0 * kWeightUp, r1 = s1 * kWeightUp;
       uint32_t b[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -351,11 +354,12 @@ struct Warp4 {
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const float c = fmaf(psum[g][nt][h], kBack, over_rows(corr[g][nt][h]));
+          const float c = fmaf(psum[g][nt][h], kWeightBack, over_rows(corr[g][nt][h]));
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             *reinterpret_cast<float2*>(mo + (size_t)r * D + 64 * g + 8 * gid + 2 * j) =
-                make_float2(fmaf(o[g][j][nt][h], j & 1 ? kBack / 16 : kBack, c), fmaf(o[g][j][nt][2 + h], j & 1 ? kBack / 16 : kBack, c));
+                make_float2(fmaf(o[g][j][nt][h], j & 1 ? kWeightBack / 16 : kWeightBack, c),
+                            fmaf(o[g][j][nt][2 + h], j & 1 ? kWeightBack / 16 : kWeightBack, c));
         }
       }
   }

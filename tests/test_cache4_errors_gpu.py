@@ -9,7 +9,9 @@ element alike.  Sums in 32 bits are of 2^-23 and do not count.
 import pytest
 import torch
 
-from tests.test_cache4_gpu import BF16, DECODE, PROMPT, _attention_case, ops_of  # noqa: F401 (a fixture)
+from leone_b200.cache import packed
+from tests.fewer_bits import Step, attention64, quantize4, values4
+from tests.test_cache4_gpu import BF16, DECODE, DEV, PROMPT, _attention_case, _gen, ops_of  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +78,28 @@ def test_the_bounds_see_what_is_wrong():
     want, off = (_plain(q, x, v, 3 * 128 ** -0.5)[None] for x in (k, k.bfloat16().double()))
     assert not _right("prompt", off, want)
     assert _right("prompt", _plain(q, k.half().double(), v, 3 * 128 ** -0.5)[None], want)
+
+
+@pytest.mark.parametrize("power", [-60, -57, -30, 30, 52])
+@pytest.mark.parametrize("d,lens,splits", [(64, [(1, 300), (1, 40)], 1), (128, [(1, 300), (1, 700)], 1), (128, [(1, 900)], 9), (64, [(60, 300)], 1),
+                                           (128, [(60, 300)], 2)])
+def test_values_of_any_size(ops_of, d, lens, splits, power):  # noqa: F811
+    """Values of 2^-60 to 2^52, whose scales are an eighth of them and more: the error in relation to the output is the same."""
+    ops = ops_of(BF16)
+    step = Step(lens, 16, DEV, seed=1)
+    pools, plain = [], []
+    for values, size in ((False, 1.0), (True, 2.0 ** power)):
+        coded = quantize4(torch.randn((step.pages, 2, 16, d), generator=_gen(3 + values), device=DEV).double() * size)
+        pools.append(packed.pack_pages(*coded, values))
+        plain.append(values4(*coded))
+    n = step.ctx.n_tokens
+    qkv = torch.randn((n, 8 * d), generator=_gen(9), device=DEV).to(BF16)
+    out = torch.zeros((n, 4 * d), dtype=BF16, device=DEV)
+    ops.force_decode4_splits = ops.force_prompt4_splits = splits
+    try:
+        ops.attention(step.ctx, qkv, out, 4, 2, d, d ** -0.5, None, step.view(*pools))
+    finally:
+        ops.force_decode4_splits = ops.force_prompt4_splits = 0
+    want, *_ = attention64(qkv[:, :4 * d].double().unflatten(1, (4, d)), *plain, lens, step.table, 16, d ** -0.5, 0)
+    out = out.double().view_as(want)
+    assert _right("prompt" if n > len(lens) else "decode", out * 2.0 ** -power, want * 2.0 ** -power), _errors(out, want)
