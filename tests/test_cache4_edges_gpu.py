@@ -207,3 +207,89 @@ def test_append_of_keys_that_are_nearly_equal(ops_of, dtype, d, n_kv, tokens, sp
     assert torch.equal(have[1].double(), s) and torch.equal(have[2].double(), z)
     assert torch.equal(have[0].long(), codes)
     assert (s.amax() < 2 * spread) and len(codes.unique()) >= 8 and step.ctx.status.tolist() == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("dtype,d,n_q,n_kv", [(BF16, 128, 32, 8), (FP32, 128, 4, 8), (BF16, 96, 16, 8)])
+def test_pages_behind_4_gib(ops_of, dtype, d, n_q, n_kv):
+    """Pools of more than 2^32 bytes: append, read, decode rows and portions on their last pages, bit for bit as in small pools."""
+    ops = ops_of(dtype)
+    n_q = max(n_q, n_kv)
+    lens = [(1, 300), (1, 20), (70, 200)]
+    step = Step(lens, 16, DEV, seed=4)
+    pages = (1 << 32) // (n_kv * 16 * packed.row_bytes(d)) + 1 + step.pages
+    far = Step(lens, 16, DEV, seed=4)
+    far.table = torch.where(step.table >= 0, step.table + (pages - step.pages), step.table)
+    small = [packed.pack_pages(*quantize4(torch.randn((step.pages, n_kv, 16, d), generator=_gen(i), device=DEV).double()), bool(i)) for i in range(2)]
+    large = [torch.zeros((pages, *t.shape[1:]), dtype=torch.uint8, device=DEV) for t in small]
+    assert large[0].numel() > 1 << 32
+    for a, b in zip(large, small):
+        a[-step.pages:] = b
+    n = step.ctx.n_tokens
+    rows = torch.randn((n, (n_q + 2 * n_kv) * d), generator=_gen(9), device=DEV).to(dtype)
+    table = build_rotary_table(400, d, 10000.0).to(DEV)
+    results = []
+    for s, pools in ((step, small), (far, large)):
+        qkv, view = rows.clone(), s.view(*pools)
+        ops.qk_norm_rope_write(s.ctx, qkv, n_q, n_kv, d, None, None, 1e-6, table, d, view)
+        held = torch.zeros((2, n, n_kv * d), dtype=dtype, device=DEV)
+        ops.read_packed_rows(s.ctx, view, n_kv, d, *held)
+        out = torch.zeros((n, n_q * d), dtype=dtype, device=DEV)
+        ops.attention(s.ctx, qkv, out, n_q, n_kv, d, d ** -0.5, None, view)
+        assert s.ctx.status.tolist() == [0, 0, 0, 0]
+        results.append((qkv, held, out, *(p[-step.pages:] for p in pools)))
+    for a, b in zip(*results):
+        assert torch.equal(a, b) and a.any()
+    assert not large[0][:1000].any() and not large[1][:1000].any()
+
+
+@pytest.mark.parametrize("splits", [1, 4, 8, 33])
+@pytest.mark.parametrize("d,window", [(64, 0), (128, 0), (128, 20)])
+def test_decode_rows_without_a_key(ops_of, d, window, splits):
+    """Rows of a step that stand for no sequence (no keys, no pages) become zeros and report nothing; the others are as they were."""
+    ops = ops_of(BF16)
+    n_q, n_kv, lens = 6, 2, [(1, 200), (1, 10), (1, 90), (1, 33)]
+    step = Step(lens, 16, DEV, seed=2, window=window)
+    pools = [packed.pack_pages(*quantize4(torch.randn((step.pages, n_kv, 16, d), generator=_gen(i), device=DEV).double()), bool(i)) for i in range(2)]
+    qkv = torch.randn((4, (n_q + 2 * n_kv) * d), generator=_gen(5), device=DEV).to(BF16)
+    outs = []
+    ops.force_decode4_splits = splits
+    try:
+        for empty in ((), (1, 3)):
+            for i in empty:
+                step.ctx.ctx_len[i], step.table[i] = 0, -1
+            out = torch.full((4, n_q * d), 7.0, dtype=BF16, device=DEV)
+            ops.attention(step.ctx, qkv, out, n_q, n_kv, d, d ** -0.5, window or None, step.view(*pools))
+            outs.append(out)
+    finally:
+        ops.force_decode4_splits = 0
+    assert torch.equal(outs[0][::2], outs[1][::2]) and not outs[1][1::2].any() and outs[0][1::2].any()
+    assert step.ctx.status.tolist() == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (BF16, 128), (FP32, 64)])
+def test_sequences_without_a_token(ops_of, dtype, d):
+    """Sequences that bring no token to a step of portions: the others' outputs are as without them."""
+    ops = ops_of(dtype)
+    n_q, n_kv = 4, 2
+    results = []
+    for lens in ([(40, 100), (3, 20)], [(40, 100), (0, 60), (3, 20), (0, 5)]):
+        step = Step(lens, 16, DEV, seed=3)
+        # the same pages' contents for the same sequences, by their place in the table
+        whole = [torch.randn((2, 12, n_kv, 16, d), generator=_gen(7 + i), device=DEV).double() for i in range(2)]
+        pools = []
+        for values, x in zip((False, True), whole):
+            t = torch.zeros((step.pages, n_kv, 16, d), dtype=torch.float64, device=DEV)
+            for which, seq in enumerate([i for i, (new, _) in enumerate(lens) if new]):
+                pages = step.table[seq][step.table[seq] >= 0].long()
+                t[pages] = x[which, :len(pages)]
+            pools.append(packed.pack_pages(*quantize4(t), values))
+        qkv = torch.randn((43, (n_q + 2 * n_kv) * d), generator=_gen(5), device=DEV).to(dtype)
+        out = torch.full((43, n_q * d), 7.0, dtype=dtype, device=DEV)
+        ops.force_prompt4_splits = ops.force_any4_splits = 1
+        try:
+            ops.attention(step.ctx, qkv, out, n_q, n_kv, d, d ** -0.5, None, step.view(*pools))
+        finally:
+            ops.force_prompt4_splits = ops.force_any4_splits = 0
+        assert step.ctx.status.tolist() == [0, 0, 0, 0]
+        results.append(out)
+    assert torch.equal(*results) and not (results[0] == 7.0).all()

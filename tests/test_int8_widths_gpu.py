@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from leone_b200.ops.int8 import NARROW, PAIRS, Int8Products
+from leone_b200.ops.int8 import MAX_K, NARROW, PAIRS, Int8Products
 from tests.test_int8_gpu import BF16, DEV, _check, _gen, _inputs, _want, ops_of  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +63,21 @@ def test_rows_that_are_one(ops_of, m, n, k):  # noqa: F811
         ops.linear(rows, w, out)
         want = _want(rows, codes, scales)
         _check(out, want, want * 0, BF16)
+
+
+@pytest.mark.parametrize("m", [1, 40, 200])
+def test_the_largest_sums(ops_of, m):  # noqa: F811
+    """The widest matrix that is taken, all codes 127: sums of 2.11e9 stay in 32 bits, in every form."""
+    ops = ops_of(BF16)
+    k, n = MAX_K, 96
+    x = torch.full((m, k), 2.0, dtype=BF16, device=DEV)
+    x[:, 1::2] *= torch.where(torch.arange(m, device=DEV) % 2 == 0, 1.0, -1.0).to(BF16)[:, None]         # (odd rows: 0)
+    codes = torch.full((n, k), 127, dtype=torch.int8, device=DEV)
+    codes[1] = -127
+    w = ops.prepare_matrix_int8(codes, torch.ones(n, device=DEV))
+    out = torch.full((m, n), 9.0, device=DEV)
+    ops.linear(x, w, out)
+    want = torch.full((m, n), 127.0 * k * 2.0, dtype=torch.float64, device=DEV)
+    want[:, 1] *= -1
+    want[1::2] = 0
+    assert ((out.double() - want).abs() <= want.abs() * 4 * 2.0 ** -24).all()
