@@ -81,3 +81,33 @@ def test_the_largest_sums(ops_of, m):  # noqa: F811
     want[:, 1] *= -1
     want[1::2] = 0
     assert ((out.double() - want).abs() <= want.abs() * 4 * 2.0 ** -24).all()
+
+
+@pytest.mark.parametrize("m", [5, 60, 200])
+@pytest.mark.parametrize("n", [96, 100, 33])
+def test_strided_rows_in_every_form(ops_of, m, n):  # noqa: F811
+    """Tokens, outputs and residuals that are columns of wider rows, on odd elements: as the same without gaps, and nothing beside them."""
+    ops = ops_of(BF16)
+    k = 208
+    x, codes, scales = _inputs(m, n, k, BF16, 2)
+    w = ops.prepare_matrix_int8(codes, scales, torch.randn(n, generator=_gen(1), device=DEV))
+    rows = torch.randn((m, k + 31), generator=_gen(2), device=DEV).to(BF16)
+    rows[:, 7:7 + k] = x
+    for dtype, residual in ((BF16, False), (torch.float32, False), (torch.float32, True)):
+        start = torch.randn((m, n), generator=_gen(3), device=DEV).to(dtype)
+        plain, wide = start.clone(), torch.full((m, n + 31), 5.0, dtype=dtype, device=DEV)
+        wide[:, 3:3 + n] = start
+        into = wide[:, 3:3 + n]
+        ops.linear(x, w, plain, residual=plain if residual else None)
+        ops.linear(rows[:, 7:7 + k], w, into, residual=into if residual else None)
+        assert torch.equal(into, plain)
+        assert (wide[:, :3] == 5).all() and (wide[:, 3 + n:] == 5).all()
+        want = _want(x, codes, scales) + w.bias.double() + (start.double() if residual else 0)
+        _check(plain, want, w.bias.double().abs() + start.double().abs(), dtype)
+    if n == 96:
+        gate = ops.prepare_gate_up_int8(codes[:48], scales[:48], codes[48:], scales[48:])
+        plain = torch.empty((m, 48), dtype=BF16, device=DEV)
+        ops.linear_swiglu(x, gate, plain)
+        flat = torch.full((m * 48 + 9,), 5.0, dtype=BF16, device=DEV)
+        ops.linear_swiglu(rows[:, 7:7 + k], gate, flat[3:-6].view(m, 48))
+        assert torch.equal(flat[3:-6].view(m, 48), plain) and (flat[:3] == 5).all() and (flat[-6:] == 5).all()
