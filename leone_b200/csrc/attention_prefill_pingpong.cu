@@ -210,7 +210,9 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 // that turn keys are what the time depends on: with the tile's largest value sought by every thread in all its rows, where the
 // four threads of a row now take one each, it was 353 us, 320 as it is.
 //
-// Values become bfloat16, and so do the weights, as in the other forms.  Keys become fp16, and queries are fp16 too, which is exact:
+// Values become bfloat16, and so do the weights, as in the other forms: with the output's own rounding (0.0017 of its norm) 0.0026.  fp16 would
+// spare most of that, but asks for a power of two that a tile's values share, by which the running sums had to be moved whenever it
+// changes, and bfloat16 takes values of any size side by side.  Keys become fp16, and queries are fp16 too, which is exact:
 // z + s c has 12 significant bits and more, and rounded to the 8 of bfloat16 its error in the scores was most of the output's (8,192
 // keys with a spread of scores of 3: 0.0075 of the output's norm, 0.0026 with the 11 of fp16).  For fp16's range a query's row is
 // multiplied by a power of two that brings its largest element to 2^7 .. 2^8, and a tile of keys by one that brings its largest value
